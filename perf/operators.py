@@ -133,8 +133,9 @@ def _inputs(case, seed):
         used = int(have.sum())
         table = torch.full((R, cols), -1, dtype=torch.int32)
         table[torch.arange(cols)[None, :] < have[:, None]] = ids[:used].to(torch.int32)
-        free = ids[used:].to(torch.int32)
-        count = int(len(free) * case["spare"])
+        free = torch.full((pages,), -1, dtype=torch.int32)        # a stack with room for every page
+        free[:pages - used] = ids[used:].to(torch.int32)
+        count = int((pages - used) * case["spare"])
         tokens = (int(new.sum()) + 15) // 16 * 16
         return dict(past=past.to(torch.int32).cuda(), new=new.to(torch.int32).cuda(), table=table.cuda(), free=free.cuda(),
                     count=_i32([count]), tokens=tokens, pages=pages, cols=cols)
