@@ -47,6 +47,28 @@ class HkvExchange(C.Structure):
     ]
 
 
+class HkvPagedGeometry(C.Structure):
+    """Mirror of `struct hkv_paged_geometry` (include/hkv.h)."""
+    _fields_ = [(n, C.c_int32) for n in (
+        "dtype", "num_heads", "num_kv_heads", "head_dim", "page_size", "num_pages", "max_requests", "max_pages",
+        "max_tokens", "window_size", "kernel_select", "flags")] + [("reserved", C.c_int32 * 4)]
+
+
+ROPE_MAX_AXES = 4
+PAGED_MAX_REQUESTS = 4096
+
+
+class HkvPagedRope(C.Structure):
+    """Mirror of `struct hkv_paged_rope` (include/hkv.h)."""
+    _fields_ = [(n, C.c_void_p) for n in (
+        "q", "k", "v", "q_out", "k_out", "q_norm_w", "k_norm_w", "k_cache", "v_cache", "d_slots", "d_positions")] + [
+        (n, C.c_int64) for n in ("q_token_stride", "kv_token_stride", "q_out_token_stride", "k_out_token_stride",
+                                 "position_axis_stride")] + [
+        ("tokens", C.c_int32), ("rotary_dim", C.c_int32), ("axes", C.c_int32), ("sections", C.c_int32 * ROPE_MAX_AXES),
+        ("interleaved", C.c_int32), ("eps", C.c_float), ("scaling_factor", C.c_float), ("theta", C.c_double),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/hkv.h declares
 _VP, _I32P, _F32P = C.c_void_p, C.c_void_p, C.c_void_p
 SIGNATURES = {
@@ -87,6 +109,17 @@ SIGNATURES = {
     "hkv_plan_sequence": (C.c_int, [C.POINTER(HkvGeometry), C.c_int32, C.c_int32] + [C.POINTER(C.c_int32)] * 4),
     "hkv_plan_prefill": (C.c_int, [C.POINTER(HkvGeometry), C.c_int32, C.c_int32, C.c_int32] + [C.POINTER(C.c_int32)] * 4),
     "hkv_preferred_prefill_chunk": (C.c_int32, [C.POINTER(HkvGeometry), C.c_int32, C.c_int32]),
+    "hkv_paged_create": (C.c_int, [C.POINTER(C.c_void_p), C.POINTER(HkvPagedGeometry)]),
+    "hkv_paged_destroy": (C.c_int, [_VP]),
+    "hkv_paged_last_error": (C.c_char_p, [_VP]),
+    "hkv_paged_device_status": (C.c_int, [_VP, _VP, C.POINTER(C.c_int32)]),
+    "hkv_paged_workspace_bytes": (C.c_size_t, [_VP]),
+    "hkv_paged_plan": (C.c_int, [_VP, C.c_int32, C.c_int32] + [_I32P] * 11 + [_VP]),
+    "hkv_paged_release": (C.c_int, [_VP, C.c_int32] + [_I32P] * 5 + [_VP]),
+    "hkv_paged_append": (C.c_int, [_VP, _VP, _VP, C.c_int64, _VP, _VP, _I32P, C.c_int32, _VP]),
+    "hkv_paged_norm_rope": (C.c_int, [_VP, C.POINTER(HkvPagedRope), _VP]),
+    "hkv_paged_attention": (C.c_int, [_VP, _VP, C.c_int64, _VP, _VP, _VP] + [_I32P] * 4 + [C.c_int32] * 3 + [C.c_float, _VP]),
+    "hkv_paged_cross_attention": (C.c_int, [_VP, _VP, C.c_int64, _VP, _VP, _VP] + [_I32P] * 4 + [C.c_int32] * 3 + [C.c_float, _VP]),
     "hkv_fill_synthetic": (C.c_int, [_VP, C.c_uint64, C.c_uint64, C.c_uint64, _VP]),
 }
 

@@ -28,6 +28,7 @@ WATCH_TESTS = os.path.join(REPO, "tests", "cpp", "hkv_watch_tests")
 SEQSPLIT_TESTS = os.path.join(REPO, "tests", "cpp", "hkv_seqsplit_tests")
 GEMMA4_TESTS = os.path.join(REPO, "tests", "cpp", "hkv_gemma4_tests")
 
+LIB_SOURCES = ["hkv_api.cu", "hkv_paged_api.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC"]
 
@@ -59,10 +60,16 @@ def build_lib(force: bool = False, verbose: bool = False) -> str:
     srcs = _sources(CSRC)
     if not force and _newer(LIB, srcs):
         return LIB
-    cmd = [_nvcc(), *ARCH, *NVCC_FLAGS, "-shared", "-o", LIB, os.path.join(CSRC, "hkv_api.cu")]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-    subprocess.run(cmd, check=True)
+    objs, running = [], []
+    for name in LIB_SOURCES:   # one compiler process per translation unit, side by side
+        objs.append(os.path.join(CSRC, name[:-3] + ".o"))
+        cmd = [_nvcc(), *ARCH, *NVCC_FLAGS, *(["-Xptxas=-v"] if verbose else []), "-c", "-o", objs[-1], os.path.join(CSRC, name)]
+        running.append((cmd, subprocess.Popen(cmd)))
+    done = [(cmd, p.wait()) for cmd, p in running]
+    for cmd, rc in done:
+        if rc != 0:
+            raise subprocess.CalledProcessError(rc, cmd)
+    subprocess.run([_nvcc(), *ARCH, "-shared", "-Xcompiler", "-fPIC", "-o", LIB, *objs], check=True)
     return LIB
 
 

@@ -1,0 +1,417 @@
+// hkv_paged.cuh — what the kernels of the paged cache share: element types, the packed batch as the kernels see it,
+// and the kernels around attention: block tables and slot maps, release, append, any-geometry attention.
+#pragma once
+
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "hkv_common.cuh"
+
+namespace hkv {
+
+// ---- element types --------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T> __device__ __forceinline__ T from_f32(float x);
+template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+// Two values rounded to nearest and packed, the first in the low half.
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) { return pack_half2(lo, hi); }
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w);
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));   // bf16 is the upper half of fp32
+}
+
+// ---- the packed batch -----------------------------------------------------------------------------------------------
+struct PagedBatch {
+    const int32_t* table;     // [requests][cols]
+    const int32_t* q_start;   // [requests(+1)]
+    const int32_t* step_len;
+    const int32_t* key_len;   // positions in the cache, the new tokens included (cross attention: encoder states)
+    int32_t* status;
+    int requests, cols, page, pages;   // page = rows per page
+    int tokens, max_step;
+    int window;               // 0 = none
+    int causal;               // 0: every query attends [0, key_len)
+};
+
+// One request, with every value that comes from device memory brought into the range the buffers allow: no array
+// content can lead an access out of bounds.
+struct PagedRequest {
+    int start, n;      // packed rows of its queries
+    int pos0;          // position of query 0 (causal); may be negative: such queries attend nothing
+    int keys;          // positions held, at most cols * page
+};
+__device__ __forceinline__ PagedRequest paged_request(const PagedBatch& a, int r) {
+    PagedRequest q;
+    q.start = a.q_start[r];
+    const int step = a.step_len[r], len = a.key_len[r];
+    q.n = step < a.max_step ? step : a.max_step;
+    if (q.start < 0 || q.start > a.tokens) q.n = 0;
+    else if (q.n > a.tokens - q.start) q.n = a.tokens - q.start;
+    if (q.n < 0) q.n = 0;
+    const int cap = a.cols * a.page;
+    q.keys = len < cap ? (len > 0 ? len : 0) : cap;
+    q.pos0 = (len > 0 ? len : 0) - (step > 0 ? step : 0);
+    return q;
+}
+// Keys [lo, hi) that query i of a request attends; hi <= lo: none.
+__device__ __forceinline__ void paged_key_range(const PagedBatch& a, const PagedRequest& q, int i, int& lo, int& hi) {
+    lo = 0;
+    hi = q.keys;
+    if (a.causal) {
+        const int p = q.pos0 + i;
+        if (p + 1 < hi) hi = p + 1;
+        if (a.window > 0 && p + 1 - a.window > 0) lo = p + 1 - a.window;
+    }
+}
+
+// ---- scans of a block -----------------------------------------------------------------------------------------------
+// Exclusive prefix sum of one value per thread over the block (at most 1024 threads); `total` gets the sum.
+// `buf` holds 33 values; ends with the block synchronised.
+__device__ __forceinline__ long long block_scan(long long v, long long* buf, long long& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = (blockDim.x + 31) >> 5;
+    long long x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += u;
+    }
+    if (lane == 31) buf[warp] = x;
+    __syncthreads();
+    if (warp == 0) {
+        long long s = lane < warps ? buf[lane] : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xffffffffu, s, o);
+            if (lane >= o) s += u;
+        }
+        buf[lane] = s;
+    }
+    __syncthreads();
+    const long long before = warp > 0 ? buf[warp - 1] : 0;
+    total = buf[warps - 1];
+    __syncthreads();
+    return before + x - v;
+}
+
+// ---- plan -----------------------------------------------------------------------------------------------------------
+// One thread-block cluster of up to 8 CTAs x 1024 threads. Every CTA scans all requests itself (at most four per
+// thread: cheaper than passing sums between CTAs) and leaves their starts, lengths and places on the free stack in
+// shared memory; after the cluster barrier — every CTA has read the state that the launch may update in place — each
+// CTA writes its share of the tables. A token finds its request by bisection over the starts in shared memory. New
+// block-table entries come from the free stack directly, so no CTA waits for another's table writes.
+// Bound: launch latency and two dependent trips to memory (lengths, then table or stack entries); the tables
+// themselves are some hundred KB at most.
+struct PlanArgs {
+    const int32_t *past, *fresh, *free_pages, *free_count;
+    int32_t *table, *total, *step, *q_start, *slots, *positions, *free_left;
+    int requests, tokens, cols, page, pages;
+};
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanMaxCluster = 8;
+constexpr int kPagedMaxRequests = 4096;
+constexpr int kPlanPer = kPagedMaxRequests / kPlanThreads;   // requests per thread
+__host__ __device__ constexpr size_t plan_smem_bytes(int requests) { return (size_t)(3 * requests + 4) * 4; }
+
+__global__ void __launch_bounds__(kPlanThreads, 1) hkv_paged_plan_kernel(const PlanArgs a) {
+    namespace cg = cooperative_groups;
+    extern __shared__ int32_t plan_smem[];
+    __shared__ long long buf[33];
+    int32_t* s_start = plan_smem;                    // [R + 1]
+    int32_t* s_past = s_start + a.requests + 1;      // [R]
+    int32_t* s_take = s_past + a.requests;           // [R] pages taken off the stack before this request, -1: not admitted
+    const int R = a.requests, tid = threadIdx.x;
+    const int per = (R + kPlanThreads - 1) / kPlanThreads;
+    const int r0 = tid * per;
+    int past[kPlanPer], fresh[kPlanPer];
+    long long sum = 0;
+#pragma unroll
+    for (int i = 0; i < kPlanPer; ++i) {
+        past[i] = fresh[i] = 0;
+        if (i < per && r0 + i < R) {
+            past[i] = a.past[r0 + i];
+            fresh[i] = a.fresh[r0 + i];
+            sum += fresh[i] > 0 ? fresh[i] : 0;
+        }
+    }
+    const int count = *a.free_count, avail = count < a.pages ? count : a.pages;
+    long long tokens_all, need_all;
+    long long at = block_scan(sum, buf, tokens_all);
+    long long need[kPlanPer], need_sum = 0;
+#pragma unroll
+    for (int i = 0; i < kPlanPer; ++i) {
+        need[i] = -1;                                // not admitted
+        if (i < per && r0 + i < R) {
+            s_start[r0 + i] = (int)(at < a.tokens ? at : a.tokens);
+            s_past[r0 + i] = past[i];
+            const long long end = at + (fresh[i] > 0 ? fresh[i] : 0);
+            const long long len = (long long)past[i] + fresh[i];
+            if (past[i] >= 0 && fresh[i] >= 0 && len <= (long long)a.cols * a.page && end <= a.tokens) {
+                need[i] = (len + a.page - 1) / a.page - ((long long)past[i] + a.page - 1) / a.page;
+                need_sum += need[i];
+            }
+            at = end;
+        }
+    }
+    if (tid == 0) s_start[R] = (int)(tokens_all < a.tokens ? tokens_all : a.tokens);
+    long long before = block_scan(need_sum, buf, need_all);
+    long long taken = 0;                             // of this thread's admitted requests
+#pragma unroll
+    for (int i = 0; i < kPlanPer; ++i) {
+        if (i < per && r0 + i < R) {
+            const bool ok = need[i] == 0 || (need[i] > 0 && before + need[i] <= avail);
+            s_take[r0 + i] = ok ? (int)before : -1;
+            if (need[i] > 0) {
+                if (ok) taken += need[i];
+                before += need[i];
+            }
+        }
+    }
+    // `before` of a request that needs no page may exceed `avail`; it takes none, so its value is only a mark
+    long long taken_all;
+    block_scan(taken, buf, taken_all);               // (also orders the shared-memory tables)
+
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
+    cluster.sync();                                  // past, new and the count are read everywhere: state may change
+
+    auto new_len = [&](int r) { return s_take[r] >= 0 ? a.fresh[r] : 0; };
+    // per-request outputs and new block-table entries
+    for (int r = rank * kPlanThreads + tid; r < R; r += ctas * kPlanThreads) {
+        const int n = new_len(r), p = s_past[r];
+        a.q_start[r] = s_start[r];
+        a.step[r] = n;
+        a.total[r] = p + n;
+        if (n > 0) {
+            const int j0 = (p + a.page - 1) / a.page, j1 = (p + n + a.page - 1) / a.page;
+            const int top = avail - 1 - s_take[r];   // stack entry of the request's first new page
+            if (j1 - j0 <= 32)
+                for (int j = j0; j < j1; ++j) a.table[(long long)r * a.cols + j] = a.free_pages[top - (j - j0)];
+        }
+    }
+    if (rank == 0 && tid == 0) {
+        a.q_start[R] = s_start[R];
+        *a.free_left = (int)(avail - taken_all);
+    }
+    // requests that open many pages: a warp each
+    const int warp = tid >> 5, lane = tid & 31;
+    for (int r = rank * 32 + warp; r < R; r += ctas * 32) {
+        const int n = new_len(r), p = s_past[r];
+        if (n <= 0) continue;
+        const int j0 = (p + a.page - 1) / a.page, j1 = (p + n + a.page - 1) / a.page;
+        if (j1 - j0 <= 32) continue;
+        const int top = avail - 1 - s_take[r];
+        for (int j = j0 + lane; j < j1; j += 32) a.table[(long long)r * a.cols + j] = a.free_pages[top - (j - j0)];
+    }
+    // slot and position of every packed token
+    for (int t = rank * kPlanThreads + tid; t < a.tokens; t += ctas * kPlanThreads) {
+        int slot = -1, pos = -1;
+        if (t < s_start[R]) {
+            int lo = 0, hi = R - 1;                  // the last request that starts at or before t
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (s_start[mid] <= t) lo = mid; else hi = mid - 1;
+            }
+            if (s_take[lo] >= 0) {
+                const int p = s_past[lo], j0 = (p + a.page - 1) / a.page;
+                pos = p + t - s_start[lo];
+                const int j = pos / a.page;
+                const int pg = j < j0 ? a.table[(long long)lo * a.cols + j] : a.free_pages[avail - 1 - s_take[lo] - (j - j0)];
+                slot = pg >= 0 && pg < a.pages ? pg * a.page + pos % a.page : -1;
+            }
+        }
+        a.slots[t] = slot;
+        a.positions[t] = pos;
+    }
+}
+
+// ---- release --------------------------------------------------------------------------------------------------------
+struct ReleaseArgs {
+    const int32_t *finished, *table;
+    int32_t *seq_len, *free_pages, *free_count;
+    int requests, cols, page, pages;
+};
+__global__ void __launch_bounds__(kPlanThreads, 1) hkv_paged_release_kernel(const ReleaseArgs a) {
+    extern __shared__ int32_t rel_smem[];            // [R] first place on the stack, [R] pages
+    __shared__ long long buf[33];
+    const int R = a.requests, tid = threadIdx.x;
+    const int per = (R + kPlanThreads - 1) / kPlanThreads;
+    const int r0 = tid * per;
+    int n[kPlanPer];
+    long long sum = 0;
+#pragma unroll
+    for (int i = 0; i < kPlanPer; ++i) {
+        n[i] = 0;
+        if (i < per && r0 + i < R && a.finished[r0 + i]) {
+            const int len = a.seq_len[r0 + i];
+            const int held = len > 0 ? (int)(((long long)len + a.page - 1) / a.page) : 0;
+            n[i] = held < a.cols ? held : a.cols;
+            a.seq_len[r0 + i] = 0;                   // this thread alone reads and writes it
+        }
+        sum += n[i];
+    }
+    const int count = *a.free_count, have = count > 0 ? (count < a.pages ? count : a.pages) : 0;
+    long long all;
+    long long at = block_scan(sum, buf, all);
+#pragma unroll
+    for (int i = 0; i < kPlanPer; ++i)
+        if (i < per && r0 + i < R) {
+            rel_smem[r0 + i] = (int)at;
+            rel_smem[R + r0 + i] = n[i];
+            at += n[i];
+        }
+    __syncthreads();
+    const int warp = tid >> 5, lane = tid & 31;
+    for (int r = warp; r < R; r += kPlanThreads / 32)
+        for (int j = lane; j < rel_smem[R + r]; j += 32) {
+            const long long to = (long long)have + rel_smem[r] + j;
+            if (to < a.pages) a.free_pages[to] = a.table[(long long)r * a.cols + j];
+        }
+    if (tid == 0) {
+        const long long now = have + all;
+        *a.free_count = (int)(now < a.pages ? now : a.pages);
+    }
+}
+
+// ---- append ---------------------------------------------------------------------------------------------------------
+// A warp per token: its K row and its V row are one list of pieces dealt to the lanes, four loads in flight per lane.
+// Bound: HBM (each row read once, written once).
+struct PagedAppendArgs {
+    const void *k, *v;
+    void *k_cache, *v_cache;
+    const int32_t* slots;
+    int32_t* status;
+    long long stride;      // elements between tokens
+    long long rows;        // pages * page
+    int tokens, row_elems;
+};
+template <typename VecT>
+__global__ void __launch_bounds__(256) hkv_paged_append_kernel(const PagedAppendArgs a) {
+    constexpr int kPer = (int)(sizeof(VecT) / 2);
+    const int lane = threadIdx.x & 31, pieces = a.row_elems / kPer;
+    for (long long t = (blockIdx.x * 256ll + threadIdx.x) >> 5; t < a.tokens; t += gridDim.x * 8ll) {
+        const int slot = a.slots[t];
+        if (slot < 0) continue;
+        if (slot >= a.rows) {
+            if (lane == 0) atomicOr(a.status, kStatusBoundCheck);
+            continue;
+        }
+        const VecT* src[2] = {reinterpret_cast<const VecT*>((const uint16_t*)a.k + t * a.stride),
+                              reinterpret_cast<const VecT*>((const uint16_t*)a.v + t * a.stride)};
+        VecT* dst[2] = {reinterpret_cast<VecT*>((uint16_t*)a.k_cache + (long long)slot * a.row_elems),
+                        reinterpret_cast<VecT*>((uint16_t*)a.v_cache + (long long)slot * a.row_elems)};
+        for (int p0 = lane; p0 < 2 * pieces; p0 += 128) {
+            VecT x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int p = p0 + 32 * u;
+                if (p < 2 * pieces) x[u] = p < pieces ? src[0][p] : src[1][p - pieces];
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int p = p0 + 32 * u;
+                if (p < pieces) dst[0][p] = x[u];
+                else if (p < 2 * pieces) dst[1][p - pieces] = x[u];
+            }
+        }
+    }
+}
+
+// ---- attention, any geometry ----------------------------------------------------------------------------------------
+// One CTA of 4 warps per (packed token, query head): warp w takes the keys lo+w, lo+w+4, ..., lanes stride the head
+// dimension, online softmax per warp in the log2 domain, the warps merged in shared memory. For what the staged kernels
+// do not take (head sizes, page sizes, alignment); every K/V row is read once per query head.
+struct PagedAttnArgs {
+    PagedBatch b;
+    const void *q, *k_cache, *v_cache;
+    void* out;
+    long long q_stride;
+    int H, KVH, HD;
+    float scale_log2;
+};
+constexpr int kPagedGenWarps = 4;
+
+template <typename T>
+__global__ void __launch_bounds__(kPagedGenWarps * 32) hkv_paged_generic_kernel(const PagedAttnArgs a) {
+    const int t = blockIdx.x, h = blockIdx.y;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int lo = 0, hi = a.b.requests - 1;               // the last request that starts at or before t
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (a.b.q_start[mid] <= t) lo = mid; else hi = mid - 1;
+    }
+    const PagedRequest rq = paged_request(a.b, lo);
+    const int i = t - rq.start;
+    if (i < 0 || i >= rq.n) return;                  // a row of no query
+    int k_lo, k_hi;
+    paged_key_range(a.b, rq, i, k_lo, k_hi);
+    const int kvh = h / (a.H / a.KVH);
+    const T* qp = (const T*)a.q + t * a.q_stride + (long long)h * a.HD;
+    float qr[16], acc[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const int d = lane + 32 * e;
+        qr[e] = d < a.HD ? to_f32(qp[d]) : 0.0f;
+        acc[e] = 0.0f;
+    }
+    float m = kNegBig, l = 0.0f;
+    const int32_t* table = a.b.table + (long long)lo * a.b.cols;
+    for (int s = k_lo + warp; s < k_hi; s += kPagedGenWarps) {
+        const int pg = table[s / a.b.page];
+        const bool in = pg >= 0 && pg < a.b.pages;   // an entry outside the planes: rows of zeros
+        if (!in && lane == 0) atomicOr(a.b.status, kStatusBoundCheck);
+        const long long row = (((long long)(in ? pg : 0) * a.b.page + s % a.b.page) * a.KVH + kvh) * a.HD;
+        const T* kr = (const T*)a.k_cache + row;
+        const T* vr = (const T*)a.v_cache + row;
+        float dot = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int d = lane + 32 * e;
+            if (in && d < a.HD) dot = fmaf(qr[e], to_f32(kr[d]), dot);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        const float sc = dot * a.scale_log2;
+        const float mn = fmaxf(m, sc);
+        const float corr = exp2f(m - mn), e2 = exp2f(sc - mn);
+        l = l * corr + e2;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int d = lane + 32 * e;
+            if (d < a.HD) acc[e] = fmaf(e2, in ? to_f32(vr[d]) : 0.0f, acc[e] * corr);
+        }
+        m = mn;
+    }
+    __shared__ float s_m[kPagedGenWarps], s_l[kPagedGenWarps];
+    __shared__ float s_acc[kPagedGenWarps][512];
+    if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s_acc[warp][lane + 32 * e] = acc[e];
+    __syncthreads();
+    float gm = s_m[0];
+#pragma unroll
+    for (int w = 1; w < kPagedGenWarps; ++w) gm = fmaxf(gm, s_m[w]);
+    float gl = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kPagedGenWarps; ++w) gl += s_l[w] * exp2f(s_m[w] - gm);
+    const float inv = gl > 0.0f ? 1.0f / gl : 0.0f;
+    T* op = (T*)a.out + ((long long)t * a.H + h) * a.HD;
+    for (int d = threadIdx.x; d < a.HD; d += kPagedGenWarps * 32) {
+        float o = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kPagedGenWarps; ++w) o += s_acc[w][d] * exp2f(s_m[w] - gm);
+        op[d] = from_f32<T>(o * inv);
+    }
+}
+
+}  // namespace hkv

@@ -1,0 +1,404 @@
+// hkv_paged_api.cu — C ABI of the paged cache (declared in include/hkv.h): argument checks, the context with its
+// workspace, dispatch. Host side only enqueues work; there is no CPU compute path.
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdio>
+#include <new>
+#include <string>
+
+#include "../../include/hkv.h"
+#include "hkv_paged.cuh"
+#include "hkv_paged_rope.cuh"
+
+using namespace hkv;
+
+struct hkv_paged_ctx {
+    hkv_paged_geometry g;
+    int device = -1;
+    int sm_count = 0;
+    int32_t* d_status = nullptr;
+    size_t workspace_bytes = 0;
+    bool ready = false;
+    std::string err;
+};
+
+namespace {
+
+int fail(hkv_paged_ctx* c, int code, const char* msg) {
+    if (c) {
+        try { c->err = msg; } catch (...) {}
+    }
+    return code;
+}
+int fail_cuda(hkv_paged_ctx* c, cudaError_t e, const char* where) {
+    char buf[256];
+    snprintf(buf, sizeof buf, "%s: %s", where, cudaGetErrorString(e));
+    return fail(c, HKV_ERR_CUDA, buf);
+}
+bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) % n) == 0; }
+
+int validate(const hkv_paged_geometry* g, const char** why) {
+    if (!g) { *why = "geometry is null"; return HKV_ERR_INVALID_ARG; }
+    if (g->dtype != HKV_DTYPE_F16 && g->dtype != HKV_DTYPE_BF16) { *why = "unknown dtype"; return HKV_ERR_INVALID_ARG; }
+    if (g->head_dim <= 0 || g->head_dim > 512 || g->num_kv_heads <= 0 || g->num_heads <= 0 ||
+        g->num_heads % g->num_kv_heads != 0 || g->num_heads > 65535) {
+        *why = "unsupported head geometry";
+        return HKV_ERR_GEOMETRY;
+    }
+    if (g->page_size <= 0 || g->num_pages <= 0 || g->max_requests <= 0 || g->max_pages <= 0 || g->max_tokens <= 0 ||
+        g->window_size < 0) {
+        *why = "page_size, num_pages, max_requests, max_pages and max_tokens must be positive, window_size non-negative";
+        return HKV_ERR_INVALID_ARG;
+    }
+    if (g->kernel_select < 0 || g->kernel_select > 2 || (g->flags & ~HKV_FLAG_APPEND_ONLY) != 0 || g->reserved[0] ||
+        g->reserved[1] || g->reserved[2] || g->reserved[3]) {
+        *why = "unknown kernel_select or flag, or a reserved field set";
+        return HKV_ERR_INVALID_ARG;
+    }
+    if (g->max_requests > HKV_PAGED_MAX_REQUESTS) { *why = "max_requests exceeds HKV_PAGED_MAX_REQUESTS"; return HKV_ERR_TOO_LARGE; }
+    if ((long long)g->num_pages * g->page_size > 0x7fffffffll || (long long)g->max_pages * g->page_size > 0x7fffffffll) {
+        *why = "num_pages * page_size and max_pages * page_size are limited to 2^31 - 1";
+        return HKV_ERR_TOO_LARGE;
+    }
+    return HKV_OK;
+}
+
+int check(hkv_paged_ctx* c) {
+    if (!c) return HKV_ERR_INVALID_ARG;
+    if (!c->ready) return fail(c, HKV_ERR_INVALID_ARG, "context not initialised");
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess) {
+        cudaGetLastError();
+        return fail(c, HKV_ERR_CUDA, "cudaGetDevice failed");
+    }
+    if (dev != c->device) {
+        char buf[96];
+        snprintf(buf, sizeof buf, "context belongs to device %d, current device is %d", c->device, dev);
+        return fail(c, HKV_ERR_INVALID_ARG, buf);
+    }
+    return HKV_OK;
+}
+#define PAGED_CHECK(c)                  \
+    do {                                \
+        const int chk_ = check(c);      \
+        if (chk_ != HKV_OK) return chk_; \
+    } while (0)
+
+int launched(hkv_paged_ctx* c, const char* what) {
+    const cudaError_t e = cudaPeekAtLastError();
+    return e == cudaSuccess ? HKV_OK : fail_cuda(c, e, what);
+}
+
+// A token stride: 0 = dense, else at least one token's row.
+bool stride_ok(int64_t given, long long row, long long* out) {
+    if (given != 0 && given < row) return false;
+    *out = given ? given : row;
+    return true;
+}
+
+int attention(hkv_paged_ctx* c, const void* q, int64_t q_token_stride, const void* k_cache,
+              const void* v_cache, void* out, const int32_t* d_block_table, const int32_t* d_q_start,
+              const int32_t* d_step_len, const int32_t* d_key_len, int32_t requests, int32_t tokens, int32_t max_step,
+              float scale, void* stream, bool causal) {
+    PAGED_CHECK(c);
+    const hkv_paged_geometry& g = c->g;
+    if (g.flags & HKV_FLAG_APPEND_ONLY) return fail(c, HKV_ERR_WORKSPACE, "attention: the context was created append-only");
+    if (!q || !k_cache || !v_cache || !out || !d_block_table || !d_q_start || !d_step_len || !d_key_len)
+        return fail(c, HKV_ERR_INVALID_ARG, "attention: null argument");
+    if (requests < 0 || tokens < 0 || max_step < 0) return fail(c, HKV_ERR_INVALID_ARG, "attention: negative count");
+    if (requests > g.max_requests || tokens > g.max_tokens)
+        return fail(c, HKV_ERR_TOO_LARGE, "attention: more requests or tokens than the context was created for");
+    if (!std::isfinite(scale)) return fail(c, HKV_ERR_INVALID_ARG, "attention: scale is not finite");
+    PagedAttnArgs a{};
+    if (!stride_ok(q_token_stride, (long long)g.num_heads * g.head_dim, &a.q_stride))
+        return fail(c, HKV_ERR_INVALID_ARG, "attention: q_token_stride smaller than one token's row");
+    if (!aligned(q, 2) || !aligned(k_cache, 2) || !aligned(v_cache, 2) || !aligned(out, 2) || !aligned(d_block_table, 4) ||
+        !aligned(d_q_start, 4) || !aligned(d_step_len, 4) || !aligned(d_key_len, 4))
+        return fail(c, HKV_ERR_ALIGNMENT, "attention: a tensor is not aligned to its element size");
+    if (requests == 0 || tokens == 0 || max_step == 0) return HKV_OK;
+    a.b.table = d_block_table;
+    a.b.q_start = d_q_start;
+    a.b.step_len = d_step_len;
+    a.b.key_len = d_key_len;
+    a.b.status = c->d_status;
+    a.b.requests = requests;
+    a.b.cols = g.max_pages;
+    a.b.page = g.page_size;
+    a.b.pages = g.num_pages;
+    a.b.tokens = tokens;
+    a.b.max_step = max_step;
+    a.b.window = causal ? g.window_size : 0;
+    a.b.causal = causal ? 1 : 0;
+    a.q = q;
+    a.k_cache = k_cache;
+    a.v_cache = v_cache;
+    a.out = out;
+    a.H = g.num_heads;
+    a.KVH = g.num_kv_heads;
+    a.HD = g.head_dim;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    const cudaStream_t st = (cudaStream_t)stream;
+    const dim3 grid((unsigned)tokens, (unsigned)g.num_heads);
+    if (g.dtype == HKV_DTYPE_F16) hkv_paged_generic_kernel<__half><<<grid, kPagedGenWarps * 32, 0, st>>>(a);
+    else hkv_paged_generic_kernel<__nv_bfloat16><<<grid, kPagedGenWarps * 32, 0, st>>>(a);
+    return launched(c, "attention launch");
+}
+
+}  // namespace
+
+extern "C" {
+
+int hkv_paged_create(hkv_paged_ctx** out, const hkv_paged_geometry* geometry) {
+    if (!out) return HKV_ERR_INVALID_ARG;
+    *out = nullptr;
+    hkv_paged_ctx* c = new (std::nothrow) hkv_paged_ctx();
+    if (!c) return HKV_ERR_CUDA;
+    *out = c;
+    const char* why = "";
+    const int vst = validate(geometry, &why);
+    if (vst) return fail(c, vst, why);
+    c->g = *geometry;
+    int dev = 0, ndev = 0, major = 0;
+    if (cudaGetDeviceCount(&ndev) != cudaSuccess || ndev == 0) {
+        cudaGetLastError();
+        return fail(c, HKV_ERR_NO_DEVICE, "no CUDA device");
+    }
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return fail_cuda(c, e, "cudaGetDevice");
+    cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
+    cudaDeviceGetAttribute(&c->sm_count, cudaDevAttrMultiProcessorCount, dev);
+    if (major != 10) return fail(c, HKV_ERR_NO_DEVICE, "device is not compute capability 10.x (built for sm_100a only)");
+    c->device = dev;
+    e = cudaMalloc(&c->d_status, sizeof(int32_t));
+    if (e != cudaSuccess) return fail_cuda(c, e, "cudaMalloc(status)");
+    e = cudaMemset(c->d_status, 0, sizeof(int32_t));
+    if (e != cudaSuccess) return fail_cuda(c, e, "cudaMemset(status)");
+    e = cudaFuncSetAttribute((const void*)hkv_paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)plan_smem_bytes(kPagedMaxRequests));
+    if (e != cudaSuccess) return fail_cuda(c, e, "cudaFuncSetAttribute(plan shared memory)");
+    c->ready = true;
+    return HKV_OK;
+}
+
+int hkv_paged_destroy(hkv_paged_ctx* c) {
+    if (!c) return HKV_OK;
+    if (c->d_status) cudaFree(c->d_status);
+    delete c;
+    return HKV_OK;
+}
+
+const char* hkv_paged_last_error(const hkv_paged_ctx* c) { return c ? c->err.c_str() : "null context"; }
+size_t hkv_paged_workspace_bytes(const hkv_paged_ctx* c) { return c ? c->workspace_bytes : 0; }
+
+int hkv_paged_device_status(hkv_paged_ctx* c, void* stream, int32_t* status_out) {
+    if (!c || !status_out) return HKV_ERR_INVALID_ARG;
+    PAGED_CHECK(c);
+    cudaError_t e = cudaStreamSynchronize((cudaStream_t)stream);
+    if (e != cudaSuccess) return fail_cuda(c, e, "cudaStreamSynchronize");
+    e = cudaMemcpy(status_out, c->d_status, sizeof(int32_t), cudaMemcpyDeviceToHost);
+    if (e != cudaSuccess) return fail_cuda(c, e, "cudaMemcpy(status)");
+    if (*status_out != 0) {
+        cudaMemset(c->d_status, 0, sizeof(int32_t));
+        return fail(c, HKV_ERR_DEVICE_FAULT, "device status word is non-zero");
+    }
+    return HKV_OK;
+}
+
+int hkv_paged_plan(hkv_paged_ctx* c, int32_t requests, int32_t tokens, const int32_t* d_past_len,
+                   const int32_t* d_new_len, int32_t* d_block_table, const int32_t* d_free_pages,
+                   const int32_t* d_free_count, int32_t* d_total_len, int32_t* d_step_len, int32_t* d_q_start,
+                   int32_t* d_slots, int32_t* d_positions, int32_t* d_free_left, void* stream) {
+    PAGED_CHECK(c);
+    if (!d_past_len || !d_new_len || !d_block_table || !d_free_pages || !d_free_count || !d_total_len || !d_step_len ||
+        !d_q_start || !d_slots || !d_positions || !d_free_left)
+        return fail(c, HKV_ERR_INVALID_ARG, "plan: null argument");
+    if (requests < 0 || tokens < 0) return fail(c, HKV_ERR_INVALID_ARG, "plan: negative count");
+    if (requests > c->g.max_requests || tokens > c->g.max_tokens)
+        return fail(c, HKV_ERR_TOO_LARGE, "plan: more requests or tokens than the context was created for");
+    for (const void* p : {(const void*)d_past_len, (const void*)d_new_len, (const void*)d_block_table, (const void*)d_free_pages,
+                          (const void*)d_free_count, (const void*)d_total_len, (const void*)d_step_len, (const void*)d_q_start,
+                          (const void*)d_slots, (const void*)d_positions, (const void*)d_free_left})
+        if (!aligned(p, 4)) return fail(c, HKV_ERR_ALIGNMENT, "plan: an int32 array is not 4-byte aligned");
+    PlanArgs a{};
+    a.past = d_past_len;
+    a.fresh = d_new_len;
+    a.free_pages = d_free_pages;
+    a.free_count = d_free_count;
+    a.table = d_block_table;
+    a.total = d_total_len;
+    a.step = d_step_len;
+    a.q_start = d_q_start;
+    a.slots = d_slots;
+    a.positions = d_positions;
+    a.free_left = d_free_left;
+    a.requests = requests;
+    a.tokens = tokens;
+    a.cols = c->g.max_pages;
+    a.page = c->g.page_size;
+    a.pages = c->g.num_pages;
+    int ctas = 1;
+    while (ctas < kPlanMaxCluster && (long long)ctas * kPlanThreads * 2 < (long long)tokens + requests) ctas *= 2;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(kPlanThreads);
+    cfg.dynamicSmemBytes = plan_smem_bytes(requests);
+    cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)ctas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, hkv_paged_plan_kernel, a);
+    return e == cudaSuccess ? HKV_OK : fail_cuda(c, e, "plan launch");
+}
+
+int hkv_paged_release(hkv_paged_ctx* c, int32_t requests, const int32_t* d_finished, int32_t* d_seq_len,
+                      const int32_t* d_block_table, int32_t* d_free_pages, int32_t* d_free_count, void* stream) {
+    PAGED_CHECK(c);
+    if (!d_finished || !d_seq_len || !d_block_table || !d_free_pages || !d_free_count)
+        return fail(c, HKV_ERR_INVALID_ARG, "release: null argument");
+    if (requests < 0) return fail(c, HKV_ERR_INVALID_ARG, "release: negative count");
+    if (requests > c->g.max_requests) return fail(c, HKV_ERR_TOO_LARGE, "release: more requests than the context was created for");
+    for (const void* p : {(const void*)d_finished, (const void*)d_seq_len, (const void*)d_block_table,
+                          (const void*)d_free_pages, (const void*)d_free_count})
+        if (!aligned(p, 4)) return fail(c, HKV_ERR_ALIGNMENT, "release: an int32 array is not 4-byte aligned");
+    if (requests == 0) return HKV_OK;
+    ReleaseArgs a{};
+    a.finished = d_finished;
+    a.table = d_block_table;
+    a.seq_len = d_seq_len;
+    a.free_pages = d_free_pages;
+    a.free_count = d_free_count;
+    a.requests = requests;
+    a.cols = c->g.max_pages;
+    a.page = c->g.page_size;
+    a.pages = c->g.num_pages;
+    hkv_paged_release_kernel<<<1, kPlanThreads, (size_t)requests * 8, (cudaStream_t)stream>>>(a);
+    return launched(c, "release launch");
+}
+
+int hkv_paged_append(hkv_paged_ctx* c, const void* k_new, const void* v_new, int64_t kv_token_stride, void* k_cache,
+                     void* v_cache, const int32_t* d_slots, int32_t tokens, void* stream) {
+    PAGED_CHECK(c);
+    if (!k_new || !v_new || !k_cache || !v_cache || !d_slots) return fail(c, HKV_ERR_INVALID_ARG, "append: null argument");
+    if (tokens < 0) return fail(c, HKV_ERR_INVALID_ARG, "append: negative tokens");
+    if (tokens > c->g.max_tokens) return fail(c, HKV_ERR_TOO_LARGE, "append: more tokens than the context was created for");
+    if (!aligned(k_new, 2) || !aligned(v_new, 2) || !aligned(k_cache, 2) || !aligned(v_cache, 2) || !aligned(d_slots, 4))
+        return fail(c, HKV_ERR_ALIGNMENT, "append: a tensor is not aligned to its element size");
+    PagedAppendArgs a{};
+    a.row_elems = c->g.num_kv_heads * c->g.head_dim;
+    if (!stride_ok(kv_token_stride, a.row_elems, &a.stride))
+        return fail(c, HKV_ERR_INVALID_ARG, "append: kv_token_stride smaller than one token's row");
+    if (tokens == 0) return HKV_OK;
+    a.k = k_new;
+    a.v = v_new;
+    a.k_cache = k_cache;
+    a.v_cache = v_cache;
+    a.slots = d_slots;
+    a.status = c->d_status;
+    a.rows = (long long)c->g.num_pages * c->g.page_size;
+    a.tokens = tokens;
+    const bool vec = aligned(k_new, 16) && aligned(v_new, 16) && aligned(k_cache, 16) && aligned(v_cache, 16) &&
+                     a.row_elems % 8 == 0 && a.stride % 8 == 0;
+    const unsigned blocks = (unsigned)std::min<long long>(((long long)tokens + 7) / 8, (long long)c->sm_count * 8);
+    if (vec) hkv_paged_append_kernel<uint4><<<blocks, 256, 0, (cudaStream_t)stream>>>(a);
+    else hkv_paged_append_kernel<uint16_t><<<blocks, 256, 0, (cudaStream_t)stream>>>(a);
+    return launched(c, "append launch");
+}
+
+int hkv_paged_norm_rope(hkv_paged_ctx* c, const hkv_paged_rope* r, void* stream) {
+    PAGED_CHECK(c);
+    if (!r) return fail(c, HKV_ERR_INVALID_ARG, "norm_rope: null arguments");
+    const hkv_paged_geometry& g = c->g;
+    const bool cached = r->k_cache || r->v_cache;
+    if (!r->q || !r->k || !r->q_out || !r->d_positions || (cached && (!r->k_cache || !r->v_cache || !r->v || !r->d_slots)) ||
+        (!cached && !r->k_out))
+        return fail(c, HKV_ERR_INVALID_ARG, "norm_rope: null tensor (q, k, q_out, positions; v, slots and both planes, or k_out)");
+    if (!r->q_norm_w != !r->k_norm_w) return fail(c, HKV_ERR_INVALID_ARG, "norm_rope: one norm weight without the other");
+    if (r->tokens < 0) return fail(c, HKV_ERR_INVALID_ARG, "norm_rope: negative tokens");
+    if (r->tokens > g.max_tokens) return fail(c, HKV_ERR_TOO_LARGE, "norm_rope: more tokens than the context was created for");
+    for (const void* p : {r->q, r->k, r->v, (const void*)r->q_out, (const void*)r->k_out, r->q_norm_w, r->k_norm_w,
+                          (const void*)r->k_cache, (const void*)r->v_cache})
+        if (!aligned(p, 2)) return fail(c, HKV_ERR_ALIGNMENT, "norm_rope: a tensor is not 2-byte aligned");
+    if (!aligned(r->d_positions, 4) || !aligned(r->d_slots, 4))
+        return fail(c, HKV_ERR_ALIGNMENT, "norm_rope: an int32 array is not 4-byte aligned");
+    MropeArgs a{};
+    const int rot = r->rotary_dim == 0 ? g.head_dim : r->rotary_dim;
+    if (rot < 0 || rot > g.head_dim || rot % 2 != 0)
+        return fail(c, HKV_ERR_GEOMETRY, "norm_rope: rotary_dim must be even and at most head_dim");
+    if (!(r->theta > 0.0) || !std::isfinite(r->theta) || !std::isfinite(r->scaling_factor) || !(r->eps >= 0.0f) || !std::isfinite(r->eps))
+        return fail(c, HKV_ERR_INVALID_ARG, "norm_rope: theta must be positive, eps non-negative, all finite");
+    const int axes = r->axes == 0 ? 1 : r->axes;
+    if (axes < 1 || axes > HKV_ROPE_MAX_AXES) return fail(c, HKV_ERR_INVALID_ARG, "norm_rope: axes outside 1..HKV_ROPE_MAX_AXES");
+    if (r->interleaved != 0 && r->interleaved != 1) return fail(c, HKV_ERR_INVALID_ARG, "norm_rope: interleaved is 0 or 1");
+    const int half = rot / 2;
+    if (axes > 1) {
+        long long sum = 0;
+        for (int i = 0; i < axes; ++i) {
+            if (r->sections[i] < 0) return fail(c, HKV_ERR_INVALID_ARG, "norm_rope: negative section");
+            sum += r->sections[i];
+        }
+        if (sum != half) return fail(c, HKV_ERR_INVALID_ARG, "norm_rope: sections must sum to rotary_dim / 2");
+        int at = 0;
+        for (int i = 0; i < axes; ++i) {
+            if (r->interleaved) {
+                // the last pair of axis i is i + axes * (sections[i] - 1)
+                if (i > 0 && r->sections[i] > 0 && i + (long long)axes * (r->sections[i] - 1) >= half)
+                    return fail(c, HKV_ERR_INVALID_ARG, "norm_rope: an interleaved section reaches past rotary_dim / 2");
+                if (i > 0) for (int j = 0; j < r->sections[i]; ++j) a.axis[i + axes * j] = (uint8_t)i;
+            } else {
+                for (int j = 0; j < r->sections[i]; ++j) a.axis[at++] = (uint8_t)i;
+            }
+        }
+    }
+    const long long qrow = (long long)g.num_heads * g.head_dim, krow = (long long)g.num_kv_heads * g.head_dim;
+    if (!stride_ok(r->q_token_stride, qrow, &a.q_stride) || !stride_ok(r->q_out_token_stride, qrow, &a.qo_stride) ||
+        !stride_ok(r->kv_token_stride, krow, &a.kv_stride) || !stride_ok(r->k_out_token_stride, krow, &a.ko_stride))
+        return fail(c, HKV_ERR_INVALID_ARG, "norm_rope: a token stride is smaller than one token's row");
+    if ((r->q_out == r->q && a.qo_stride != a.q_stride) || (!cached && r->k_out == r->k && a.ko_stride != a.kv_stride))
+        return fail(c, HKV_ERR_INVALID_ARG, "norm_rope: in place needs the same token stride on both sides");
+    if (r->position_axis_stride != 0 && r->position_axis_stride < r->tokens)
+        return fail(c, HKV_ERR_INVALID_ARG, "norm_rope: position_axis_stride smaller than tokens");
+    if (r->tokens == 0) return HKV_OK;
+    a.q = r->q; a.k = r->k; a.v = r->v; a.q_w = r->q_norm_w; a.k_w = r->k_norm_w;
+    a.q_out = r->q_out; a.k_out = r->k_out; a.k_cache = r->k_cache; a.v_cache = r->v_cache;
+    a.slots = r->d_slots; a.pos = r->d_positions;
+    a.status = c->d_status;
+    a.axis_stride = r->position_axis_stride ? r->position_axis_stride : r->tokens;
+    a.rows = (long long)g.num_pages * g.page_size;
+    a.tokens = r->tokens; a.H = g.num_heads; a.KVH = g.num_kv_heads; a.HD = g.head_dim; a.rot = rot;
+    a.eps = r->eps;
+    const double scaling = r->scaling_factor > 0.0f ? (double)r->scaling_factor : 1.0;
+    for (int i = 0; i < half; ++i) a.turns[i] = std::pow(r->theta, -2.0 * i / rot) / (scaling * 6.283185307179586476925);
+    // enough warps to fill the machine: a token is shared by several when there are few
+    const int heads = g.num_heads + 2 * g.num_kv_heads;
+    a.parts = (int)std::max<long long>(1, std::min<long long>(heads, (long long)c->sm_count * 16 / r->tokens));
+    const long long units = (long long)r->tokens * a.parts;
+    const unsigned blocks = (unsigned)std::min<long long>((units + kMropeWarps - 1) / kMropeWarps, (long long)c->sm_count * 8);
+    if (g.dtype == HKV_DTYPE_F16) hkv_paged_norm_rope_any_kernel<__half><<<blocks, kMropeThreads, 0, (cudaStream_t)stream>>>(a);
+    else hkv_paged_norm_rope_any_kernel<__nv_bfloat16><<<blocks, kMropeThreads, 0, (cudaStream_t)stream>>>(a);
+    return launched(c, "norm_rope launch");
+}
+
+int hkv_paged_attention(hkv_paged_ctx* c, const void* q, int64_t q_token_stride, const void* k_cache, const void* v_cache,
+                        void* out, const int32_t* d_block_table, const int32_t* d_q_start, const int32_t* d_step_len,
+                        const int32_t* d_total_len, int32_t requests, int32_t tokens, int32_t max_step, float scale,
+                        void* stream) {
+    return attention(c, q, q_token_stride, k_cache, v_cache, out, d_block_table, d_q_start, d_step_len,
+                     d_total_len, requests, tokens, max_step, scale, stream, true);
+}
+
+int hkv_paged_cross_attention(hkv_paged_ctx* c, const void* q, int64_t q_token_stride, const void* k_cache,
+                              const void* v_cache, void* out, const int32_t* d_block_table, const int32_t* d_q_start,
+                              const int32_t* d_step_len, const int32_t* d_key_len, int32_t requests, int32_t tokens,
+                              int32_t max_step, float scale, void* stream) {
+    return attention(c, q, q_token_stride, k_cache, v_cache, out, d_block_table, d_q_start, d_step_len,
+                     d_key_len, requests, tokens, max_step, scale, stream, false);
+}
+
+}  // extern "C"

@@ -21,6 +21,7 @@
  *   k/v plane     [batch, slots, num_kv_heads, head_dim]    src/kv_cache.hpp:175-189
  *   k_new, v_new  [batch, seq_new, num_kv_heads, head_dim]  kernels/attention.cu:1092-1094
  *   prefill q/out [seq_new, num_heads, head_dim], batch 1   kernels/attention.cu:665-668
+ *   paged cache   see the section "paged cache" below (fp16 or bf16)
  */
 #ifndef HKV_H_
 #define HKV_H_
@@ -379,6 +380,148 @@ int hkv_plan_prefill(const hkv_geometry* geometry, int32_t seq_new, int32_t past
  * 1.2 PFLOP/s where 2 048 run at 1.0). Returns the smallest such size when `target` is below it,
  * `target` itself for geometries the tensor-core kernels do not take, <= 0 on bad arguments. */
 int32_t hkv_preferred_prefill_chunk(const hkv_geometry* geometry, int32_t sm_count, int32_t target);
+
+/* ---- paged cache ------------------------------------------------------------------- */
+
+/* A paged cache keeps the K/V rows of all requests in ONE pool of pages instead of a plane of `slots`
+ * rows per sequence: position p of request r lives in row p % page_size of page
+ * block_table[r][p / page_size]. The reference has no paged cache; the row format inside a page is its
+ * plane format (src/kv_cache.hpp:175-189).
+ *
+ *   k/v plane      [num_pages, page_size, num_kv_heads, head_dim]   binary16 or bfloat16 (`dtype`)
+ *   block table    [max_requests][max_pages] int32, entries 0 .. num_pages-1, -1 = not assigned
+ *   packed batch   the new tokens of all requests back to back: request r owns the rows
+ *                  q_start[r] .. q_start[r] + step_len[r] - 1 of q, k_new, v_new, out
+ *   slot           page * page_size + row; -1 = the token is not stored
+ *
+ * One step of a serving loop: hkv_paged_plan (block tables and slot maps from the request lengths),
+ * then per layer hkv_paged_norm_rope or hkv_paged_append (K/V rows to their slots) and
+ * hkv_paged_attention. All of it depends on DEVICE arrays only, so a captured step can be replayed
+ * with other lengths; the host gives upper bounds (`tokens`, `max_step`).
+ *
+ * A context's calls must be ordered on the GPU (one stream, or streams joined by events; graphs that
+ * were captured with one context must not be replayed concurrently): hkv_paged_attention keeps
+ * partial rows in the context's workspace. Two streams take two contexts. */
+typedef enum hkv_dtype { HKV_DTYPE_F16 = 0, HKV_DTYPE_BF16 = 1 } hkv_dtype;
+
+/* Zero-initialise, then fill in. */
+typedef struct hkv_paged_geometry {
+    int32_t dtype;        /* hkv_dtype of q, k, v, the norm weights, the planes and out          */
+    int32_t num_heads;    /* query heads H                                                       */
+    int32_t num_kv_heads; /* KV heads; H % KVH == 0                                              */
+    int32_t head_dim;     /* 1..512                                                              */
+    int32_t page_size;    /* rows per page                                                       */
+    int32_t num_pages;    /* pages per plane; num_pages * page_size <= 2^31 - 1                  */
+    int32_t max_requests; /* rows of the block table, 1..HKV_PAGED_MAX_REQUESTS                  */
+    int32_t max_pages;    /* columns of the block table; max_pages * page_size <= 2^31 - 1       */
+    int32_t max_tokens;   /* upper bound of a call's packed tokens                               */
+    int32_t window_size;  /* 0 = attend everything; W = the last W positions                     */
+    int32_t kernel_select;/* hkv_kernel_select: AUTO, or GENERIC to force the any-geometry kernel,
+                             or TMA to require the staged kernels (HKV_ERR_GEOMETRY otherwise)   */
+    int32_t flags;        /* HKV_FLAG_APPEND_ONLY: no attention workspace                        */
+    int32_t reserved[4];
+} hkv_paged_geometry;
+#define HKV_PAGED_MAX_REQUESTS 4096
+
+typedef struct hkv_paged_ctx hkv_paged_ctx;
+
+/* Validates the geometry and allocates the attention workspace and the status word on the CURRENT
+ * device. On failure *out still holds a context that only carries the message; destroy it. */
+int hkv_paged_create(hkv_paged_ctx** out, const hkv_paged_geometry* geometry);
+int hkv_paged_destroy(hkv_paged_ctx* ctx);
+const char* hkv_paged_last_error(const hkv_paged_ctx* ctx);
+/* As hkv_ctx_device_status. Bit 2 is set by a block-table entry outside 0..num_pages-1 that attention
+ * had to read (its rows count as zeros) or a slot >= num_pages*page_size (not stored). */
+int hkv_paged_device_status(hkv_paged_ctx* ctx, void* stream, int32_t* status_out);
+/* Bytes of device memory the context holds for attention. */
+size_t hkv_paged_workspace_bytes(const hkv_paged_ctx* ctx);
+
+/* Block tables and slot maps of one step, built on the GPU from request lengths. `requests` rows,
+ * `tokens` packed rows (padding included).
+ *   in    d_past_len[r]  positions of request r already in the cache, d_new_len[r] tokens it adds;
+ *         d_free_pages[num_pages] / *d_free_count: stack of free pages, taken from its end (a count
+ *         above num_pages counts as num_pages);
+ *         d_block_table: entries 0 .. ceil(past/page_size)-1 of a request with past > 0
+ *   out   d_block_table: the entries of the pages its new tokens open, in request order, then position
+ *         order (nothing else of the table is written);
+ *         d_q_start[requests+1] = exclusive prefix sums of new_len (negative ones count 0), at most
+ *         `tokens`; d_step_len[r] = new_len or 0; d_total_len[r] = past_len + step_len;
+ *         d_slots[tokens], d_positions[tokens]: slot and position of each packed token, -1 where no
+ *         admitted request has one; *d_free_left = pages left on the stack.
+ * A request is NOT admitted — step_len 0, total_len = past_len, no page taken, its packed rows keep
+ * their place with slot -1 — when a length is negative, past + new exceeds max_pages * page_size, its
+ * rows end beyond `tokens`, or it needs pages and the pages needed up to and including it (over the
+ * requests that pass the other rules) exceed the free ones. A request that needs no page is always
+ * admitted. d_total_len may be d_past_len and d_free_left may be d_free_count (state updated in
+ * place); other overlaps are not allowed. */
+int hkv_paged_plan(hkv_paged_ctx* ctx, int32_t requests, int32_t tokens, const int32_t* d_past_len,
+                   const int32_t* d_new_len, int32_t* d_block_table, const int32_t* d_free_pages,
+                   const int32_t* d_free_count, int32_t* d_total_len, int32_t* d_step_len,
+                   int32_t* d_q_start, int32_t* d_slots, int32_t* d_positions, int32_t* d_free_left,
+                   void* stream);
+
+/* Gives the pages of every request with d_finished[r] != 0 back to the stack (request order, then
+ * table order) and sets its d_seq_len[r] to 0; a request of length 0 gives nothing back, so releasing
+ * twice is harmless. d_free_pages must hold num_pages entries. */
+int hkv_paged_release(hkv_paged_ctx* ctx, int32_t requests, const int32_t* d_finished, int32_t* d_seq_len,
+                      const int32_t* d_block_table, int32_t* d_free_pages, int32_t* d_free_count, void* stream);
+
+/* K and V rows of `tokens` packed tokens to their slots; rows with a negative slot are left out, and
+ * no other row of the planes is touched. kv_token_stride: elements between consecutive tokens of k_new
+ * (= v_new), 0 = dense — views into a fused QKV activation need no copy. No two tokens may share a slot. */
+int hkv_paged_append(hkv_paged_ctx* ctx, const void* k_new, const void* v_new, int64_t kv_token_stride,
+                     void* k_cache, void* v_cache, const int32_t* d_slots, int32_t tokens, void* stream);
+
+/* Per-head RMSNorm (optional) + rotary embedding with one or several position axes (text; time, height
+ * and width of images and video) of packed tokens, K and V written through the slot map.
+ *   x_n = x * rsqrt(mean(x^2) + eps) * w  (x itself without weights)
+ *   pair i < rotary_dim/2 = elements (i, i + rotary_dim/2), turned by
+ *       positions[axis(i)][token] / scaling_factor * theta^(-2i/rotary_dim);
+ *   elements >= rotary_dim pass through normalised; V is copied.
+ *   axis(i), axes > 1: `sections` (sum = rotary_dim/2) give the pairs of each axis — as consecutive
+ *   blocks, or interleaved: pair i belongs to axis a = i % axes where a > 0 and i < axes * sections[a],
+ *   and to axis 0 otherwise (then axes * sections[a] <= rotary_dim/2 + axes - 1 for a > 0).
+ * Angles are reduced in 64 bits, so far positions lose nothing. q_out may be q (in place), then with
+ * the same strides. Without cache planes (both NULL) the turned k goes to k_out (may be k) and v is
+ * ignored. */
+#define HKV_ROPE_MAX_AXES 4
+typedef struct hkv_paged_rope {
+    const void *q, *k, *v;              /* [tokens][heads][head_dim], token strides below         */
+    void *q_out, *k_out;                /* k_out: only without cache planes                       */
+    const void *q_norm_w, *k_norm_w;    /* [head_dim], both or neither                            */
+    void *k_cache, *v_cache;            /* both or neither                                        */
+    const int32_t* d_slots;             /* [tokens]; with cache planes                            */
+    const int32_t* d_positions;         /* [axes][tokens]                                         */
+    int64_t q_token_stride, kv_token_stride, q_out_token_stride, k_out_token_stride; /* 0 = dense  */
+    int64_t position_axis_stride;       /* elements between axes; 0 = tokens                      */
+    int32_t tokens;
+    int32_t rotary_dim;                 /* even, 0 = head_dim                                     */
+    int32_t axes;                       /* 1..HKV_ROPE_MAX_AXES; 0 = 1                            */
+    int32_t sections[HKV_ROPE_MAX_AXES];
+    int32_t interleaved;                /* 0 = blocks, 1 = interleaved                            */
+    float eps, scaling_factor;          /* scaling_factor <= 0 means 1                            */
+    double theta;
+} hkv_paged_rope;
+int hkv_paged_norm_rope(hkv_paged_ctx* ctx, const hkv_paged_rope* args, void* stream);
+
+/* Attention of the new tokens of every request over its pages, their own rows included (append first):
+ * query i of request r sits at position total_len[r] - step_len[r] + i and attends the positions up to
+ * its own, the last window_size of them with a window. From single tokens to whole prompts, mixed in
+ * one call. q [tokens][H][head_dim] with q_token_stride elements between tokens (0 = dense); out dense.
+ * Rows of `out` that belong to no query are left as they were; a query that attends nothing gets zeros.
+ * max_step: upper bound of step_len (queries beyond it are left out); with max_step * H / KVH <= 16 only
+ * the single-token kernel is launched. */
+int hkv_paged_attention(hkv_paged_ctx* ctx, const void* q, int64_t q_token_stride, const void* k_cache,
+                        const void* v_cache, void* out, const int32_t* d_block_table, const int32_t* d_q_start,
+                        const int32_t* d_step_len, const int32_t* d_total_len, int32_t requests, int32_t tokens,
+                        int32_t max_step, float scale, void* stream);
+
+/* Cross attention: the queries of request r attend ALL of the key_len[r] cached rows of its pages — an
+ * encoder's states, of a length of their own; no causal mask, no window. key_len 0 gives zero rows. */
+int hkv_paged_cross_attention(hkv_paged_ctx* ctx, const void* q, int64_t q_token_stride, const void* k_cache,
+                              const void* v_cache, void* out, const int32_t* d_block_table,
+                              const int32_t* d_q_start, const int32_t* d_step_len, const int32_t* d_key_len,
+                              int32_t requests, int32_t tokens, int32_t max_step, float scale, void* stream);
 
 /* ---- utilities ------------------------------------------------------------------- */
 
