@@ -340,19 +340,13 @@ struct PagedAttnArgs {
     float scale_log2;
 };
 constexpr int kPagedGenWarps = 4;
+constexpr float kLow = -3.3e38f;          // start of a running maximum: below every score that is finite
 
+// One output row: query i of request r (packed row t), head h. The whole block takes part.
 template <typename T>
-__global__ void __launch_bounds__(kPagedGenWarps * 32) hkv_paged_generic_kernel(const PagedAttnArgs a) {
-    const int t = blockIdx.x, h = blockIdx.y;
+__device__ __forceinline__ void paged_row(const PagedAttnArgs& a, const int r, const PagedRequest& rq, const int i, const int h) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int lo = 0, hi = a.b.requests - 1;               // the last request that starts at or before t
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (a.b.q_start[mid] <= t) lo = mid; else hi = mid - 1;
-    }
-    const PagedRequest rq = paged_request(a.b, lo);
-    const int i = t - rq.start;
-    if (i < 0 || i >= rq.n) return;                  // a row of no query
+    const long long t = rq.start + i;
     int k_lo, k_hi;
     paged_key_range(a.b, rq, i, k_lo, k_hi);
     const int kvh = h / (a.H / a.KVH);
@@ -364,8 +358,8 @@ __global__ void __launch_bounds__(kPagedGenWarps * 32) hkv_paged_generic_kernel(
         qr[e] = d < a.HD ? to_f32(qp[d]) : 0.0f;
         acc[e] = 0.0f;
     }
-    float m = kNegBig, l = 0.0f;
-    const int32_t* table = a.b.table + (long long)lo * a.b.cols;
+    float m = kLow, l = 0.0f;
+    const int32_t* table = a.b.table + (long long)r * a.b.cols;
     for (int s = k_lo + warp; s < k_hi; s += kPagedGenWarps) {
         const int pg = table[s / a.b.page];
         const bool in = pg >= 0 && pg < a.b.pages;   // an entry outside the planes: rows of zeros
@@ -405,12 +399,41 @@ __global__ void __launch_bounds__(kPagedGenWarps * 32) hkv_paged_generic_kernel(
 #pragma unroll
     for (int w = 0; w < kPagedGenWarps; ++w) gl += s_l[w] * exp2f(s_m[w] - gm);
     const float inv = gl > 0.0f ? 1.0f / gl : 0.0f;
-    T* op = (T*)a.out + ((long long)t * a.H + h) * a.HD;
+    T* op = (T*)a.out + (t * a.H + h) * a.HD;
     for (int d = threadIdx.x; d < a.HD; d += kPagedGenWarps * 32) {
         float o = 0.0f;
 #pragma unroll
         for (int w = 0; w < kPagedGenWarps; ++w) o += s_acc[w][d] * exp2f(s_m[w] - gm);
         op[d] = from_f32<T>(o * inv);
+    }
+    __syncthreads();
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kPagedGenWarps * 32) hkv_paged_generic_kernel(const PagedAttnArgs a) {
+    const int t = blockIdx.x;
+    int lo = 0, hi = a.b.requests - 1;               // the last request that starts at or before t
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (a.b.q_start[mid] <= t) lo = mid; else hi = mid - 1;
+    }
+    const PagedRequest rq = paged_request(a.b, lo);
+    const int i = t - rq.start;
+    if (i < 0 || i >= rq.n) return;                  // a row of no query
+    paged_row<T>(a, lo, rq, i, blockIdx.y);
+}
+
+// Requests marked by the staged kernels: a value of V that is not finite sits where only some of the request's queries
+// look, and 0 * NaN would have reached the others. Their rows are computed again key by key. Marks are taken back.
+template <typename T>
+__global__ void __launch_bounds__(kPagedGenWarps * 32) hkv_paged_fix_kernel(const PagedAttnArgs a, int* fix) {
+    for (int r = blockIdx.x; r < a.b.requests; r += gridDim.x) {
+        if (!fix[r]) continue;                       // (the same word for the whole block, written below by itself only)
+        const PagedRequest rq = paged_request(a.b, r);
+        for (int i = 0; i < rq.n; ++i)
+            for (int h = 0; h < a.H; ++h) paged_row<T>(a, r, rq, i, h);
+        __syncthreads();
+        if (threadIdx.x == 0) fix[r] = 0;
     }
 }
 

@@ -12,6 +12,7 @@
 
 #include "../../include/hkv.h"
 #include "hkv_paged.cuh"
+#include "hkv_paged_decode.cuh"
 #include "hkv_paged_rope.cuh"
 
 using namespace hkv;
@@ -21,6 +22,12 @@ struct hkv_paged_ctx {
     int device = -1;
     int sm_count = 0;
     int32_t* d_status = nullptr;
+    size_t smem_optin = 0, smem_sm = 0;
+    bool staged = false;            // the geometry allows the staged kernels
+    // attention workspace: partial rows of cut requests, the merge kernel's entries, marks of requests to be done again
+    float* part = nullptr;
+    int4* cuts = nullptr;
+    int* fix = nullptr;
     size_t workspace_bytes = 0;
     bool ready = false;
     std::string err;
@@ -93,6 +100,144 @@ int launched(hkv_paged_ctx* c, const char* what) {
     return e == cudaSuccess ? HKV_OK : fail_cuda(c, e, what);
 }
 
+// ---- staged kernels -----------------------------------------------------------------------------------------------
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_tiled_fn() {
+    static EncodeTiledFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult qres;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qres) == cudaSuccess &&
+            qres == cudaDriverEntryPointSuccess)
+            return reinterpret_cast<EncodeTiledFn>(p);
+        return (EncodeTiledFn) nullptr;
+    }();
+    return fn;
+}
+
+// head_dim 64, 96, 128, 256; pages of a power of two of rows, at least 8 (a box of the copy engine is a whole number of
+// 8-row swizzle groups and never crosses a page); groups up to 128.
+bool staged_geometry(const hkv_paged_geometry& g) {
+    const int G = g.num_heads / g.num_kv_heads;
+    const bool hd = g.head_dim == 64 || g.head_dim == 96 || g.head_dim == 128 || g.head_dim == 256;
+    return hd && G <= 128 && g.page_size >= 8 && (g.page_size & (g.page_size - 1)) == 0;
+}
+
+// Map of a plane as [page][row][kv head][head_dim], boxes of `rows` rows of one head, `width` elements wide.
+int encode_plane(hkv_paged_ctx* c, const void* base, int width, int rows, CUtensorMap* out) {
+    const hkv_paged_geometry& g = c->g;
+    const cuuint64_t dims[4] = {(cuuint64_t)g.head_dim, (cuuint64_t)g.num_kv_heads, (cuuint64_t)g.page_size, (cuuint64_t)g.num_pages};
+    const cuuint64_t row = (cuuint64_t)g.num_kv_heads * g.head_dim * 2;
+    const cuuint64_t strides[3] = {(cuuint64_t)g.head_dim * 2, row, row * g.page_size};
+    const cuuint32_t box[4] = {(cuuint32_t)width, 1u, (cuuint32_t)rows, 1u}, one[4] = {1u, 1u, 1u, 1u};
+    const CUresult r = encode_tiled_fn()(
+        out, g.dtype == HKV_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+        const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+        width == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r == CUDA_SUCCESS) return HKV_OK;
+    char buf[96];
+    snprintf(buf, sizeof buf, "cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
+    return fail(c, HKV_ERR_CUDA, buf);
+}
+
+typedef void (*DecodeKernel)(const CUtensorMap, const CUtensorMap, const PagedDecodeArgs, const int);
+template <typename T, int HD>
+DecodeKernel pick_decode_hd(int nt, int groups) {
+    if (nt == 1) return groups == 1 ? hkv_paged_decode_kernel<T, HD, 1, 1> : hkv_paged_decode_kernel<T, HD, 1, 2>;
+    if (HD == 256) return hkv_paged_decode_kernel<T, HD, 2, 1>;    // (two groups of it do not fit the registers)
+    return groups == 1 ? hkv_paged_decode_kernel<T, HD, 2, 1> : hkv_paged_decode_kernel<T, HD, 2, 2>;
+}
+template <typename T>
+DecodeKernel pick_decode_t(int hd, int nt, int groups) {
+    return hd == 64 ? pick_decode_hd<T, 64>(nt, groups) : hd == 96 ? pick_decode_hd<T, 96>(nt, groups)
+         : hd == 128 ? pick_decode_hd<T, 128>(nt, groups) : pick_decode_hd<T, 256>(nt, groups);
+}
+DecodeKernel pick_decode(int dtype, int hd, int nt, int groups) {
+    return dtype == HKV_DTYPE_F16 ? pick_decode_t<__half>(hd, nt, groups) : pick_decode_t<__nv_bfloat16>(hd, nt, groups);
+}
+
+// CTAs that share a span: one per KV head, or two, four, eight heads per CTA where that leaves fewer CTAs idle.
+int gang_for(int kv_heads, int grid) {
+    int best = 1;
+    double best_util = 0.0;
+    for (int per_cta = 1; per_cta <= 8; per_cta *= 2) {
+        if (kv_heads % per_cta != 0) break;
+        const int gang = kv_heads / per_cta;
+        if (gang > grid) continue;
+        const double util = (double)(grid / gang) * gang / grid;
+        if (util >= 0.94) return gang;
+        if (util > best_util) { best_util = util; best = gang; }
+    }
+    return best;
+}
+size_t part_bytes(const hkv_paged_geometry& g, int sm_count) {
+    size_t most = 0;
+    for (int grid : {sm_count, 2 * sm_count})
+        most = std::max(most, (size_t)2 * (grid / gang_for(g.num_kv_heads, grid)) * g.num_kv_heads * kSmallCols * (g.head_dim + 2) * 4);
+    return most;
+}
+
+// Shape of the few-token kernel: two CTAs per SM with one consumer group each, or one CTA with two groups. Two stream a
+// little faster and hide each other's merges; they also double the spans, and with them the parts a request is cut into,
+// which is what a launch of one or two requests spends its time on.
+struct DecodeShape { int groups, grid, gang; PagedDecodePlan plan; };
+DecodeShape decode_shape(const hkv_paged_ctx* c, int cols, int requests) {
+    const hkv_paged_geometry& g = c->g;
+    DecodeShape s{};
+    const int two = 2 * c->sm_count / gang_for(g.num_kv_heads, 2 * c->sm_count);
+    const bool wide = g.head_dim == 256;     // its tiles need the whole shared memory
+    s.groups = two / requests > 40 || wide ? 2 : 1;
+    if (s.groups == 1) {
+        s.plan = paged_decode_plan(g.head_dim, cols, 4, requests, c->smem_sm / 2 - 2048);
+        if (s.plan.stages < 2) s.groups = 2;
+    }
+    if (s.groups == 2) s.plan = paged_decode_plan(g.head_dim, cols, 8, requests, c->smem_optin);
+    s.grid = s.groups == 1 ? 2 * c->sm_count : c->sm_count;
+    if (s.plan.stages < 2 || (wide && cols > 8)) {   // one CTA per SM, one consumer group, the whole shared memory
+        s.groups = 1;
+        s.plan = paged_decode_plan(g.head_dim, cols, 4, requests, c->smem_optin);
+        s.grid = c->sm_count;
+    }
+    s.gang = gang_for(g.num_kv_heads, s.grid);
+    return s;
+}
+
+int launch_small(hkv_paged_ctx* c, const PagedAttnArgs& t, int cols, cudaStream_t st) {
+    const hkv_paged_geometry& g = c->g;
+    const DecodeShape s = decode_shape(c, cols, t.b.requests);
+    if (s.plan.stages < 2) return fail(c, HKV_ERR_GEOMETRY, "attention: shared memory too small for two stages");
+    CUtensorMap mk, mv;
+    PagedDecodeArgs a{};
+    a.t = t;
+    a.part = c->part;
+    a.cuts = c->cuts;
+    a.fix = c->fix;
+    a.gang = s.gang;
+    a.cols = cols;
+    a.box_rows = std::min(g.page_size, kTileRows);
+    a.pieces = kTileRows / a.box_rows;
+    const int width = paged_chunk_width(g.head_dim);
+    int e = encode_plane(c, t.k_cache, width, a.box_rows, &mk);
+    if (!e) e = encode_plane(c, t.v_cache, width, a.box_rows, &mv);
+    if (e) return e;
+    pick_decode(g.dtype, g.head_dim, cols > 8 ? 2 : 1, s.groups)<<<s.grid, (s.groups * 4 + 1) * 32, s.plan.bytes, st>>>(mk, mv, a, s.plan.stages);
+    PagedMergeArgs m{};
+    m.b = t.b;
+    m.part = c->part;
+    m.cuts = c->cuts;
+    m.out = t.out;
+    m.H = t.H;
+    m.KVH = t.KVH;
+    m.HD = t.HD;
+    m.cols = cols;
+    const dim3 grid((unsigned)(s.grid / s.gang), (unsigned)t.KVH, (unsigned)cols);
+    if (g.dtype == HKV_DTYPE_F16) hkv_paged_merge_kernel<__half><<<grid, 256, 0, st>>>(m);
+    else hkv_paged_merge_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(m);
+    return launched(c, "attention launch");
+}
+
 // A token stride: 0 = dense, else at least one token's row.
 bool stride_ok(int64_t given, long long row, long long* out) {
     if (given != 0 && given < row) return false;
@@ -142,6 +287,20 @@ int attention(hkv_paged_ctx* c, const void* q, int64_t q_token_stride, const voi
     a.HD = g.head_dim;
     a.scale_log2 = scale * 1.4426950408889634f;
     const cudaStream_t st = (cudaStream_t)stream;
+    const int G = g.num_heads / g.num_kv_heads;
+    const bool tensors_ok = aligned(q, 16) && aligned(k_cache, 16) && aligned(v_cache, 16) && aligned(out, 16) && a.q_stride % 8 == 0;
+    const bool staged = c->staged && tensors_ok;
+    if (!staged && g.kernel_select == HKV_KERNEL_TMA)
+        return fail(c, HKV_ERR_ALIGNMENT, "attention: the staged kernels need 16-byte aligned tensors and strides");
+    if (staged && (long long)max_step * G <= kSmallCols) {
+        int e = launch_small(c, a, max_step * G, st);
+        if (e) return e;
+        if (max_step == 1) return HKV_OK;      // a single query: nothing is hidden from it alone
+        const unsigned blocks = (unsigned)std::min(requests, c->sm_count);
+        if (g.dtype == HKV_DTYPE_F16) hkv_paged_fix_kernel<__half><<<blocks, kPagedGenWarps * 32, 0, st>>>(a, c->fix);
+        else hkv_paged_fix_kernel<__nv_bfloat16><<<blocks, kPagedGenWarps * 32, 0, st>>>(a, c->fix);
+        return launched(c, "attention launch");
+    }
     const dim3 grid((unsigned)tokens, (unsigned)g.num_heads);
     if (g.dtype == HKV_DTYPE_F16) hkv_paged_generic_kernel<__half><<<grid, kPagedGenWarps * 32, 0, st>>>(a);
     else hkv_paged_generic_kernel<__nv_bfloat16><<<grid, kPagedGenWarps * 32, 0, st>>>(a);
@@ -180,12 +339,40 @@ int hkv_paged_create(hkv_paged_ctx** out, const hkv_paged_geometry* geometry) {
     e = cudaFuncSetAttribute((const void*)hkv_paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              (int)plan_smem_bytes(kPagedMaxRequests));
     if (e != cudaSuccess) return fail_cuda(c, e, "cudaFuncSetAttribute(plan shared memory)");
+    int optin = 0, per_sm = 0;
+    cudaDeviceGetAttribute(&optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev);
+    cudaDeviceGetAttribute(&per_sm, cudaDevAttrMaxSharedMemoryPerMultiprocessor, dev);
+    c->smem_optin = (size_t)optin;
+    c->smem_sm = (size_t)per_sm;
+    c->staged = staged_geometry(*geometry) && geometry->kernel_select != HKV_KERNEL_GENERIC;
+    if (geometry->kernel_select == HKV_KERNEL_TMA && !c->staged)
+        return fail(c, HKV_ERR_GEOMETRY, "the staged kernels need head_dim in {64,96,128,256}, group <= 128, page_size a power of two >= 8");
+    if (c->staged && !(geometry->flags & HKV_FLAG_APPEND_ONLY)) {
+        if (!encode_tiled_fn()) return fail(c, HKV_ERR_CUDA, "cuTensorMapEncodeTiled entry point not available");
+        for (int nt = 1; nt <= 2; ++nt)
+            for (int groups = 1; groups <= 2; ++groups) {
+                // the attribute belongs to the kernel: always the device maximum, so that contexts never lower it for each other
+                e = cudaFuncSetAttribute((const void*)pick_decode(geometry->dtype, geometry->head_dim, nt, groups),
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, optin - 1024);
+                if (e != cudaSuccess) return fail_cuda(c, e, "cudaFuncSetAttribute(shared memory)");
+            }
+        c->smem_optin = (size_t)optin - 1024;   // (the kernels hold a few hundred bytes of their own)
+        const size_t nb = part_bytes(*geometry, c->sm_count);
+        if ((e = cudaMalloc(&c->part, nb)) != cudaSuccess) return fail_cuda(c, e, "cudaMalloc(partial rows)");
+        if ((e = cudaMalloc(&c->cuts, sizeof(int4) * 2 * c->sm_count)) != cudaSuccess) return fail_cuda(c, e, "cudaMalloc(cuts)");
+        if ((e = cudaMalloc(&c->fix, sizeof(int) * geometry->max_requests)) != cudaSuccess) return fail_cuda(c, e, "cudaMalloc(marks)");
+        if ((e = cudaMemset(c->fix, 0, sizeof(int) * geometry->max_requests)) != cudaSuccess) return fail_cuda(c, e, "cudaMemset(marks)");
+        c->workspace_bytes = nb + sizeof(int4) * 2 * c->sm_count + sizeof(int) * geometry->max_requests;
+    }
     c->ready = true;
     return HKV_OK;
 }
 
 int hkv_paged_destroy(hkv_paged_ctx* c) {
     if (!c) return HKV_OK;
+    if (c->part) cudaFree(c->part);
+    if (c->cuts) cudaFree(c->cuts);
+    if (c->fix) cudaFree(c->fix);
     if (c->d_status) cudaFree(c->d_status);
     delete c;
     return HKV_OK;

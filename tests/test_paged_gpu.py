@@ -334,6 +334,49 @@ def test_attention_growing_maxima(hkv, cuda, heads, steps):
     run_attention(hkv, cuda, heads=heads, page=16, steps=steps, keys=[700, 1500], scale=0.0)
 
 
+@pytest.mark.parametrize("value", [float("nan"), float("inf")], ids=str)
+@pytest.mark.parametrize("heads", [(28, 4, 128), (8, 8, 96), (16, 8, 256), (4, 2, 64), (6, 2, 80)], ids=str)
+@pytest.mark.parametrize("steps", [[2, 1, 2], [2, 70, 300]], ids=["tokens", "chunks"])
+def test_values_hidden_from_a_query_never_reach_it(hkv, cuda, heads, steps, value):
+    """NaN and infinities in the K and V rows of later tokens of a chunk, and in rows that only the window of the first
+    queries reaches: the other queries' results are those of clean rows, the ones that look at them are not finite."""
+    torch = cuda
+    H, KVH, HD = heads
+    gen = torch.Generator().manual_seed(11)
+    keys, page, window = [40, 333, 700], 16, 150
+    kc, vc, table = P.make_pages(torch, gen, keys, page, 70, 50, KVH, HD, torch.float16)
+    q = torch.randn(sum(steps), H, HD, generator=gen).half().cuda()
+    ctx = hkv.PagedContext(hkv.PagedGeometry(num_heads=H, num_kv_heads=KVH, head_dim=HD, page_size=page, num_pages=70,
+                                             max_requests=3, max_pages=50, max_tokens=sum(steps), window_size=window))
+    starts = np.concatenate([[0], np.cumsum(steps)])
+    args = (table, i32(torch, starts), i32(torch, steps), i32(torch, keys))
+    clean, got = torch.empty_like(q), torch.empty_like(q)
+    ctx.attention(q, kc, vc, clean, *args, max_step=max(steps))
+    for r in range(3):
+        for j in {keys[r] - 1, max(0, keys[r] - steps[r] + 1 - window)}:      # the newest row; the first query's oldest
+            for plane in (vc, kc):
+                pg, row = int(table[r, j // page]), j % page
+                old = plane[pg, row].clone()
+                plane[pg, row, 0, 3] = value
+                ctx.attention(q, kc, vc, got, *args, max_step=max(steps))
+                plane[pg, row] = old
+                pos = keys[r] - steps[r] + torch.arange(steps[r], device="cuda")
+                sees = torch.zeros(q.shape[0], dtype=torch.bool, device="cuda")
+                sees[starts[r]:starts[r] + steps[r]] = (pos >= j) & (pos < j + window)
+                assert torch.isfinite(got[~sees]).all()
+                assert (got[~sees].double() - clean[~sees].double()).abs().max() < 4e-3     # one more rounding order, no more
+                G = H // KVH
+                hit = got[sees][:, :G]
+                bad = ~torch.isfinite(hit[..., 3] if plane is vc else hit)
+                if plane is vc or value != value:
+                    assert bad.all()
+                assert torch.isfinite(got[:, G:]).all()                         # other KV heads
+    ctx.attention(q, kc, vc, got, *args, max_step=max(steps))
+    assert torch.equal(got, clean), "a mark was left behind"
+    assert ctx.device_status() == 0
+    ctx.close()
+
+
 @pytest.mark.parametrize("heads", [(28, 4, 128), (16, 8, 256), (6, 2, 80)], ids=str)
 @pytest.mark.parametrize("steps", [[1, 1], [60, 200]], ids=["tokens", "chunks"])
 def test_bad_pages_are_reported_and_never_followed(hkv, cuda, heads, steps):
