@@ -61,7 +61,7 @@ __device__ __forceinline__ PagedRequest paged_request(const PagedBatch& a, int r
     if (q.n < 0) q.n = 0;
     const int cap = a.cols * a.page;
     q.keys = len < cap ? (len > 0 ? len : 0) : cap;
-    q.pos0 = (len > 0 ? len : 0) - (step > 0 ? step : 0);
+    q.pos0 = q.keys - (step > 0 ? step : 0);
     return q;
 }
 // Keys [lo, hi) that query i of a request attends; hi <= lo: none.
@@ -423,17 +423,44 @@ __global__ void __launch_bounds__(kPagedGenWarps * 32) hkv_paged_generic_kernel(
     paged_row<T>(a, lo, rq, i, blockIdx.y);
 }
 
-// Requests marked by the staged kernels: a value of V that is not finite sits where only some of the request's queries
-// look, and 0 * NaN would have reached the others. Their rows are computed again key by key. Marks are taken back.
+// Work to be done again: the staged kernels drop values of V that are not finite where only some queries of an item look
+// (0 * NaN would reach the others) and leave the item here. An item is a block of queries of a request and KV head;
+// block -1: all its queries. More items than the list holds: every row of the call is done again.
+constexpr int kFixMax = 1020;
+struct PagedFix {
+    int* head;        // items; CTAs done
+    int4* items;      // [kFixMax]
+    __device__ __forceinline__ void push(int r, int block, int kvh) const {
+        const int at = atomicAdd(head, 1);
+        if (at < kFixMax) items[at] = make_int4(r, block, kvh, 0);
+        else atomicMin(head, 2 * kFixMax);   // (the count stays far from its range's end)
+    }
+};
+
+// The rows of those items, key by key, so that each query sees exactly its own keys. Returns at once in any other call.
+// The last CTA to finish empties the list.
 template <typename T>
-__global__ void __launch_bounds__(kPagedGenWarps * 32) hkv_paged_fix_kernel(const PagedAttnArgs a, int* fix) {
-    for (int r = blockIdx.x; r < a.b.requests; r += gridDim.x) {
-        if (!fix[r]) continue;                       // (the same word for the whole block, written below by itself only)
-        const PagedRequest rq = paged_request(a.b, r);
-        for (int i = 0; i < rq.n; ++i)
-            for (int h = 0; h < a.H; ++h) paged_row<T>(a, r, rq, i, h);
-        __syncthreads();
-        if (threadIdx.x == 0) fix[r] = 0;
+__global__ void __launch_bounds__(kPagedGenWarps * 32) hkv_paged_fix_kernel(const PagedAttnArgs a, const PagedFix fix, const int QB) {
+    const int count = *reinterpret_cast<volatile int*>(fix.head);
+    if (count == 0) return;
+    const int G = a.H / a.KVH;
+    if (count <= kFixMax) {
+        for (int e = 0; e < count; ++e) {
+            const int4 item = fix.items[e];
+            const PagedRequest rq = paged_request(a.b, item.x);
+            const int i0 = item.y < 0 ? 0 : item.y * QB, i1 = item.y < 0 || i0 + QB > rq.n ? rq.n : i0 + QB;
+            for (int x = blockIdx.x; x < (i1 - i0) * G; x += gridDim.x) paged_row<T>(a, item.x, rq, i0 + x / G, item.z * G + x % G);
+        }
+    } else {
+        for (int r = 0; r < a.b.requests; ++r) {
+            const PagedRequest rq = paged_request(a.b, r);
+            for (long long x = blockIdx.x; x < (long long)rq.n * a.H; x += gridDim.x) paged_row<T>(a, r, rq, (int)(x / a.H), (int)(x % a.H));
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0 && atomicAdd(fix.head + 1, 1) == (int)gridDim.x - 1) {
+        fix.head[1] = 0;
+        *reinterpret_cast<volatile int*>(fix.head) = 0;
     }
 }
 

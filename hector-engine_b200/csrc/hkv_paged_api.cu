@@ -12,6 +12,7 @@
 
 #include "../../include/hkv.h"
 #include "hkv_paged.cuh"
+#include "hkv_paged_chunk.cuh"
 #include "hkv_paged_decode.cuh"
 #include "hkv_paged_rope.cuh"
 
@@ -25,9 +26,9 @@ struct hkv_paged_ctx {
     size_t smem_optin = 0, smem_sm = 0;
     bool staged = false;            // the geometry allows the staged kernels
     // attention workspace: partial rows of cut requests, the merge kernel's entries, marks of requests to be done again
-    float* part = nullptr;
-    int4* cuts = nullptr;
-    int* fix = nullptr;
+    float *part = nullptr, *chunk_part = nullptr;
+    int4 *cuts = nullptr, *chunk_cuts = nullptr;
+    int4* fix = nullptr;            // [1 + kFixMax], the count in the first
     size_t workspace_bytes = 0;
     bool ready = false;
     std::string err;
@@ -142,6 +143,8 @@ int encode_plane(hkv_paged_ctx* c, const void* base, int width, int rows, CUtens
     return fail(c, HKV_ERR_CUDA, buf);
 }
 
+PagedFix fix_of(const hkv_paged_ctx* c) { return PagedFix{reinterpret_cast<int*>(c->fix), c->fix + 1}; }
+
 typedef void (*DecodeKernel)(const CUtensorMap, const CUtensorMap, const PagedDecodeArgs, const int);
 template <typename T, int HD>
 DecodeKernel pick_decode_hd(int nt, int groups) {
@@ -213,7 +216,7 @@ int launch_small(hkv_paged_ctx* c, const PagedAttnArgs& t, int cols, cudaStream_
     a.t = t;
     a.part = c->part;
     a.cuts = c->cuts;
-    a.fix = c->fix;
+    a.fix = fix_of(c);
     a.gang = s.gang;
     a.cols = cols;
     a.box_rows = std::min(g.page_size, kTileRows);
@@ -235,6 +238,79 @@ int launch_small(hkv_paged_ctx* c, const PagedAttnArgs& t, int cols, cudaStream_
     const dim3 grid((unsigned)(s.grid / s.gang), (unsigned)t.KVH, (unsigned)cols);
     if (g.dtype == HKV_DTYPE_F16) hkv_paged_merge_kernel<__half><<<grid, 256, 0, st>>>(m);
     else hkv_paged_merge_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(m);
+    return launched(c, "attention launch");
+}
+
+// ---- prompt chunks ----
+int staged_hd(int hd) { return hd == 96 ? 128 : hd; }
+bool chunk_geometry(const hkv_paged_geometry& g) { return g.head_dim != 256; }
+
+typedef void (*ChunkKernel)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const PagedChunkArgs);
+ChunkKernel pick_chunk(int dtype, int hd) {
+    if (dtype == HKV_DTYPE_F16) return staged_hd(hd) == 64 ? hkv_paged_chunk_kernel<__half, 64> : hkv_paged_chunk_kernel<__half, 128>;
+    return staged_hd(hd) == 64 ? hkv_paged_chunk_kernel<__nv_bfloat16, 64> : hkv_paged_chunk_kernel<__nv_bfloat16, 128>;
+}
+size_t chunk_part_bytes(const hkv_paged_geometry& g, int sm_count) { return 2ull * sm_count * 2 * kCkRows * (g.head_dim + 4) * sizeof(float); }
+
+// The line's table counts units of 128 << shift keys; the shift keeps the largest batch the context allows inside 31 bits.
+int line_shift(const hkv_paged_geometry& g, int QB) {
+    const double keys = (double)g.max_pages * g.page_size + kLineOverhead + QB;
+    const double units = ((double)g.max_tokens / QB + g.max_requests) * g.num_kv_heads * (keys / kLineUnit + 1.0);
+    int shift = 0;
+    while (units / (double)(1ll << shift) > 1.0e9) ++shift;
+    return shift;
+}
+
+int launch_chunk(hkv_paged_ctx* c, const PagedAttnArgs& t, const void* q, bool small, cudaStream_t st) {
+    const hkv_paged_geometry& g = c->g;
+    const int G = g.num_heads / g.num_kv_heads;
+    PagedChunkArgs a{};
+    a.t = t;
+    a.QT = kCkRows / G;
+    a.line.G = G;
+    a.line.KVH = g.num_kv_heads;
+    a.line.QB = 2 * a.QT;
+    a.line.keys = kCkKeys;
+    a.line.shift = line_shift(g, a.line.QB);
+    a.part = c->chunk_part;
+    a.cuts = c->chunk_cuts;
+    a.fix = fix_of(c);
+    a.box_rows = std::min(g.page_size, kCkKeys);
+    a.pieces = kCkKeys / a.box_rows;
+    a.small = small ? 1 : 0;
+    CUtensorMap mq, mk, mv;
+    const cuuint64_t dims[3] = {(cuuint64_t)g.head_dim, (cuuint64_t)g.num_heads, (cuuint64_t)t.b.tokens};
+    const cuuint64_t strides[2] = {(cuuint64_t)g.head_dim * 2, (cuuint64_t)t.q_stride * 2};
+    const cuuint32_t box[3] = {64u, (cuuint32_t)G, (cuuint32_t)a.QT}, one[3] = {1u, 1u, 1u};
+    const CUresult r = encode_tiled_fn()(
+        &mq, g.dtype == HKV_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q),
+        dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(c, HKV_ERR_CUDA, "cuTensorMapEncodeTiled failed (queries)");
+    int e = encode_plane(c, t.k_cache, 64, a.box_rows, &mk);
+    if (!e) e = encode_plane(c, t.v_cache, 64, a.box_rows, &mv);
+    if (e) return e;
+    pick_chunk(g.dtype, g.head_dim)<<<c->sm_count, kCkThreads, chunk_smem_bytes(staged_hd(g.head_dim), t.b.requests), st>>>(mq, mk, mv, a);
+    PagedChunkMergeArgs m{};
+    m.b = t.b;
+    m.part = c->chunk_part;
+    m.cuts = c->chunk_cuts;
+    m.out = t.out;
+    m.H = t.H;
+    m.KVH = t.KVH;
+    m.HD = t.HD;
+    m.QT = a.QT;
+    m.QB = a.line.QB;
+    m.tiles = 2;
+    const dim3 grid((unsigned)c->sm_count, 8);
+    if (g.dtype == HKV_DTYPE_F16) hkv_paged_chunk_merge_kernel<__half><<<grid, 256, 0, st>>>(m);
+    else hkv_paged_chunk_merge_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(m);
+    return launched(c, "attention launch");
+}
+
+int launch_fix(hkv_paged_ctx* c, const PagedAttnArgs& t, int QB, cudaStream_t st) {
+    if (c->g.dtype == HKV_DTYPE_F16) hkv_paged_fix_kernel<__half><<<c->sm_count, kPagedGenWarps * 32, 0, st>>>(t, fix_of(c), QB);
+    else hkv_paged_fix_kernel<__nv_bfloat16><<<c->sm_count, kPagedGenWarps * 32, 0, st>>>(t, fix_of(c), QB);
     return launched(c, "attention launch");
 }
 
@@ -292,14 +368,15 @@ int attention(hkv_paged_ctx* c, const void* q, int64_t q_token_stride, const voi
     const bool staged = c->staged && tensors_ok;
     if (!staged && g.kernel_select == HKV_KERNEL_TMA)
         return fail(c, HKV_ERR_ALIGNMENT, "attention: the staged kernels need 16-byte aligned tensors and strides");
-    if (staged && (long long)max_step * G <= kSmallCols) {
-        int e = launch_small(c, a, max_step * G, st);
-        if (e) return e;
-        if (max_step == 1) return HKV_OK;      // a single query: nothing is hidden from it alone
-        const unsigned blocks = (unsigned)std::min(requests, c->sm_count);
-        if (g.dtype == HKV_DTYPE_F16) hkv_paged_fix_kernel<__half><<<blocks, kPagedGenWarps * 32, 0, st>>>(a, c->fix);
-        else hkv_paged_fix_kernel<__nv_bfloat16><<<blocks, kPagedGenWarps * 32, 0, st>>>(a, c->fix);
-        return launched(c, "attention launch");
+    const bool only_small = (long long)max_step * G <= kSmallCols;
+    // (the prompt kernel takes the row maximum before the scale, which it can for a positive one)
+    if (staged && (only_small || (chunk_geometry(g) && scale > 0.0f))) {
+        const bool small = G <= kSmallCols;              // some step_len can be one of the few-token kernel's
+        int e = HKV_OK;
+        if (small) e = launch_small(c, a, std::min(kSmallCols, only_small ? max_step * G : kSmallCols / G * G), st);
+        if (!e && !only_small) e = launch_chunk(c, a, q, small, st);
+        if (!e && max_step > 1) e = launch_fix(c, a, 2 * (kCkRows / G), st);   // (nothing is hidden from a single query)
+        return e;
     }
     const dim3 grid((unsigned)tokens, (unsigned)g.num_heads);
     if (g.dtype == HKV_DTYPE_F16) hkv_paged_generic_kernel<__half><<<grid, kPagedGenWarps * 32, 0, st>>>(a);
@@ -357,12 +434,23 @@ int hkv_paged_create(hkv_paged_ctx** out, const hkv_paged_geometry* geometry) {
                 if (e != cudaSuccess) return fail_cuda(c, e, "cudaFuncSetAttribute(shared memory)");
             }
         c->smem_optin = (size_t)optin - 1024;   // (the kernels hold a few hundred bytes of their own)
+        if (chunk_geometry(*geometry)) {
+            const size_t need = chunk_smem_bytes(staged_hd(geometry->head_dim), geometry->max_requests);
+            if (need > c->smem_optin) return fail(c, HKV_ERR_TOO_LARGE, "shared memory too small for the request table");
+            e = cudaFuncSetAttribute((const void*)pick_chunk(geometry->dtype, geometry->head_dim),
+                                     cudaFuncAttributeMaxDynamicSharedMemorySize, optin - 1024);
+            if (e != cudaSuccess) return fail_cuda(c, e, "cudaFuncSetAttribute(shared memory)");
+            const size_t cb = chunk_part_bytes(*geometry, c->sm_count);
+            if ((e = cudaMalloc(&c->chunk_part, cb)) != cudaSuccess) return fail_cuda(c, e, "cudaMalloc(partial rows)");
+            if ((e = cudaMalloc(&c->chunk_cuts, sizeof(int4) * c->sm_count)) != cudaSuccess) return fail_cuda(c, e, "cudaMalloc(cuts)");
+            c->workspace_bytes += cb + sizeof(int4) * c->sm_count;
+        }
         const size_t nb = part_bytes(*geometry, c->sm_count);
         if ((e = cudaMalloc(&c->part, nb)) != cudaSuccess) return fail_cuda(c, e, "cudaMalloc(partial rows)");
         if ((e = cudaMalloc(&c->cuts, sizeof(int4) * 2 * c->sm_count)) != cudaSuccess) return fail_cuda(c, e, "cudaMalloc(cuts)");
-        if ((e = cudaMalloc(&c->fix, sizeof(int) * geometry->max_requests)) != cudaSuccess) return fail_cuda(c, e, "cudaMalloc(marks)");
-        if ((e = cudaMemset(c->fix, 0, sizeof(int) * geometry->max_requests)) != cudaSuccess) return fail_cuda(c, e, "cudaMemset(marks)");
-        c->workspace_bytes = nb + sizeof(int4) * 2 * c->sm_count + sizeof(int) * geometry->max_requests;
+        if ((e = cudaMalloc(&c->fix, sizeof(int4) * (1 + kFixMax))) != cudaSuccess) return fail_cuda(c, e, "cudaMalloc(list)");
+        if ((e = cudaMemset(c->fix, 0, sizeof(int4) * (1 + kFixMax))) != cudaSuccess) return fail_cuda(c, e, "cudaMemset(list)");
+        c->workspace_bytes += nb + sizeof(int4) * (2 * c->sm_count + 1 + kFixMax);
     }
     c->ready = true;
     return HKV_OK;
@@ -373,6 +461,8 @@ int hkv_paged_destroy(hkv_paged_ctx* c) {
     if (c->part) cudaFree(c->part);
     if (c->cuts) cudaFree(c->cuts);
     if (c->fix) cudaFree(c->fix);
+    if (c->chunk_part) cudaFree(c->chunk_part);
+    if (c->chunk_cuts) cudaFree(c->chunk_cuts);
     if (c->d_status) cudaFree(c->d_status);
     delete c;
     return HKV_OK;

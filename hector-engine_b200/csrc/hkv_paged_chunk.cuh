@@ -1,0 +1,592 @@
+// hkv_paged_chunk.cuh — attention of prompt chunks over a paged cache on the 5th-generation tensor cores (tcgen05, tensor
+// memory): the requests of a ragged batch that have more query rows per KV head than the few-token kernel takes.
+// head_dim 64, 128, and 96 staged as 128 with columns of zeros.
+//
+// Bound: the tensor cores (4 H HD flops per attended pair), with exp2 and the softmax warps' issue slots close behind.
+//   * Item = two tiles A and B of 128 query rows (row = query, head of the group) of one request and KV head; both are
+//     contracted with the same staged K and V tiles of 128 positions. A block of queries that fits one tile leaves B out.
+//   * The items of the batch form a line that is cut into equal spans, one per CTA (hkv_paged_line.cuh): a batch of any
+//     mix keeps every SM busy to the end, and one short chunk over a long request is spread over all of them. An item that
+//     is cut leaves partial rows, two sets per CTA at most, which the merge kernel joins.
+//   * Warps: 0-3 softmax of tile A, 4-7 of tile B (one thread per row), 8 producer, 9 MMA issuer, 10 writes the merge
+//     kernel's entry, 11 completes the warpgroup for setmaxnreg. A key tile is a set of boxes, one per page: the
+//     producer's lanes look up one page each, a tile ahead, and issue side by side.
+//   * Tensor memory: S_A, S_B (128 columns each; P is written over the first half of its S), O_A, O_B. Per key tile:
+//     PV_A QK_A(next) PV_B QK_B(next), so that one tile's softmax runs under the other's products. O is rescaled only
+//     when a row's maximum outgrows its reference by 2^8. P is rounded to the element type (its sum is not). 3 of 8 pairs
+//     take a polynomial on the FMA pipe instead of ex2, the narrowest unit.
+//   * Every wait is bounded and reports through the status word; tensor memory is freed on every path.
+#pragma once
+
+#include <cuda.h>
+
+#include "hkv_paged_decode.cuh"
+#include "hkv_paged_line.cuh"
+#include "hkv_tc_ops.cuh"
+
+namespace hkv {
+
+constexpr int kCkRows = 128, kCkKeys = 128;
+constexpr int kCkStages = 2;              // K tiles and V tiles in flight
+constexpr int kCkThreads = 384;
+constexpr int kCkEmuOf8 = 3;              // pairs of every 8 whose exp2 runs on the FMA pipe
+constexpr int kCkDesc = 16;               // words of a work descriptor
+// A row sum beyond this comes from a score that is not a number: sums of n probabilities stay below n * 2^8.
+constexpr float kSumLimit = 1.0e30f;
+
+struct PagedChunkArgs {
+    PagedAttnArgs t;
+    PagedLine line;           // `pre` is filled in by the kernel
+    float* part;              // [2 * grid][rows per item][HD + 4]: o, maximum (log2 domain), sum
+    int4* cuts;               // [grid]: the item that starts in a CTA's span and goes on behind it: {request, kv head, block, parts}
+    PagedFix fix;
+    int QT;                   // queries per 128-row tile
+    int box_rows, pieces;     // rows of a box; boxes per tile and column block
+    int small;                // 1: the few-token kernel takes the requests with few rows
+};
+__host__ __device__ constexpr size_t chunk_smem_bytes(int HD /*staged*/, int requests) {
+    return 1024 + (size_t)(2 + 2 * kCkStages) * kCkRows * HD * 2 + 32 * 8 + 16 + 4 * kCkDesc * 4 + (size_t)(requests + 1) * 4 + 16;
+}
+__device__ __forceinline__ bool chunk_takes(const PagedChunkArgs& a, const PagedRequest& q) {
+    return q.n > 0 && !(a.small && paged_is_small(q, a.line.G));
+}
+
+// Units before each request, over the block; returns the units of all. `pre` [requests + 1] in shared memory.
+template <typename Args>
+__device__ __forceinline__ uint32_t chunk_line(const Args& a, uint32_t* pre, long long* buf) {
+    const PagedBatch& b = a.t.b;
+    const int tid = threadIdx.x, R = b.requests;
+    const int per = (R + (int)blockDim.x - 1) / (int)blockDim.x, r0 = tid * per, r1 = r0 + per < R ? r0 + per : R;
+    long long sum = 0;
+    for (int r = r0; r < r1; ++r) {
+        const PagedRequest q = paged_request(b, r);
+        const long long n = chunk_takes(a, q) ? line_units(b, a.line, q) : 0;
+        pre[r] = (uint32_t)n;
+        sum += n;
+    }
+    long long all;
+    long long at = block_scan(sum, buf, all);
+    for (int r = r0; r < r1; ++r) {
+        const uint32_t n = pre[r];
+        pre[r] = (uint32_t)at;
+        at += n;
+    }
+    if (tid == 0) pre[R] = (uint32_t)all;
+    __syncthreads();
+    return (uint32_t)all;
+}
+
+// The merge kernel's entry of CTA `cta`, by one warp: the item that starts in its span and goes on behind it.
+__device__ __forceinline__ void chunk_cut_entry(const PagedBatch& b, const PagedLine& l, const uint32_t W, const int ctas, const int cta,
+                                                int4* cuts) {
+    const int lane = threadIdx.x & 31;
+    int4 entry = make_int4(0, 0, 0, 0);
+    if (cta < ctas) {
+        // lanes 0 and 1: this span's cuts; an item that goes on past the end cut was begun here if the span does not start inside it
+        const LineCut mine = line_locate(b, l, line_boundary(W, ctas, cta + (lane & 1)), W);
+        LineCut c0, c1;
+        c0.r = __shfl_sync(0xffffffffu, mine.r, 0); c0.kvh = __shfl_sync(0xffffffffu, mine.kvh, 0);
+        c0.p = __shfl_sync(0xffffffffu, mine.p, 0); c0.t = __shfl_sync(0xffffffffu, mine.t, 0);
+        c1.r = __shfl_sync(0xffffffffu, mine.r, 1); c1.kvh = __shfl_sync(0xffffffffu, mine.kvh, 1);
+        c1.p = __shfl_sync(0xffffffffu, mine.p, 1); c1.t = __shfl_sync(0xffffffffu, mine.t, 1);
+        if (c1.r < b.requests && c1.t > 0 && !(line_same_item(c0, c1) && c0.t > 0)) {
+            int parts = 2;
+            for (int base = cta + 2;; base += 32) {          // further cuts inside the same item
+                const int c = base + lane;
+                const LineCut x = line_locate(b, l, line_boundary(W, ctas, c < ctas ? c : ctas), W);
+                const unsigned in = __ballot_sync(0xffffffffu, c < ctas && line_same_item(x, c1) && x.t > 0);
+                parts += __popc(in);
+                if (in != 0xffffffffu) break;
+            }
+            entry = make_int4(c1.r, c1.kvh, c1.p, parts);
+        }
+    }
+    if (lane == 0) cuts[cta] = entry;
+}
+
+// The producer's walk over its span: calls piece(r, request, kvh, p, first key tile, tiles, slot) for every piece of work;
+// slot -1: the whole item. Warp-uniform. Stops when piece() returns false.
+template <typename F>
+__device__ __forceinline__ void chunk_walk(const PagedBatch& b, const PagedLine& l, const uint32_t W, const int ctas, const int cta, F piece) {
+    if (cta >= ctas || W == 0) return;
+    const int lane = threadIdx.x & 31;
+    const LineCut mine = line_locate(b, l, line_boundary(W, ctas, cta + (lane & 1)), W);
+    LineCut c, e;
+    c.r = __shfl_sync(0xffffffffu, mine.r, 0); c.kvh = __shfl_sync(0xffffffffu, mine.kvh, 0);
+    c.p = __shfl_sync(0xffffffffu, mine.p, 0); c.t = __shfl_sync(0xffffffffu, mine.t, 0);
+    e.r = __shfl_sync(0xffffffffu, mine.r, 1); e.kvh = __shfl_sync(0xffffffffu, mine.kvh, 1);
+    e.p = __shfl_sync(0xffffffffu, mine.p, 1); e.t = __shfl_sync(0xffffffffu, mine.t, 1);
+    while (c.r < b.requests && line_before(c, e)) {
+        if (l.pre[c.r + 1] == l.pre[c.r]) { ++c.r; c.kvh = c.p = c.t = 0; continue; }   // not this kernel's request
+        const PagedRequest q = paged_request(b, c.r);
+        int kt0, nt;
+        line_tiles(b, l, q, c.p, kt0, nt);
+        const int end = line_same_item(c, e) ? e.t : nt;
+        const int slot = c.t == 0 && end == nt ? -1 : 2 * cta + (c.t == 0 ? 1 : 0);
+        if (end > c.t && !piece(c.r, q, c.kvh, c.p, kt0 + c.t, end - c.t, slot)) return;
+        c.t = 0;
+        if (++c.p >= line_blocks(q.n, l.QB)) {
+            c.p = 0;
+            if (++c.kvh == l.KVH) { c.kvh = 0; ++c.r; }
+        }
+    }
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kCkThreads, 1)
+hkv_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                       const __grid_constant__ CUtensorMap tm_v, const PagedChunkArgs a) {
+    static_assert(HD == 64 || HD == 128, "staged head_dim 64 or 128");
+    constexpr int NCH = HD / 64;                       // 64-element column blocks
+    constexpr int CHUNK_BYTES = kCkRows * 128;
+    constexpr int TILE_BYTES = kCkRows * HD * 2;
+    constexpr uint32_t TMEM_COLS = 512;
+    constexpr uint32_t COL_S = 0, COL_O = 256;         // + 128 * group
+    constexpr uint32_t FMT = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);   // operand type of the MMA
+    constexpr uint32_t IDESC_QK = FMT | (1u << 4) | ((uint32_t)(kCkKeys >> 3) << 17) | ((uint32_t)(kCkRows >> 4) << 24);
+    constexpr uint32_t IDESC_PV = FMT | (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kCkRows >> 4) << 24);
+
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t* k_gen = smem + 2 * TILE_BYTES;                   // after the query tiles A, B
+    uint8_t* v_gen = k_gen + kCkStages * TILE_BYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(v_gen + kCkStages * TILE_BYTES);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 32);
+    volatile int* queue = reinterpret_cast<volatile int*>(tmem_slot + 4);   // [4][kCkDesc]
+    uint32_t* pre = tmem_slot + 4 + 4 * kCkDesc;                            // [requests + 1]
+    __shared__ long long scan_buf[33];
+    const uint32_t q_smem = smem_u32(smem), k_smem = smem_u32(k_gen), v_smem = smem_u32(v_gen), bar0 = smem_u32(bars);
+    const uint32_t B_QFULL = bar0, B_QEMPTY = bar0 + 8, B_KFULL = bar0 + 16, B_KEMPTY = bar0 + 32, B_VFULL = bar0 + 48,
+                   B_VEMPTY = bar0 + 64, B_SFULL = bar0 + 80, B_PFULL = bar0 + 96, B_OFULL = bar0 + 112, B_DONE = bar0 + 128,
+                   B_WF = bar0 + 144, B_WE = bar0 + 176;      // work queue: slot full [4], slot read [4]
+    const PagedBatch& bt = a.t.b;
+    const int G = a.line.G, H = a.t.H, D = a.t.HD;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        mbar_init(B_QFULL, 1); mbar_init(B_QEMPTY, 1); mbar_init(B_DONE, 1);
+        for (int s = 0; s < kCkStages; ++s) {
+            mbar_init(B_KFULL + 8 * s, 1); mbar_init(B_KEMPTY + 8 * s, 1);
+            mbar_init(B_VFULL + 8 * s, 1); mbar_init(B_VEMPTY + 8 * s, 1);
+        }
+        for (int g = 0; g < 2; ++g) { mbar_init(B_SFULL + 8 * g, 1); mbar_init(B_PFULL + 8 * g, 128); mbar_init(B_OFULL + 8 * g, 1); }
+        for (int i = 0; i < 4; ++i) { mbar_init(B_WF + 8 * i, 1); mbar_init(B_WE + 8 * i, 9); }
+        fence_mbar_init();
+        tma_prefetch_desc(&tm_q); tma_prefetch_desc(&tm_k); tma_prefetch_desc(&tm_v);
+    }
+    const uint32_t W = chunk_line(a, pre, scan_buf);
+    PagedLine line = a.line;
+    line.pre = pre;
+    const int ctas = line_ctas(W, (int)gridDim.x);
+    if (warp == 9) tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    // entry k of the queue lives in slot k % 4, phase k / 4
+    auto queue_wait = [&](uint32_t k) -> bool { return mbar_wait(B_WF + 8 * (k & 3), (k >> 2) & 1, bt.status); };
+
+    if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
+    if (warp == 8) {
+        // ------------------------------ producer (the whole warp) ------------------------------
+        uint32_t gt = 0, it = 0;
+        bool ok = true;
+        auto publish = [&](int r, const PagedRequest& q, int kvh, int p, int kt, int nt, int slot, int two) -> bool {
+            const uint32_t s = it & 3;
+            if (it >= 4 && !__all_sync(0xffffffffu, mbar_wait(B_WE + 8 * s, ((it >> 2) - 1) & 1, bt.status))) return false;
+            if (lane == 0) {
+                volatile int* d = queue + s * kCkDesc;
+                d[0] = r; d[1] = kvh; d[2] = p; d[3] = kt; d[4] = nt; d[5] = slot; d[6] = two;
+                d[7] = q.start; d[8] = q.n; d[9] = q.pos0; d[10] = q.keys;
+                mbar_arrive(B_WF + 8 * s);
+            }
+            __syncwarp();
+            return true;
+        };
+        const int page_shift = 31 - __clz(bt.page);
+        const int my_piece = lane % a.pieces;          // the page this lane looks up: one per box of a column block
+        chunk_walk(bt, line, W, ctas, blockIdx.x, [&](int r, const PagedRequest& q, int kvh, int p, int kt, int nt, int slot) -> bool {
+            const int i0 = p * a.line.QB, two = i0 + a.QT < q.n ? 1 : 0;
+            if (!publish(r, q, kvh, p, kt, nt, slot, two)) { ok = false; return false; }
+            if (!__all_sync(0xffffffffu, mbar_wait(B_QEMPTY, (it & 1) ^ 1, bt.status))) { ok = false; return false; }
+            if (lane == 0) {
+                mbar_expect_tx(B_QFULL, (uint32_t)((1 + two) * NCH * a.QT * G * 128));
+                for (int t2 = 0; t2 <= two; ++t2)
+#pragma unroll
+                    for (int c = 0; c < NCH; ++c)
+                        tma_load_3d(q_smem + t2 * TILE_BYTES + c * CHUNK_BYTES, &tm_q, B_QFULL, c * 64, kvh * G, q.start + i0 + t2 * a.QT);
+            }
+            __syncwarp();
+            ++it;
+            int lo, hi, x, y;
+            paged_key_range(bt, q, i0, lo, x);
+            const int i1 = (i0 + a.line.QB < q.n ? i0 + a.line.QB : q.n) - 1;
+            paged_key_range(bt, q, i1, y, hi);
+            const int32_t* table = bt.table + (long long)r * bt.cols;
+            // page of a box: behind the tensor (zeros, nothing read) where no query of the item looks
+            auto look_up = [&](int pos) -> int {
+                if (pos >= hi || pos + a.box_rows <= lo) return bt.pages;
+                const int pg = __ldg(table + (pos >> page_shift));
+                if (pg >= 0 && pg < bt.pages) return pg;
+                atomicOr(bt.status, kStatusBoundCheck);
+                return bt.pages;
+            };
+            int pg = look_up(kt * kCkKeys + my_piece * a.box_rows);
+            for (int t = 0; t < nt; ++t, ++gt) {
+                const int pos0 = (kt + t) * kCkKeys;
+                const int pg_next = t + 1 < nt ? look_up(pos0 + kCkKeys + my_piece * a.box_rows) : 0;
+                const uint32_t s = gt % kCkStages, ph = (gt / kCkStages) & 1;
+                for (int kv = 0; kv < 2; ++kv) {
+                    const uint32_t full = (kv ? B_VFULL : B_KFULL) + 8 * s, empty = (kv ? B_VEMPTY : B_KEMPTY) + 8 * s;
+                    if (!__all_sync(0xffffffffu, mbar_wait(empty, ph ^ 1, bt.status))) {
+                        if (kv && lane == 0) mbar_wait(B_KFULL + 8 * s, ph, bt.status);   // the K copies above are in flight
+                        ok = false;
+                        return false;
+                    }
+                    if (lane == 0) mbar_expect_tx(full, TILE_BYTES);
+                    __syncwarp();
+                    const uint32_t dst = (kv ? v_smem : k_smem) + s * TILE_BYTES;
+                    for (int b0 = 0; b0 < NCH * a.pieces; b0 += 32) {
+                        const int bx = b0 + lane, piece = bx % a.pieces, c = bx / a.pieces;
+                        if (bx < NCH * a.pieces)
+                            tma_load_4d(dst + c * CHUNK_BYTES + piece * a.box_rows * 128, kv ? &tm_v : &tm_k, full, c * 64, kvh,
+                                        (pos0 + piece * a.box_rows) & (bt.page - 1), pg);
+                    }
+                }
+                pg = pg_next;
+            }
+            return true;
+        });
+        // no more work (also after a wait that ran out: the other roles leave at once)
+        const uint32_t pieces_done = it;
+        const PagedRequest none{0, 0, 0, 0};
+        publish(-1, none, 0, 0, 0, 0, 0, 0);
+        // copies in flight have landed before the CTA retires (tiles 0..gt-1 were issued)
+        if (lane == 0) {
+            if (pieces_done > 0) mbar_wait(B_QFULL, (pieces_done - 1) & 1, bt.status);
+            for (uint32_t i = 1; i <= (uint32_t)kCkStages && i <= gt; ++i) {
+                const uint32_t g = gt - i;
+                mbar_wait(B_KFULL + 8 * (g % kCkStages), (g / kCkStages) & 1, bt.status);
+                mbar_wait(B_VFULL + 8 * (g % kCkStages), (g / kCkStages) & 1, bt.status);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 10) {
+        chunk_cut_entry(bt, line, W, ctas, blockIdx.x, a.cuts);
+    } else if (warp == 9) {
+        // ------------------------------ MMA issuer ------------------------------
+        if (elect_one()) {
+            uint32_t gt = 0, it = 0, gb = 0;               // tiles; items; tiles of tile B
+            bool ok = true;
+            const uint64_t qdesc0 = umma_desc_sw128(q_smem, 16), kdesc0 = umma_desc_sw128(k_smem, 16);
+            const uint64_t vdesc0 = umma_desc_sw128(v_smem, CHUNK_BYTES);
+            const uint32_t desc_hi = (uint32_t)(qdesc0 >> 32);
+            const uint32_t q_lo = (uint32_t)qdesc0, k_lo = (uint32_t)kdesc0, v_lo = (uint32_t)vdesc0;
+            const int ksteps = (D + 15) / 16;              // zero-filled k-steps are skipped
+            auto issue_qk = [&](uint32_t g, int grp) {     // S_grp = Q_grp K(g)^T
+                const uint32_t kd = k_lo + (((g % kCkStages) * TILE_BYTES) >> 4);
+                const uint32_t qd = q_lo + ((grp * TILE_BYTES) >> 4);
+                const uint32_t d = tmem + COL_S + 128u * grp;
+#pragma unroll
+                for (int kk = 0; kk < HD / 16; ++kk) {
+                    const uint32_t off = (uint32_t)(((kk / 4) * CHUNK_BYTES + (kk % 4) * 32) >> 4);
+                    if (kk == 0) tc_mma_ss_i<false>(d, qd + off, kd + off, desc_hi, IDESC_QK);
+                    else if (kk < ksteps) tc_mma_ss_i<true>(d, qd + off, kd + off, desc_hi, IDESC_QK);
+                }
+                tc_commit(B_SFULL + 8 * grp);
+            };
+            auto issue_pv = [&](uint32_t g, int grp, bool accumulate) {   // O_grp (+)= P_grp V(g)
+                const uint32_t vd = v_lo + (((g % kCkStages) * TILE_BYTES) >> 4);
+                const uint32_t pbase = tmem + COL_S + 128u * grp, d = tmem + COL_O + 128u * grp;
+                if (accumulate) tc_mma_ts_i<true>(d, pbase, vd, desc_hi, IDESC_PV);
+                else tc_mma_ts_i<false>(d, pbase, vd, desc_hi, IDESC_PV);
+#pragma unroll
+                for (int kk = 1; kk < kCkKeys / 16; ++kk)
+                    tc_mma_ts_i<true>(d, pbase + kk * 8, vd + (uint32_t)((kk * 2048) >> 4), desc_hi, IDESC_PV);
+            };
+            for (; ok; ++it) {
+                if (!queue_wait(it)) { ok = false; break; }
+                const volatile int* d = queue + (it & 3) * kCkDesc;
+                const int r = d[0], nt = d[4], two = d[6];
+                mbar_arrive(B_WE + 8 * (it & 3));
+                if (r < 0) break;
+                if (!mbar_wait(B_QFULL, it & 1, bt.status) ||
+                    !mbar_wait(B_KFULL + 8 * (gt % kCkStages), (gt / kCkStages) & 1, bt.status)) { ok = false; break; }
+                tc_fence_after();
+                issue_qk(gt, 0);
+                if (two) issue_qk(gt, 1);
+                tc_commit(B_KEMPTY + 8 * (gt % kCkStages));
+                if (nt == 1) tc_commit(B_QEMPTY);
+                for (int t = 0; t < nt && ok; ++t, ++gt) {
+                    const bool more = t + 1 < nt;
+                    const uint32_t vs = gt % kCkStages, ks1 = (gt + 1) % kCkStages;
+                    // operand tiles first (they land long before P does)
+                    if (!mbar_wait(B_VFULL + 8 * vs, (gt / kCkStages) & 1, bt.status) ||
+                        (more && !mbar_wait(B_KFULL + 8 * ks1, ((gt + 1) / kCkStages) & 1, bt.status))) { ok = false; break; }
+#pragma unroll
+                    for (int grp = 0; grp < 2; ++grp) {
+                        if (grp == 1 && !two) break;
+                        if (!mbar_wait(B_PFULL + 8 * grp, (grp ? gb : gt) & 1, bt.status)) { ok = false; break; }
+                        tc_fence_after();
+                        issue_pv(gt, grp, t > 0);
+                        if (!more) tc_commit(B_OFULL + 8 * grp);
+                        if (grp == two) tc_commit(B_VEMPTY + 8 * vs);       // every tile has consumed V(g)
+                        if (more) {
+                            issue_qk(gt + 1, grp);
+                            if (grp == two) {
+                                tc_commit(B_KEMPTY + 8 * ks1);
+                                if (t + 2 == nt) tc_commit(B_QEMPTY);       // last score products of the item issued
+                            }
+                        }
+                    }
+                    gb += two;
+                }
+            }
+            // every product issued has completed before tensor memory is freed
+            tc_commit(B_DONE);
+            mbar_wait(B_DONE, 0, bt.status);
+        }
+    }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+        // ------------------------------ softmax / output rows ------------------------------
+        const int quad = warp & 3, grp = warp >> 2;
+        const int row = quad * 32 + lane;          // row of the tile = lane of tensor memory
+        const uint32_t lane_sel = (uint32_t)(quad * 32) << 16;
+        const uint32_t s_addr = tmem + lane_sel + COL_S + 128u * grp;
+        const uint32_t o_addr = tmem + lane_sel + COL_O + 128u * grp;
+        const uint32_t b_sfull = B_SFULL + 8 * grp, b_pfull = B_PFULL + 8 * grp, b_ofull = B_OFULL + 8 * grp;
+        const int ql = row / G, g = row % G;
+        uint32_t gt = 0, si = 0;   // tiles and items of this group (barrier phases); group A's tiles are the CTA's
+        bool ok = true;            // kept warp-uniform: a wait that ran out for any lane stops the warp
+        for (uint32_t qk = 0; ok; ++qk) {
+            ok = __all_sync(0xffffffffu, queue_wait(qk));
+            if (!ok) break;
+            const volatile int* d = queue + (qk & 3) * kCkDesc;
+            const int r = d[0], kvh = d[1], p = d[2], kt = d[3], nt = d[4], slot = d[5], two = d[6];
+            PagedRequest q;
+            q.start = d[7]; q.n = d[8]; q.pos0 = d[9]; q.keys = d[10];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(B_WE + 8 * (qk & 3));
+            if (r < 0) break;
+            if (grp > two) continue;               // the block of queries fits tile A
+            const int i0 = p * a.line.QB;
+            const int qi = i0 + grp * a.QT + ql;
+            const bool row_valid = ql < a.QT && qi < q.n;
+            // rows without a query take the bounds of the last one, so that they never hold up their warp
+            int lo_row, hi_row;
+            paged_key_range(bt, q, qi < q.n ? qi : q.n - 1, lo_row, hi_row);
+            // item-wide bounds: a tile outside them holds keys that not every query sees
+            int lo_first, hi_first, lo_last, hi_last;
+            paged_key_range(bt, q, i0, lo_first, hi_first);
+            paged_key_range(bt, q, (i0 + a.line.QB < q.n ? i0 + a.line.QB : q.n) - 1, lo_last, hi_last);
+            float m_ref = kLow, l_run = 0.0f;      // m_ref: the reference P and O are scaled by
+
+            for (int t = 0; t < nt; ++t, ++gt) {
+                ok = __all_sync(0xffffffffu, ok && mbar_wait(b_sfull, gt & 1, bt.status));
+                if (!ok) continue;
+                tc_fence_after();
+                uint32_t sv[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld32(sv[c], s_addr + c * 32);
+                const int kstart = (kt + t) * kCkKeys;
+                const int lo = lo_row - kstart, hi = hi_row - kstart;   // attended columns [lo, hi)
+                const bool all_in = __all_sync(0xffffffffu, lo <= 0 && hi >= kCkKeys);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tc_wait_ld_dep(sv[c]);
+                // ---- row maximum of the raw scores (the scale is positive) ----
+                float mx;
+                {
+                    float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;   // independent chains
+                    if (all_in) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+#pragma unroll
+                            for (int j = 0; j < 32; j += 8) {
+                                m0 = fmax3(m0, __uint_as_float(sv[c][j]), __uint_as_float(sv[c][j + 1]));
+                                m1 = fmax3(m1, __uint_as_float(sv[c][j + 2]), __uint_as_float(sv[c][j + 3]));
+                                m2 = fmax3(m2, __uint_as_float(sv[c][j + 4]), __uint_as_float(sv[c][j + 5]));
+                                m3 = fmax3(m3, __uint_as_float(sv[c][j + 6]), __uint_as_float(sv[c][j + 7]));
+                            }
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                const int col = c * 32 + j;
+                                const float sc = (col >= lo && col < hi) ? __uint_as_float(sv[c][j]) : -INFINITY;
+                                sv[c][j] = __float_as_uint(sc);
+                                m0 = fmaxf(m0, sc);
+                            }
+                    }
+                    mx = fmaxf(fmax3(m0, m1, m2), m3);
+                }
+                mx *= a.t.scale_log2;
+                const bool move = mx > m_ref + 8.0f;
+                if (__any_sync(0xffffffffu, move)) {
+                    const float m_to = move ? mx : m_ref;
+                    const float alpha = ex2_approx(m_ref - m_to);   // 1 for rows that keep their reference
+                    // the score product of this tile was issued after P V of the previous one: O is complete up to t-1
+                    if (t > 0) tmem_scale_columns(o_addr, HD / 32, alpha);
+                    l_run *= alpha;
+                    m_ref = m_to;
+                }
+                // ---- p = 2^(s*scale - m_ref), row sum, P back to tensor memory ----
+                float lsum0 = 0.0f, lsum1 = 0.0f, lsum2 = 0.0f, lsum3 = 0.0f;
+                const float neg_m = -m_ref;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        float x0, x1, x2, x3;
+                        ffma2_bcast(x0, x1, __uint_as_float(sv[c][j]), __uint_as_float(sv[c][j + 1]), a.t.scale_log2, neg_m);
+                        ffma2_bcast(x2, x3, __uint_as_float(sv[c][j + 2]), __uint_as_float(sv[c][j + 3]), a.t.scale_log2, neg_m);
+                        float p0, p1, p2, p3;
+                        if (((j / 4) * 2) % 8 < kCkEmuOf8) ex2_emu2_nan(p0, p1, x0, x1);
+                        else { p0 = ex2_approx(x0); p1 = ex2_approx(x1); }
+                        if (((j / 4) * 2 + 1) % 8 < kCkEmuOf8) ex2_emu2_nan(p2, p3, x2, x3);
+                        else { p2 = ex2_approx(x2); p3 = ex2_approx(x3); }
+                        fadd2_acc(lsum0, lsum1, p0, p1);
+                        fadd2_acc(lsum2, lsum3, p2, p3);
+                        pk[j / 2] = pack2<T>(p0, p1);
+                        pk[j / 2 + 1] = pack2<T>(p2, p3);
+                    }
+                    tmem_st16(s_addr + c * 16, pk);    // over the scores, all of which are in registers
+                }
+                tc_wait_st();
+                l_run += (lsum0 + lsum1) + (lsum2 + lsum3);
+                // Tiles that not every query of the item sees whole: group A zeroes the V rows that none attends and drops
+                // values that are not finite from the others (0 * NaN), before its arrival, which precedes both output products.
+                if (grp == 0 && (kstart < lo_last || kstart + kCkKeys > hi_first)) {
+                    const uint32_t vs = gt % kCkStages;
+                    ok = __all_sync(0xffffffffu, mbar_wait(B_VFULL + 8 * vs, (gt / kCkStages) & 1, bt.status));
+                    if (!ok) continue;
+                    uint8_t* vt = v_gen + (size_t)vs * TILE_BYTES;
+                    const int head = lo_last - kstart < 0 ? 0 : (lo_last - kstart < kCkKeys ? lo_last - kstart : kCkKeys);
+                    int tail = hi_first - kstart < 0 ? 0 : (hi_first - kstart < kCkKeys ? hi_first - kstart : kCkKeys);
+                    if (tail < head) tail = head;
+                    bool bad = false;
+                    for (int idx = tid; idx < (head + kCkKeys - tail) * 8 * NCH; idx += 128) {
+                        const int k = idx / (8 * NCH), u = idx % (8 * NCH);
+                        const int vr = k < head ? k : tail + k - head, pos = kstart + vr;
+                        uint4* at = reinterpret_cast<uint4*>(vt + (u / 8) * CHUNK_BYTES + vr * 128 + (u % 8) * 16);
+                        uint4 x = make_uint4(0, 0, 0, 0);
+                        if (pos >= lo_first && pos < hi_last) {
+                            x = *at;
+                            if (!drop_nonfinite<T>(x)) continue;
+                            bad = true;
+                        }
+                        *at = x;
+                    }
+                    if (__any_sync(0xffffffffu, bad) && lane == 0) a.fix.push(r, p, kvh);
+                    fence_proxy_async_smem();
+                }
+                tc_fence_before();
+                mbar_arrive(b_pfull);
+            }
+            // the item's last P V of this tile, then the row goes out
+            ok = __all_sync(0xffffffffu, ok && mbar_wait(b_ofull, si & 1, bt.status));
+            ++si;
+            if (!ok) continue;
+            tc_fence_after();
+            const float inv = l_run == 0.0f ? 0.0f : (l_run < kSumLimit ? 1.0f / l_run : NAN);
+            float* prow = slot >= 0 ? a.part + ((long long)slot * (2 * kCkRows) + grp * kCkRows + row) * (D + 4) : nullptr;
+            T* op = (T*)a.t.out + ((long long)(q.start + qi) * H + (long long)kvh * G + g) * D;
+#pragma unroll
+            for (int c = 0; c < HD / 32; ++c) {
+                uint32_t v[32];
+                tmem_ld32(v, o_addr + c * 32);
+                tc_wait_ld_dep(v);
+                if (c * 32 >= D || !row_valid) continue;   // columns of zeros (head_dim 96); rows without a query
+                if (prow) {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4)
+                        *reinterpret_cast<uint4*>(prow + c * 32 + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8) {
+                        uint4 w;
+                        w.x = pack2<T>(__uint_as_float(v[j]) * inv, __uint_as_float(v[j + 1]) * inv);
+                        w.y = pack2<T>(__uint_as_float(v[j + 2]) * inv, __uint_as_float(v[j + 3]) * inv);
+                        w.z = pack2<T>(__uint_as_float(v[j + 4]) * inv, __uint_as_float(v[j + 5]) * inv);
+                        w.w = pack2<T>(__uint_as_float(v[j + 6]) * inv, __uint_as_float(v[j + 7]) * inv);
+                        *reinterpret_cast<uint4*>(op + c * 32 + j) = w;
+                    }
+                }
+            }
+            if (prow && row_valid) *reinterpret_cast<float2*>(prow + D) = make_float2(m_ref, l_run);
+            tc_fence_before();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) tmem_dealloc(tmem, TMEM_COLS);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Merge of the items that were cut, one warp per row: blockIdx.x = the CTA whose entry names an item, blockIdx.y = a
+// share of its rows. `tiles` tiles of 128 rows per item.
+// ---------------------------------------------------------------------------------------------------------------------
+struct PagedChunkMergeArgs {
+    PagedBatch b;
+    const float* part;
+    const int4* cuts;
+    void* out;
+    int H, KVH, HD, QT, QB, tiles;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) hkv_paged_chunk_merge_kernel(const PagedChunkMergeArgs a) {
+    const int4 cut = a.cuts[blockIdx.x];
+    const int parts = cut.w;
+    if (parts <= 1) return;
+    const PagedRequest q = paged_request(a.b, cut.x);
+    const int G = a.H / a.KVH, HD = a.HD, PW = HD + 4, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int row = blockIdx.y * 8 + warp; row < a.tiles * 128; row += gridDim.y * 8) {
+        const int ql = row % 128 / G, i = cut.z * a.QB + row / 128 * a.QT + ql;
+        if (ql >= a.QT || i >= q.n) continue;
+        // part 0 sits in this CTA's second slot, the others in the first slots of the CTAs behind it
+        const float* base = a.part + (long long)row * PW;
+        const long long set = (long long)a.tiles * 128 * PW;
+        float M = kLow, L = 0.0f;
+        float2 acc[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = make_float2(0.0f, 0.0f);
+        for (int p0 = 0; p0 < parts; p0 += 2) {
+            float2 ml[2], x[2][4];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int pt = p0 + u;
+                const float* r = base + (2ll * (blockIdx.x + pt) + (pt == 0 ? 1 : 0)) * set;
+                ml[u] = pt < parts ? *reinterpret_cast<const float2*>(r + HD) : make_float2(kLow, 0.0f);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int d = 2 * lane + 64 * e;
+                    x[u][e] = pt < parts && d < HD ? *reinterpret_cast<const float2*>(r + d) : make_float2(0.0f, 0.0f);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const float Mn = fmaxf(M, ml[u].x), keep = exp2f(M - Mn), w = exp2f(ml[u].x - Mn);
+                L = fmaf(ml[u].y, w, L * keep);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    acc[e].x = fmaf(x[u][e].x, w, acc[e].x * keep);
+                    acc[e].y = fmaf(x[u][e].y, w, acc[e].y * keep);
+                }
+                M = Mn;
+            }
+        }
+        const float inv = L == 0.0f ? 0.0f : (L < kSumLimit ? 1.0f / L : NAN);
+        T* op = (T*)a.out + ((long long)(q.start + i) * a.H + (long long)cut.y * G + row % 128 % G) * HD;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int d = 2 * lane + 64 * e;
+            if (d < HD) *reinterpret_cast<uint32_t*>(op + d) = pack2<T>(acc[e].x * inv, acc[e].y * inv);
+        }
+    }
+}
+
+}  // namespace hkv

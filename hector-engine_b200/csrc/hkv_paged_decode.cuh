@@ -7,7 +7,7 @@
 //     every CTA does the same number of tiles whatever the lengths. The lengths are read on the device.
 //   * One producer warp fills a ring of stages with bulk-tensor copies. A tile is 64 / min(page, 64) pieces, each a box
 //     of min(page, 64) rows of one page; the lanes look up one page each and issue their boxes side by side, so a tile of
-//     small pages costs no more issue time than one box. Positions behind the last key and entries outside the planes are
+//     small pages costs no more issue time than one box. Positions that no query looks at and entries outside the planes are
 //     fetched from a coordinate behind the tensor: the copy engine writes zeros and reads nothing.
 //   * Four consumer warps per tile, 16 rows each:  S^T = K Q^T  and  O^T += V^T P^T  with mma.m16n8k16, the query rows in
 //     N (8 or 16), K and V by ldmatrix, P^T from the score fragment by movmatrix; softmax over rows by shuffles, with a
@@ -35,7 +35,7 @@ struct PagedDecodeArgs {
     PagedAttnArgs t;
     float* part;          // [2 * spans][KVH][cols][HD + 2]: o, maximum (log2 domain), sum
     int4* cuts;           // [spans]: request that starts in this span and goes on behind it: {request, spans, -, -}; spans 0: none
-    int* fix;             // [max_requests]: set where a value that is not finite was hidden from some queries of a request
+    PagedFix fix;
     int gang, cols;       // cols = query rows per KV head that the partial rows hold
     int box_rows, pieces; // rows of a box, boxes per tile and column block
 };
@@ -195,9 +195,10 @@ hkv_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                 const int nt = nb - off < u1 - u ? nb - off : u1 - u;
                 u += nt;
                 const PagedRequest q = paged_request(bt, r);
-                int tile_lo, n_tiles, lo, hi;
+                int tile_lo, n_tiles, lo, hi, x_;
                 paged_tiles(bt, q, tile_lo, n_tiles);
-                paged_key_range(bt, q, q.n - 1, lo, hi);
+                paged_key_range(bt, q, 0, lo, x_);
+                paged_key_range(bt, q, q.n - 1, x_, hi);
                 const int32_t* table = bt.table + (long long)r * bt.cols;
                 for (int t = 0; t < nt; ++t) {
                     if (round > 0) ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * stage, (uint32_t)(round - 1) & 1u, bt.status));
@@ -211,7 +212,7 @@ hkv_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                         const int piece = x % a.pieces, c = x / a.pieces % NCH, kv = x / (a.pieces * NCH);
                         const int p = pos0 + piece * a.box_rows;
                         int pg = bt.pages;            // behind the tensor: zeros
-                        if (p < hi) {
+                        if (p < hi && p + a.box_rows > lo) {
                             pg = __ldg(table + (p >> page_shift));
                             if (pg < 0 || pg >= bt.pages) {
                                 atomicOr(bt.status, kStatusBoundCheck);
@@ -327,7 +328,7 @@ hkv_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                             touched = true;
                         }
                     }
-                    if (bad) a.fix[r] = 1;
+                    if (__any_sync(0xffffffffu, bad) && lane == 0) a.fix.push(r, -1, kvh);
                     if (__any_sync(0xffffffffu, touched)) fence_proxy_async_smem();
                     __syncwarp();
                 }

@@ -55,72 +55,6 @@ __host__ __device__ inline int prefill_span_owner(long long x, long long W, int 
     return (int)(((x + 1) * grid + W - 1) / W - 1);
 }
 
-// tcgen05.wait::ld that also names the registers of the load it completes, so that no use of
-// them can be scheduled above the wait.
-__device__ __forceinline__ void tc_wait_ld_dep(uint32_t (&v)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
-                   "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]),
-                   "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]),
-                   "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
-                 :
-                 : "memory");
-}
-
-// 2^x for two values on the FMA pipe (the MUFU pipe is the narrowest unit of the softmax: 16
-// ex2 per clock per SM). x is clamped to [-100, +inf); callers keep x <= ~9. Round-to-nearest
-// split x = n + f, f in [-0.5, 0.5], by adding 1.5*2^23; 2^f by a degree-3 minimax polynomial
-// (max relative error 7.5e-5, below half an ulp of the fp16 the result is rounded to); 2^n by
-// adding n to the exponent field.
-__device__ __forceinline__ void ex2_emu2(float& p0, float& p1, float x0, float x1) {
-    x0 = fmaxf(x0, -100.0f);
-    x1 = fmaxf(x1, -100.0f);
-    uint32_t t0, t1, q0, q1;
-    asm("{\n\t.reg .b64 rx, rt, rr, rf, rp, rc;\n\t"
-        "mov.b64 rx, {%4, %5};\n\t"
-        "mov.b64 rc, {0f4B400000, 0f4B400000};\n\t"      // 12582912.0
-        "add.rn.f32x2 rt, rx, rc;\n\t"                    // n in the low mantissa bits
-        "sub.rn.f32x2 rr, rt, rc;\n\t"                    // n as a float
-        "sub.rn.f32x2 rf, rx, rr;\n\t"                    // f = x - n
-        "mov.b64 rp, {0f3D61FB59, 0f3D61FB59};\n\t"      // 0.055171344
-        "mov.b64 rc, {0f3E786ED8, 0f3E786ED8};\n\t"      // 0.24261034
-        "fma.rn.f32x2 rp, rp, rf, rc;\n\t"
-        "mov.b64 rc, {0f3F31798D, 0f3F31798D};\n\t"      // 0.69326097
-        "fma.rn.f32x2 rp, rp, rf, rc;\n\t"
-        "mov.b64 rc, {0f3F7FFB4A, 0f3F7FFB4A};\n\t"      // 0.9999281
-        "fma.rn.f32x2 rp, rp, rf, rc;\n\t"
-        "mov.b64 {%0, %1}, rt;\n\t"
-        "mov.b64 {%2, %3}, rp;\n\t}"
-        : "=r"(t0), "=r"(t1), "=r"(q0), "=r"(q1)
-        : "f"(x0), "f"(x1));
-    p0 = __uint_as_float(q0 + (t0 << 23));
-    p1 = __uint_as_float(q1 + (t1 << 23));
-}
-
-// MMA wrappers for the issuing thread's inner loops: the accumulate flag is an immediate and the
-// 64-bit shared-memory descriptors are passed as (low, high) words — every descriptor of this kernel
-// has the same high word (8-row group stride 1024 B, version, 128-byte swizzle), and the low word
-// (start address, leading-dimension offset) moves by a compile-time constant per instruction, so
-// the loop costs one 32-bit add per operand instead of 64-bit descriptor arithmetic.
-template <bool ACC>
-__device__ __forceinline__ void tc_mma_ss_i(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t desc_hi, uint32_t idesc) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %5, 0;\n\t"
-        "mov.b64 da, {%1, %3};\n\tmov.b64 db, {%2, %3};\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t}"
-        ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "n"(ACC ? 1 : 0)
-        : "memory");
-}
-template <bool ACC>
-__device__ __forceinline__ void tc_mma_ts_i(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t desc_hi, uint32_t idesc) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %5, 0;\n\t"
-        "mov.b64 db, {%2, %3};\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}"
-        ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(desc_hi), "r"(idesc), "n"(ACC ? 1 : 0)
-        : "memory");
-}
-
 template <int HD>
 __global__ void __launch_bounds__(kPf2Threads, 1)
 hkv_prefill_tc2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,

@@ -93,7 +93,7 @@ def attend_model(torch, q, k_plane, v_plane, table, q_start, step, keys, scale, 
         K, V = k_plane[pg, j % page].double(), v_plane[pg, j % page].double()      # [L, KVH, HD]
         K, V = K.repeat_interleave(G, 1), V.repeat_interleave(G, 1)
         x = q[at0:at0 + m].double()
-        pos = int(keys[r]) - n + torch.arange(m, device=q.device)
+        pos = L - n + torch.arange(m, device=q.device)
         seen = torch.ones(m, L, dtype=torch.bool, device=q.device)
         if causal:
             seen = j[None] <= pos[:, None]
