@@ -15,6 +15,7 @@
 #include "hkv_paged_chunk.cuh"
 #include "hkv_paged_decode.cuh"
 #include "hkv_paged_rope.cuh"
+#include "hkv_paged_wide.cuh"
 
 using namespace hkv;
 
@@ -243,14 +244,23 @@ int launch_small(hkv_paged_ctx* c, const PagedAttnArgs& t, int cols, cudaStream_
 
 // ---- prompt chunks ----
 int staged_hd(int hd) { return hd == 96 ? 128 : hd; }
-bool chunk_geometry(const hkv_paged_geometry& g) { return g.head_dim != 256; }
+bool wide(const hkv_paged_geometry& g) { return g.head_dim == kWdHD; }    // one query tile per item, keys by 64
+// Queries per item of the prompt kernels.
+int block_queries(const hkv_paged_geometry& g) { return (wide(g) ? 1 : 2) * (kCkRows / (g.num_heads / g.num_kv_heads)); }
+size_t chunk_smem(const hkv_paged_geometry& g, int requests) {
+    return wide(g) ? wide_smem_bytes(requests) : chunk_smem_bytes(staged_hd(g.head_dim), requests);
+}
 
 typedef void (*ChunkKernel)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const PagedChunkArgs);
 ChunkKernel pick_chunk(int dtype, int hd) {
     if (dtype == HKV_DTYPE_F16) return staged_hd(hd) == 64 ? hkv_paged_chunk_kernel<__half, 64> : hkv_paged_chunk_kernel<__half, 128>;
     return staged_hd(hd) == 64 ? hkv_paged_chunk_kernel<__nv_bfloat16, 64> : hkv_paged_chunk_kernel<__nv_bfloat16, 128>;
 }
-size_t chunk_part_bytes(const hkv_paged_geometry& g, int sm_count) { return 2ull * sm_count * 2 * kCkRows * (g.head_dim + 4) * sizeof(float); }
+const void* chunk_kernel(const hkv_paged_geometry& g) {
+    if (wide(g)) return g.dtype == HKV_DTYPE_F16 ? (const void*)hkv_paged_wide_kernel<__half> : (const void*)hkv_paged_wide_kernel<__nv_bfloat16>;
+    return (const void*)pick_chunk(g.dtype, g.head_dim);
+}
+size_t chunk_part_bytes(const hkv_paged_geometry& g, int sm_count) { return 2ull * sm_count * (wide(g) ? 1 : 2) * kCkRows * (g.head_dim + 4) * sizeof(float); }
 
 // The line's table counts units of 128 << shift keys; the shift keeps the largest batch the context allows inside 31 bits.
 int line_shift(const hkv_paged_geometry& g, int QB) {
@@ -269,28 +279,34 @@ int launch_chunk(hkv_paged_ctx* c, const PagedAttnArgs& t, const void* q, bool s
     a.QT = kCkRows / G;
     a.line.G = G;
     a.line.KVH = g.num_kv_heads;
-    a.line.QB = 2 * a.QT;
-    a.line.keys = kCkKeys;
+    a.line.QB = block_queries(g);
+    a.line.keys = wide(g) ? kWdKeys : kCkKeys;
     a.line.shift = line_shift(g, a.line.QB);
     a.part = c->chunk_part;
     a.cuts = c->chunk_cuts;
     a.fix = fix_of(c);
-    a.box_rows = std::min(g.page_size, kCkKeys);
-    a.pieces = kCkKeys / a.box_rows;
+    a.box_rows = std::min(g.page_size, a.line.keys);
+    a.pieces = a.line.keys / a.box_rows;
     a.small = small ? 1 : 0;
     CUtensorMap mq, mk, mv;
-    const cuuint64_t dims[3] = {(cuuint64_t)g.head_dim, (cuuint64_t)g.num_heads, (cuuint64_t)t.b.tokens};
-    const cuuint64_t strides[2] = {(cuuint64_t)g.head_dim * 2, (cuuint64_t)t.q_stride * 2};
-    const cuuint32_t box[3] = {64u, (cuuint32_t)G, (cuuint32_t)a.QT}, one[3] = {1u, 1u, 1u};
-    const CUresult r = encode_tiled_fn()(
-        &mq, g.dtype == HKV_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q),
-        dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return fail(c, HKV_ERR_CUDA, "cuTensorMapEncodeTiled failed (queries)");
     int e = encode_plane(c, t.k_cache, 64, a.box_rows, &mk);
     if (!e) e = encode_plane(c, t.v_cache, 64, a.box_rows, &mv);
     if (e) return e;
-    pick_chunk(g.dtype, g.head_dim)<<<c->sm_count, kCkThreads, chunk_smem_bytes(staged_hd(g.head_dim), t.b.requests), st>>>(mq, mk, mv, a);
+    const size_t smem = chunk_smem(g, t.b.requests);
+    if (wide(g)) {
+        if (g.dtype == HKV_DTYPE_F16) hkv_paged_wide_kernel<__half><<<c->sm_count, kWdThreads, smem, st>>>(mk, mv, a);
+        else hkv_paged_wide_kernel<__nv_bfloat16><<<c->sm_count, kWdThreads, smem, st>>>(mk, mv, a);
+    } else {
+        const cuuint64_t dims[3] = {(cuuint64_t)g.head_dim, (cuuint64_t)g.num_heads, (cuuint64_t)t.b.tokens};
+        const cuuint64_t strides[2] = {(cuuint64_t)g.head_dim * 2, (cuuint64_t)t.q_stride * 2};
+        const cuuint32_t box[3] = {64u, (cuuint32_t)G, (cuuint32_t)a.QT}, one[3] = {1u, 1u, 1u};
+        const CUresult r = encode_tiled_fn()(
+            &mq, g.dtype == HKV_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q),
+            dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (r != CUDA_SUCCESS) return fail(c, HKV_ERR_CUDA, "cuTensorMapEncodeTiled failed (queries)");
+        pick_chunk(g.dtype, g.head_dim)<<<c->sm_count, kCkThreads, smem, st>>>(mq, mk, mv, a);
+    }
     PagedChunkMergeArgs m{};
     m.b = t.b;
     m.part = c->chunk_part;
@@ -301,7 +317,7 @@ int launch_chunk(hkv_paged_ctx* c, const PagedAttnArgs& t, const void* q, bool s
     m.HD = t.HD;
     m.QT = a.QT;
     m.QB = a.line.QB;
-    m.tiles = 2;
+    m.tiles = wide(g) ? 1 : 2;
     const dim3 grid((unsigned)c->sm_count, 8);
     if (g.dtype == HKV_DTYPE_F16) hkv_paged_chunk_merge_kernel<__half><<<grid, 256, 0, st>>>(m);
     else hkv_paged_chunk_merge_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(m);
@@ -370,12 +386,12 @@ int attention(hkv_paged_ctx* c, const void* q, int64_t q_token_stride, const voi
         return fail(c, HKV_ERR_ALIGNMENT, "attention: the staged kernels need 16-byte aligned tensors and strides");
     const bool only_small = (long long)max_step * G <= kSmallCols;
     // (the prompt kernel takes the row maximum before the scale, which it can for a positive one)
-    if (staged && (only_small || (chunk_geometry(g) && scale > 0.0f))) {
+    if (staged && (only_small || scale > 0.0f)) {
         const bool small = G <= kSmallCols;              // some step_len can be one of the few-token kernel's
         int e = HKV_OK;
         if (small) e = launch_small(c, a, std::min(kSmallCols, only_small ? max_step * G : kSmallCols / G * G), st);
         if (!e && !only_small) e = launch_chunk(c, a, q, small, st);
-        if (!e && max_step > 1) e = launch_fix(c, a, 2 * (kCkRows / G), st);   // (nothing is hidden from a single query)
+        if (!e && max_step > 1) e = launch_fix(c, a, block_queries(g), st);   // (nothing is hidden from a single query)
         return e;
     }
     const dim3 grid((unsigned)tokens, (unsigned)g.num_heads);
@@ -434,11 +450,10 @@ int hkv_paged_create(hkv_paged_ctx** out, const hkv_paged_geometry* geometry) {
                 if (e != cudaSuccess) return fail_cuda(c, e, "cudaFuncSetAttribute(shared memory)");
             }
         c->smem_optin = (size_t)optin - 1024;   // (the kernels hold a few hundred bytes of their own)
-        if (chunk_geometry(*geometry)) {
-            const size_t need = chunk_smem_bytes(staged_hd(geometry->head_dim), geometry->max_requests);
+        {
+            const size_t need = chunk_smem(*geometry, geometry->max_requests);
             if (need > c->smem_optin) return fail(c, HKV_ERR_TOO_LARGE, "shared memory too small for the request table");
-            e = cudaFuncSetAttribute((const void*)pick_chunk(geometry->dtype, geometry->head_dim),
-                                     cudaFuncAttributeMaxDynamicSharedMemorySize, optin - 1024);
+            e = cudaFuncSetAttribute(chunk_kernel(*geometry), cudaFuncAttributeMaxDynamicSharedMemorySize, optin - 1024);
             if (e != cudaSuccess) return fail_cuda(c, e, "cudaFuncSetAttribute(shared memory)");
             const size_t cb = chunk_part_bytes(*geometry, c->sm_count);
             if ((e = cudaMalloc(&c->chunk_part, cb)) != cudaSuccess) return fail_cuda(c, e, "cudaMalloc(partial rows)");
