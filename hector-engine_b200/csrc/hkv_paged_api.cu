@@ -330,6 +330,17 @@ int launch_fix(hkv_paged_ctx* c, const PagedAttnArgs& t, int QB, cudaStream_t st
     return launched(c, "attention launch");
 }
 
+template <typename T>
+void launch_rope(const MropeArgs& a, int lph, unsigned blocks, cudaStream_t st) {
+    switch (lph) {
+        case 4: hkv_paged_norm_rope_kernel<T, 4><<<blocks, kMropeThreads, 0, st>>>(a); break;
+        case 8: hkv_paged_norm_rope_kernel<T, 8><<<blocks, kMropeThreads, 0, st>>>(a); break;
+        case 16: hkv_paged_norm_rope_kernel<T, 16><<<blocks, kMropeThreads, 0, st>>>(a); break;
+        case 32: hkv_paged_norm_rope_kernel<T, 32><<<blocks, kMropeThreads, 0, st>>>(a); break;
+        default: hkv_paged_norm_rope_any_kernel<T><<<blocks, kMropeThreads, 0, st>>>(a); break;
+    }
+}
+
 // A token stride: 0 = dense, else at least one token's row.
 bool stride_ok(int64_t given, long long row, long long* out) {
     if (given != 0 && given < row) return false;
@@ -667,13 +678,21 @@ int hkv_paged_norm_rope(hkv_paged_ctx* c, const hkv_paged_rope* r, void* stream)
     a.eps = r->eps;
     const double scaling = r->scaling_factor > 0.0f ? (double)r->scaling_factor : 1.0;
     for (int i = 0; i < half; ++i) a.turns[i] = std::pow(r->theta, -2.0 * i / rot) / (scaling * 6.283185307179586476925);
-    // enough warps to fill the machine: a token is shared by several when there are few
-    const int heads = g.num_heads + 2 * g.num_kv_heads;
-    a.parts = (int)std::max<long long>(1, std::min<long long>(heads, (long long)c->sm_count * 16 / r->tokens));
+    // 16-byte pieces whose pair partner is a whole piece away; everything else goes element by element
+    bool pieces = g.head_dim % 16 == 0 && rot % 16 == 0 && a.q_stride % 8 == 0 && a.kv_stride % 8 == 0 && a.qo_stride % 8 == 0 &&
+                  a.ko_stride % 8 == 0;
+    for (const void* p : {a.q, a.k, a.v, (const void*)a.q_out, (const void*)a.k_out, a.q_w, a.k_w, (const void*)a.k_cache, (const void*)a.v_cache})
+        pieces = pieces && aligned(p, 16);
+    int lph = 4;                             // lanes per head
+    while (lph * 16 < g.head_dim) lph *= 2;
+    // enough warps to fill the machine: a token is shared by several, a round of heads each at least, when there are few
+    const int heads = g.num_heads + (cached ? 2 : 1) * g.num_kv_heads, rounds = pieces ? (heads + 32 / lph - 1) / (32 / lph) : heads;
+    a.parts = (int)std::max<long long>(1, std::min<long long>(rounds, (long long)c->sm_count * 16 / r->tokens));
     const long long units = (long long)r->tokens * a.parts;
     const unsigned blocks = (unsigned)std::min<long long>((units + kMropeWarps - 1) / kMropeWarps, (long long)c->sm_count * 8);
-    if (g.dtype == HKV_DTYPE_F16) hkv_paged_norm_rope_any_kernel<__half><<<blocks, kMropeThreads, 0, (cudaStream_t)stream>>>(a);
-    else hkv_paged_norm_rope_any_kernel<__nv_bfloat16><<<blocks, kMropeThreads, 0, (cudaStream_t)stream>>>(a);
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (g.dtype == HKV_DTYPE_F16) launch_rope<__half>(a, pieces ? lph : 0, blocks, st);
+    else launch_rope<__nv_bfloat16>(a, pieces ? lph : 0, blocks, st);
     return launched(c, "norm_rope launch");
 }
 
