@@ -105,13 +105,13 @@ __device__ __forceinline__ long long block_scan(long long v, long long* buf, lon
 }
 
 // ---- plan -----------------------------------------------------------------------------------------------------------
-// One thread-block cluster of up to 8 CTAs x 1024 threads. Every CTA scans all requests itself (at most four per
-// thread: cheaper than passing sums between CTAs) and leaves their starts, lengths and places on the free stack in
-// shared memory; after the cluster barrier — every CTA has read the state that the launch may update in place — each
-// CTA writes its share of the tables. A token finds its request by bisection over the starts in shared memory. New
-// block-table entries come from the free stack directly, so no CTA waits for another's table writes.
-// Bound: launch latency and two dependent trips to memory (lengths, then table or stack entries); the tables
-// themselves are some hundred KB at most.
+// One thread-block cluster of up to 8 CTAs. Every CTA scans all requests itself (at most four per thread: cheaper than
+// passing sums between CTAs) and leaves their starts, lengths and places on the free stack in shared memory; after the
+// cluster barrier — every CTA has read the state that the launch may update in place — each CTA writes its share of the
+// tables. A packed token finds its request by bisection over the starts, a new page by bisection over the places on the
+// stack, so both are dealt evenly and read and written in order whatever the lengths. New pages come from the stack
+// directly, so no CTA waits for another's table writes.
+// Bound: latency — the launch and three dependent trips to memory (lengths, then table or stack entry, then the store).
 struct PlanArgs {
     const int32_t *past, *fresh, *free_pages, *free_count;
     int32_t *table, *total, *step, *q_start, *slots, *positions, *free_left;
@@ -120,118 +120,169 @@ struct PlanArgs {
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanMaxCluster = 8;
 constexpr int kPagedMaxRequests = 4096;
-constexpr int kPlanPer = kPagedMaxRequests / kPlanThreads;   // requests per thread
+constexpr int kPlanPer = 4;           // requests per thread
 __host__ __device__ constexpr size_t plan_smem_bytes(int requests) { return (size_t)(3 * requests + 4) * 4; }
+
+// Exclusive prefix sum over the block, sums held at `cap` (min(a + b, cap) is associative for values up to cap <= 2^31).
+__device__ __forceinline__ uint32_t block_scan_cap(uint32_t v, const uint32_t cap, uint32_t* buf, uint32_t& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    uint32_t x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x = min(x + u, cap);
+    }
+    if (lane == 31) buf[warp] = x;
+    __syncthreads();
+    // every warp sums the warps before it on its own: one barrier, no second round
+    uint32_t w = lane < warps ? buf[lane] : 0u;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t u = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) w = min(w + u, cap);
+    }
+    total = __shfl_sync(0xffffffffu, w, 31);
+    uint32_t before = __shfl_sync(0xffffffffu, w, warp > 0 ? warp - 1 : 0);
+    if (warp == 0) before = 0;
+    const uint32_t left = __shfl_up_sync(0xffffffffu, x, 1);
+    return min(before + (lane > 0 ? left : 0u), cap);
+}
+// The last index r in [0, n) with key[r] <= x (key[0] <= x), for U values at a time: their dependent reads overlap.
+template <int U>
+__device__ __forceinline__ void last_at_most(const int32_t* key, const int n, const int (&x)[U], int (&r)[U]) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) r[u] = 0;
+    int step = 1;
+    while (step < n) step <<= 1;
+    for (step >>= 1; step > 0; step >>= 1)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (r[u] + step < n && key[r[u] + step] <= x[u]) r[u] += step;
+}
 
 __global__ void __launch_bounds__(kPlanThreads, 1) hkv_paged_plan_kernel(const PlanArgs a) {
     namespace cg = cooperative_groups;
     extern __shared__ int32_t plan_smem[];
-    __shared__ long long buf[33];
-    int32_t* s_start = plan_smem;                    // [R + 1]
-    int32_t* s_past = s_start + a.requests + 1;      // [R]
-    int32_t* s_take = s_past + a.requests;           // [R] pages taken off the stack before this request, -1: not admitted
-    const int R = a.requests, tid = threadIdx.x;
-    const int per = (R + kPlanThreads - 1) / kPlanThreads;
-    const int r0 = tid * per;
+    __shared__ uint32_t buf[2][32];
+    __shared__ uint32_t s_taken;                     // pages taken by all admitted requests
+    const int R = a.requests, tid = threadIdx.x, threads = blockDim.x;
+    int32_t* s_start = plan_smem;                    // [R + 1] first packed row
+    int32_t* s_take = s_start + R + 1;               // [R + 1] pages wanted before this request, as far as they are taken
+    int32_t* s_past = s_take + R + 1;                // [R] past length; -1: not admitted
+    if (tid == 0) s_taken = 0;
+    const int per = (R + threads - 1) / threads, r0 = tid * per;
+    const uint32_t cap = (uint32_t)a.tokens + 1u;    // beyond the packed rows: further ones do not matter
     int past[kPlanPer], fresh[kPlanPer];
-    long long sum = 0;
+    uint32_t sum = 0;
 #pragma unroll
     for (int i = 0; i < kPlanPer; ++i) {
         past[i] = fresh[i] = 0;
         if (i < per && r0 + i < R) {
             past[i] = a.past[r0 + i];
             fresh[i] = a.fresh[r0 + i];
-            sum += fresh[i] > 0 ? fresh[i] : 0;
+            sum = min(sum + min((uint32_t)(fresh[i] > 0 ? fresh[i] : 0), cap), cap);
         }
     }
     const int count = *a.free_count, avail = count < a.pages ? count : a.pages;
-    long long tokens_all, need_all;
-    long long at = block_scan(sum, buf, tokens_all);
-    long long need[kPlanPer], need_sum = 0;
+    uint32_t tokens_all, need_all;
+    uint32_t at = block_scan_cap(sum, cap, buf[0], tokens_all);
+    uint32_t need[kPlanPer], need_sum = 0;
+    bool fits[kPlanPer];
 #pragma unroll
     for (int i = 0; i < kPlanPer; ++i) {
-        need[i] = -1;                                // not admitted
+        need[i] = 0;
+        fits[i] = false;
         if (i < per && r0 + i < R) {
-            s_start[r0 + i] = (int)(at < a.tokens ? at : a.tokens);
-            s_past[r0 + i] = past[i];
-            const long long end = at + (fresh[i] > 0 ? fresh[i] : 0);
+            s_start[r0 + i] = (int)min(at, (uint32_t)a.tokens);
+            const uint32_t end = min(at + min((uint32_t)(fresh[i] > 0 ? fresh[i] : 0), cap), cap);
             const long long len = (long long)past[i] + fresh[i];
-            if (past[i] >= 0 && fresh[i] >= 0 && len <= (long long)a.cols * a.page && end <= a.tokens) {
-                need[i] = (len + a.page - 1) / a.page - ((long long)past[i] + a.page - 1) / a.page;
-                need_sum += need[i];
-            }
+            fits[i] = past[i] >= 0 && fresh[i] >= 0 && len <= (long long)a.cols * a.page && end <= (uint32_t)a.tokens;
+            if (fits[i]) need[i] = (uint32_t)((len + a.page - 1) / a.page - ((long long)past[i] + a.page - 1) / a.page);
+            need_sum += need[i];                     // at most tokens / page + requests in all
             at = end;
         }
     }
-    if (tid == 0) s_start[R] = (int)(tokens_all < a.tokens ? tokens_all : a.tokens);
-    long long before = block_scan(need_sum, buf, need_all);
-    long long taken = 0;                             // of this thread's admitted requests
+    uint32_t before = block_scan_cap(need_sum, 0x7fffffffu, buf[1], need_all);
+    // A request that wants pages gets them if all wanted up to and including it are there; those admitted are the first
+    // ones that want any, so what they take is the largest such sum.
 #pragma unroll
     for (int i = 0; i < kPlanPer; ++i) {
         if (i < per && r0 + i < R) {
-            const bool ok = need[i] == 0 || (need[i] > 0 && before + need[i] <= avail);
-            s_take[r0 + i] = ok ? (int)before : -1;
-            if (need[i] > 0) {
-                if (ok) taken += need[i];
-                before += need[i];
-            }
+            const bool ok = fits[i] && (need[i] == 0 || (long long)before + need[i] <= avail);
+            s_take[r0 + i] = (int)before;
+            s_past[r0 + i] = ok ? past[i] : -1;
+            before += need[i];
+            if (ok && need[i] > 0) atomicMax(&s_taken, before);
         }
     }
-    // `before` of a request that needs no page may exceed `avail`; it takes none, so its value is only a mark
-    long long taken_all;
-    block_scan(taken, buf, taken_all);               // (also orders the shared-memory tables)
-
+    if (tid == 0) {
+        s_start[R] = (int)min(tokens_all, (uint32_t)a.tokens);
+        s_take[R] = (int)need_all;
+    }
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
-    cluster.sync();                                  // past, new and the count are read everywhere: state may change
+    if (ctas > 1) cluster.sync();                    // past, new and the count are read everywhere: state may change
+    else __syncthreads();
 
-    auto new_len = [&](int r) { return s_take[r] >= 0 ? a.fresh[r] : 0; };
-    // per-request outputs and new block-table entries
-    for (int r = rank * kPlanThreads + tid; r < R; r += ctas * kPlanThreads) {
-        const int n = new_len(r), p = s_past[r];
-        a.q_start[r] = s_start[r];
-        a.step[r] = n;
-        a.total[r] = p + n;
-        if (n > 0) {
-            const int j0 = (p + a.page - 1) / a.page, j1 = (p + n + a.page - 1) / a.page;
-            const int top = avail - 1 - s_take[r];   // stack entry of the request's first new page
-            if (j1 - j0 <= 32)
-                for (int j = j0; j < j1; ++j) a.table[(long long)r * a.cols + j] = a.free_pages[top - (j - j0)];
+    const int taken = (int)s_taken, gsize = ctas * threads, g = rank * threads + tid;
+    if (rank == 0) {
+        // every thread still holds its requests' lengths
+#pragma unroll
+        for (int i = 0; i < kPlanPer; ++i) {
+            if (i < per && r0 + i < R) {
+                const int n = s_past[r0 + i] >= 0 ? fresh[i] : 0;
+                a.q_start[r0 + i] = s_start[r0 + i];
+                a.step[r0 + i] = n;
+                a.total[r0 + i] = past[i] + n;
+            }
+        }
+        if (tid == 0) {
+            a.q_start[R] = s_start[R];
+            *a.free_left = avail - taken;
         }
     }
-    if (rank == 0 && tid == 0) {
-        a.q_start[R] = s_start[R];
-        *a.free_left = (int)(avail - taken_all);
-    }
-    // requests that open many pages: a warp each
-    const int warp = tid >> 5, lane = tid & 31;
-    for (int r = rank * 32 + warp; r < R; r += ctas * 32) {
-        const int n = new_len(r), p = s_past[r];
-        if (n <= 0) continue;
-        const int j0 = (p + a.page - 1) / a.page, j1 = (p + n + a.page - 1) / a.page;
-        if (j1 - j0 <= 32) continue;
-        const int top = avail - 1 - s_take[r];
-        for (int j = j0 + lane; j < j1; j += 32) a.table[(long long)r * a.cols + j] = a.free_pages[top - (j - j0)];
+    constexpr int U = 4;
+    // new block-table entries: the j-th page off the stack
+    for (int j0 = g; j0 < taken; j0 += U * gsize) {
+        int x[U], r[U], pg[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            x[u] = j0 + u * gsize;
+            pg[u] = x[u] < taken ? a.free_pages[avail - 1 - x[u]] : 0;
+        }
+        last_at_most<U>(s_take, R, x, r);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (x[u] < taken) {
+                const int p = s_past[r[u]];          // (an admitted request: only those hold places below `taken`)
+                a.table[(long long)r[u] * a.cols + (p + a.page - 1) / a.page + x[u] - s_take[r[u]]] = pg[u];
+            }
     }
     // slot and position of every packed token
-    for (int t = rank * kPlanThreads + tid; t < a.tokens; t += ctas * kPlanThreads) {
-        int slot = -1, pos = -1;
-        if (t < s_start[R]) {
-            int lo = 0, hi = R - 1;                  // the last request that starts at or before t
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if (s_start[mid] <= t) lo = mid; else hi = mid - 1;
-            }
-            if (s_take[lo] >= 0) {
-                const int p = s_past[lo], j0 = (p + a.page - 1) / a.page;
-                pos = p + t - s_start[lo];
-                const int j = pos / a.page;
-                const int pg = j < j0 ? a.table[(long long)lo * a.cols + j] : a.free_pages[avail - 1 - s_take[lo] - (j - j0)];
-                slot = pg >= 0 && pg < a.pages ? pg * a.page + pos % a.page : -1;
+    const int live = s_start[R];
+    for (int t0 = g; t0 < a.tokens; t0 += U * gsize) {
+        int x[U], r[U], pos[U], pg[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u] = t0 + u * gsize;
+        if (R > 0) last_at_most<U>(s_start, R, x, r);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            pos[u] = pg[u] = -1;
+            if (x[u] < live) {
+                const int p = s_past[r[u]];
+                if (p >= 0) {
+                    pos[u] = p + x[u] - s_start[r[u]];
+                    const int j = pos[u] / a.page, held = (p + a.page - 1) / a.page;
+                    pg[u] = j < held ? a.table[(long long)r[u] * a.cols + j] : a.free_pages[avail - 1 - s_take[r[u]] - (j - held)];
+                }
             }
         }
-        a.slots[t] = slot;
-        a.positions[t] = pos;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (x[u] < a.tokens) {
+                a.slots[x[u]] = pg[u] >= 0 && pg[u] < a.pages ? pg[u] * a.page + pos[u] % a.page : -1;
+                a.positions[x[u]] = pos[u];
+            }
     }
 }
 

@@ -271,7 +271,7 @@ int line_shift(const hkv_paged_geometry& g, int QB) {
     return shift;
 }
 
-int launch_chunk(hkv_paged_ctx* c, const PagedAttnArgs& t, const void* q, bool small, cudaStream_t st) {
+int launch_chunk(hkv_paged_ctx* c, const PagedAttnArgs& t, const void* q, int small, cudaStream_t st) {
     const hkv_paged_geometry& g = c->g;
     const int G = g.num_heads / g.num_kv_heads;
     PagedChunkArgs a{};
@@ -287,7 +287,7 @@ int launch_chunk(hkv_paged_ctx* c, const PagedAttnArgs& t, const void* q, bool s
     a.fix = fix_of(c);
     a.box_rows = std::min(g.page_size, a.line.keys);
     a.pieces = a.line.keys / a.box_rows;
-    a.small = small ? 1 : 0;
+    a.small = small;
     CUtensorMap mq, mk, mv;
     int e = encode_plane(c, t.k_cache, 64, a.box_rows, &mk);
     if (!e) e = encode_plane(c, t.v_cache, 64, a.box_rows, &mv);
@@ -398,9 +398,12 @@ int attention(hkv_paged_ctx* c, const void* q, int64_t q_token_stride, const voi
     const bool only_small = (long long)max_step * G <= kSmallCols;
     // (the prompt kernel takes the row maximum before the scale, which it can for a positive one)
     if (staged && (only_small || scale > 0.0f)) {
-        const bool small = G <= kSmallCols;              // some step_len can be one of the few-token kernel's
+        // Query rows per KV head of the few-token kernel: all that the call can have, or, beside the prompt kernel, as many
+        // tokens as fit one n8 tile (16 rows where a single token has more than 8): with two tiles every request of the
+        // launch pays for the registers (head_dim 256: one consumer group instead of two).
+        const int small = only_small ? max_step * G : G <= 8 ? 8 / G * G : G <= kSmallCols ? G : 0;
         int e = HKV_OK;
-        if (small) e = launch_small(c, a, std::min(kSmallCols, only_small ? max_step * G : kSmallCols / G * G), st);
+        if (small) e = launch_small(c, a, small, st);
         if (!e && !only_small) e = launch_chunk(c, a, q, small, st);
         if (!e && max_step > 1) e = launch_fix(c, a, block_queries(g), st);   // (nothing is hidden from a single query)
         return e;
@@ -543,11 +546,13 @@ int hkv_paged_plan(hkv_paged_ctx* c, int32_t requests, int32_t tokens, const int
     a.cols = c->g.max_pages;
     a.page = c->g.page_size;
     a.pages = c->g.num_pages;
-    int ctas = 1;
-    while (ctas < kPlanMaxCluster && (long long)ctas * kPlanThreads * 2 < (long long)tokens + requests) ctas *= 2;
+    // few requests and tokens: one small block (cheaper barriers); else a cluster with about four tokens per thread
+    int threads = kPlanThreads, ctas = 1;
+    while (threads > 128 && threads / 2 * kPlanPer >= requests && threads / 2 * 4 >= tokens) threads /= 2;
+    while (ctas < kPlanMaxCluster && (long long)ctas * threads * 4 < tokens) ctas *= 2;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)ctas);
-    cfg.blockDim = dim3(kPlanThreads);
+    cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = plan_smem_bytes(requests);
     cfg.stream = (cudaStream_t)stream;
     cudaLaunchAttribute attr[1];

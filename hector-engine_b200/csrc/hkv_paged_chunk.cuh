@@ -42,13 +42,13 @@ struct PagedChunkArgs {
     PagedFix fix;
     int QT;                   // queries per 128-row tile
     int box_rows, pieces;     // rows of a box; boxes per tile and column block
-    int small;                // 1: the few-token kernel takes the requests with few rows
+    int small;                // query rows per KV head up to which the few-token kernel takes a request; 0: none
 };
 __host__ __device__ constexpr size_t chunk_smem_bytes(int HD /*staged*/, int requests) {
     return 1024 + (size_t)(2 + 2 * kCkStages) * kCkRows * HD * 2 + 32 * 8 + 16 + 4 * kCkDesc * 4 + (size_t)(requests + 1) * 4 + 16;
 }
 __device__ __forceinline__ bool chunk_takes(const PagedChunkArgs& a, const PagedRequest& q) {
-    return q.n > 0 && !(a.small && paged_is_small(q, a.line.G));
+    return q.n > 0 && !paged_is_small(q, a.line.G, a.small);
 }
 
 // Units before each request, over the block; returns the units of all. `pre` [requests + 1] in shared memory.

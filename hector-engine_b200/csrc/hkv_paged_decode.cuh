@@ -49,8 +49,8 @@ __device__ __forceinline__ void paged_tiles(const PagedBatch& b, const PagedRequ
     tile_lo = lo / kTileRows;
     n_tiles = hi2 > lo ? (hi2 + kTileRows - 1) / kTileRows - tile_lo : 1;
 }
-// Whether the few-token kernel (this file) takes a request.
-__device__ __forceinline__ bool paged_is_small(const PagedRequest& q, int G) { return q.n > 0 && q.n * G <= kSmallCols; }
+// Whether the few-token kernel (this file) takes a request: at most `limit` query rows per KV head.
+__device__ __forceinline__ bool paged_is_small(const PagedRequest& q, int G, int limit) { return q.n > 0 && (long long)q.n * G <= limit; }
 
 template <typename T>
 __device__ __forceinline__ void mma_16816_t(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
@@ -134,7 +134,7 @@ hkv_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         for (int r = r0; r < r1; ++r) {
             const PagedRequest q = paged_request(bt, r);
             int lo, n = 0;
-            if (paged_is_small(q, G)) paged_tiles(bt, q, lo, n);
+            if (paged_is_small(q, G, a.cols)) paged_tiles(bt, q, lo, n);
             prefix[r] = n;
             sum += n;
         }

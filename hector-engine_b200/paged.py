@@ -16,6 +16,7 @@ from ._capi import HkvError, HkvPagedGeometry, HkvPagedRope
 from .ops import _ptr, _stream
 
 _DTYPES = {"float16": 0, "bfloat16": 1}
+_INT32 = None               # torch.int32, once a context exists
 
 
 def _dtype_code(dtype) -> int:
@@ -82,8 +83,17 @@ class PagedContext:
             self.close()
             raise HkvError(st, msg)
         import torch
-        self._device = torch.device("cuda", torch.cuda.current_device())
+        global _INT32
+        _INT32 = torch.int32
+        self._index = torch.cuda.current_device()
+        self._device = torch.device("cuda", self._index)
         self._dtype = torch.float16 if self._g.dtype == 0 else torch.bfloat16
+        g = self._g
+        self._heads, self._kvh, self._hd, self._cols = g.num_heads, g.num_kv_heads, g.head_dim, g.max_pages
+        self._plane_shape = (g.num_pages, g.page_size, g.num_kv_heads, g.head_dim)
+        # the raw handle of torch's current stream, without a Stream object per call
+        self._current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+            (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
     def close(self):
         if getattr(self, "_h", None):
@@ -106,44 +116,47 @@ class PagedContext:
 
     def device_status(self, stream=None) -> int:
         out = C.c_int32(0)
-        st = self.lib.hkv_paged_device_status(self._h, _stream(stream), C.byref(out))
+        st = self.lib.hkv_paged_device_status(self._h, self._stream(stream), C.byref(out))
         if st not in (_capi.HKV_OK, 8):
             self._check(st)
         return out.value
 
     # -- argument checks ------------------------------------------------------
-    def _ints(self, name, t, at_least: int):
-        import torch
-        if t.dtype != torch.int32 or t.device != self._device or not t.is_contiguous() or t.numel() < at_least:
-            raise HkvError(1, f"{name}: a contiguous int32 tensor of at least {at_least} elements on {self._device} is wanted, "
-                              f"got {t.dtype} {tuple(t.shape)} on {t.device}")
-        return t.data_ptr() or 4        # no elements: not null, and not used
+    # A decode step makes several of these calls per layer, so the checks are written for their cost: singletons are
+    # compared by identity and an error's text is put together only when there is one.
+    def _ints(self, name, t, at_least):
+        n = t.numel()
+        if t.dtype is not _INT32 or t.get_device() != self._index or n < at_least or not t.is_contiguous():
+            raise HkvError(1, f"{name}: a contiguous int32 tensor of at least {at_least} elements on cuda:{self._index} is "
+                              f"wanted, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        return t.data_ptr() if n else 4     # no elements: not null, and not used
 
-    def _rows(self, name, t, heads: int, tokens: int | None = None) -> tuple[int, int]:
+    def _rows(self, name, t, heads, tokens):
         """(pointer, token stride) of a [tokens, heads, head_dim] tensor whose tokens may lie apart."""
-        hd = self.geometry.head_dim
-        if t.dtype != self._dtype or t.device != self._device or t.dim() != 3 or tuple(t.shape[1:]) != (heads, hd) or \
-                (tokens is not None and t.shape[0] != tokens):
-            raise HkvError(1, f"{name}: [{'tokens' if tokens is None else tokens}, {heads}, {hd}] {self._dtype} on {self._device} "
-                              f"is wanted, got {tuple(t.shape)} {t.dtype} on {t.device}")
-        if t.shape[0] == 0:
-            return t.data_ptr() or 16, 0        # no rows: not null, and not used
-        if (hd > 1 and t.stride(2) != 1) or (heads > 1 and t.stride(1) != hd):
-            raise HkvError(2, f"{name}: heads and head_dim must be contiguous, strides {t.stride()}")
-        return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else 0)
+        hd = self._hd
+        if t.dtype is not self._dtype or t.get_device() != self._index or t.shape != (tokens, heads, hd):
+            raise HkvError(1, f"{name}: [{tokens}, {heads}, {hd}] {self._dtype} on cuda:{self._index} is wanted, got "
+                              f"{tuple(t.shape)} {t.dtype} on {t.device}")
+        if t.is_contiguous():
+            return (t.data_ptr() if tokens else 16), 0      # no rows: not null, and not used
+        s = t.stride()
+        if (hd > 1 and s[2] != 1) or (heads > 1 and s[1] != hd):
+            raise HkvError(2, f"{name}: heads and head_dim must be contiguous, strides {s}")
+        return t.data_ptr(), (s[0] if tokens > 1 else 0)
 
     def _plane(self, name, t):
-        g = self.geometry
-        want = (g.num_pages, g.page_size, self._g.num_kv_heads, g.head_dim)
-        if t.dtype != self._dtype or t.device != self._device or tuple(t.shape) != want or not t.is_contiguous():
-            raise HkvError(1, f"{name}: a contiguous {want} {self._dtype} plane on {self._device} is wanted, got "
+        if t.dtype is not self._dtype or t.get_device() != self._index or t.shape != self._plane_shape or not t.is_contiguous():
+            raise HkvError(1, f"{name}: a contiguous {self._plane_shape} {self._dtype} plane on cuda:{self._index} is wanted, got "
                               f"{tuple(t.shape)} {t.dtype} on {t.device}")
         return t.data_ptr()
 
-    def _table(self, t, requests: int):
-        if t.dim() != 2 or t.shape[1] != self.geometry.max_pages:
-            raise HkvError(1, f"block_table: [requests, {self.geometry.max_pages}] is wanted, got {tuple(t.shape)}")
-        return self._ints("block_table", t, requests * self.geometry.max_pages)
+    def _table(self, t, requests):
+        if t.dim() != 2 or t.shape[1] != self._cols:
+            raise HkvError(1, f"block_table: [requests, {self._cols}] is wanted, got {tuple(t.shape)}")
+        return self._ints("block_table", t, requests * self._cols)
+
+    def _stream(self, stream):
+        return self._current_stream(self._index) if stream is None else _stream(stream)
 
     # -- tables ---------------------------------------------------------------
     def new_step(self, requests: int | None = None, tokens: int | None = None) -> PagedStep:
@@ -166,7 +179,7 @@ class PagedContext:
             self._ints("free_pages", free_pages, self.geometry.num_pages), self._ints("free_count", free_count, 1),
             self._ints("total_len", total_len, r), self._ints("step_len", step.step_len, r),
             self._ints("q_start", step.q_start, r + 1), self._ints("slots", step.slots, t),
-            self._ints("positions", step.positions, t), self._ints("free_left", free_left, 1), _stream(stream)))
+            self._ints("positions", step.positions, t), self._ints("free_left", free_left, 1), self._stream(stream)))
 
     def release(self, finished, seq_len, block_table, free_pages, free_count, stream=None):
         """Gives the pages of the requests marked in `finished` back to the stack (hkv_paged_release)."""
@@ -174,70 +187,74 @@ class PagedContext:
         self._check(self.lib.hkv_paged_release(
             self._h, r, self._ints("finished", finished, r), self._ints("seq_len", seq_len, r), self._table(block_table, r),
             self._ints("free_pages", free_pages, self.geometry.num_pages), self._ints("free_count", free_count, 1),
-            _stream(stream)))
+            self._stream(stream)))
 
     # -- rows into the pages ----------------------------------------------------
     def append(self, k_new, v_new, k_cache, v_cache, slots, stream=None):
+        """K and V rows of the packed tokens to their slots (hkv_paged_append)."""
         t = slots.numel()
-        k, ks = self._rows("k_new", k_new, self._g.num_kv_heads, t)
-        v, vs = self._rows("v_new", v_new, self._g.num_kv_heads, t)
+        k, ks = self._rows("k_new", k_new, self._kvh, t)
+        v, vs = self._rows("v_new", v_new, self._kvh, t)
         if ks != vs:
             raise HkvError(2, f"k_new and v_new have different token strides ({ks}, {vs})")
-        self._check(self.lib.hkv_paged_append(self._h, k, v, ks, self._plane("k_cache", k_cache),
-                                              self._plane("v_cache", v_cache), self._ints("slots", slots, t), t,
-                                              _stream(stream)))
+        st = self.lib.hkv_paged_append(self._h, k, v, ks, self._plane("k_cache", k_cache), self._plane("v_cache", v_cache),
+                                       self._ints("slots", slots, t), t, self._stream(stream))
+        if st:
+            self._check(st)
 
     def norm_rope(self, q, k, v, positions, slots=None, k_cache=None, v_cache=None, q_out=None, k_out=None, q_norm_w=None,
                   k_norm_w=None, sections=None, interleaved=False, rotary_dim=0, eps=1e-6, theta=10000.0,
                   scaling_factor=1.0, stream=None):
         """Per-head norm (with weights) + rotary positions with `positions` [axes, tokens] (or [tokens]); K and V to their
         slots when planes are given, else the turned k to `k_out` (default: in place). q_out defaults to q."""
-        tokens, kvh, hd = q.shape[0], self._g.num_kv_heads, self.geometry.head_dim
+        tokens, kvh, hd = q.shape[0], self._kvh, self._hd
         a = HkvPagedRope()
-        a.q, a.q_token_stride = self._rows("q", q, self.geometry.num_heads)
-        a.k, a.kv_token_stride = self._rows("k", k, kvh, tokens)
-        a.q_out, a.q_out_token_stride = (a.q, a.q_token_stride) if q_out is None else \
-            self._rows("q_out", q_out, self.geometry.num_heads, tokens)
+        a.q, a.q_token_stride = self._rows("q", q, self._heads, tokens)
+        a.k, a.kv_token_stride = ks = self._rows("k", k, kvh, tokens)
+        a.q_out, a.q_out_token_stride = self._rows("q_out", q if q_out is None else q_out, self._heads, tokens)
         if k_cache is not None or v_cache is not None:
             if k_cache is None or v_cache is None or v is None or slots is None or k_out is not None:
                 raise HkvError(1, "norm_rope: with cache planes both planes, v and slots are wanted and k_out is not")
             a.v, vs = self._rows("v", v, kvh, tokens)
-            if vs != a.kv_token_stride:
-                raise HkvError(2, f"k and v have different token strides ({a.kv_token_stride}, {vs})")
+            if vs != ks[1]:
+                raise HkvError(2, f"k and v have different token strides ({ks[1]}, {vs})")
             a.k_cache, a.v_cache = self._plane("k_cache", k_cache), self._plane("v_cache", v_cache)
             a.d_slots = self._ints("slots", slots, tokens)
         else:
-            a.k_out, a.k_out_token_stride = (a.k, a.kv_token_stride) if k_out is None else self._rows("k_out", k_out, kvh, tokens)
+            a.k_out, a.k_out_token_stride = self._rows("k_out", k if k_out is None else k_out, kvh, tokens)
         for name, w in (("q_norm_w", q_norm_w), ("k_norm_w", k_norm_w)):
             if w is not None:
-                if w.dtype != self._dtype or w.device != self._device or not w.is_contiguous() or w.numel() != hd:
-                    raise HkvError(1, f"{name}: a contiguous [{hd}] {self._dtype} tensor on {self._device} is wanted")
+                if w.dtype is not self._dtype or w.get_device() != self._index or w.numel() != hd or not w.is_contiguous():
+                    raise HkvError(1, f"{name}: a contiguous [{hd}] {self._dtype} tensor on cuda:{self._index} is wanted")
                 setattr(a, name, w.data_ptr())
-        axes = 1 if positions.dim() == 1 else positions.shape[0]
-        if positions.shape[-1] != tokens or positions.dim() > 2 or axes < 1:
-            raise HkvError(1, f"positions: [axes, {tokens}] or [{tokens}] is wanted, got {tuple(positions.shape)}")
+        shape = positions.shape
+        axes = shape[0] if len(shape) == 2 else 1
+        if len(shape) not in (1, 2) or shape[-1] != tokens or axes < 1:
+            raise HkvError(1, f"positions: [axes, {tokens}] or [{tokens}] is wanted, got {tuple(shape)}")
         a.d_positions = self._ints("positions", positions, axes * tokens)
-        a.tokens, a.rotary_dim, a.axes, a.interleaved = tokens, rotary_dim, axes, int(bool(interleaved))
-        sections = list(sections or [])
-        if axes > 1 and (len(sections) != axes or axes > _capi.ROPE_MAX_AXES):
-            raise HkvError(1, f"sections: one number per axis is wanted (at most {_capi.ROPE_MAX_AXES} axes), got {sections}")
-        for i, s in enumerate(sections[:axes]):
-            a.sections[i] = s
+        a.tokens, a.rotary_dim, a.axes, a.interleaved = tokens, rotary_dim, axes, 1 if interleaved else 0
+        if axes > 1:
+            if sections is None or len(sections) != axes or axes > _capi.ROPE_MAX_AXES:
+                raise HkvError(1, f"sections: one number per axis is wanted (at most {_capi.ROPE_MAX_AXES} axes), got {sections}")
+            a.sections[:axes] = sections
         a.eps, a.theta, a.scaling_factor = eps, theta, scaling_factor
-        self._check(self.lib.hkv_paged_norm_rope(self._h, C.byref(a), _stream(stream)))
+        st = self.lib.hkv_paged_norm_rope(self._h, a, self._stream(stream))
+        if st:
+            self._check(st)
 
     # -- attention ---------------------------------------------------------------
     def _attend(self, fn, q, k_cache, v_cache, out, block_table, q_start, step_len, key_len, max_step, scale, stream):
-        scale = self.geometry.default_scale if scale is None else scale
-        r = key_len.numel()
-        qp, qs = self._rows("q", q, self.geometry.num_heads)
-        op, os_ = self._rows("out", out, self.geometry.num_heads, q.shape[0])
-        if os_ not in (0, self.geometry.num_heads * self.geometry.head_dim):
+        r, tokens = key_len.numel(), q.shape[0]
+        qp, qs = self._rows("q", q, self._heads, tokens)
+        op, os_ = self._rows("out", out, self._heads, tokens)
+        if os_:
             raise HkvError(2, f"out must be dense, token stride {os_}")
-        self._check(fn(self._h, qp, qs, self._plane("k_cache", k_cache), self._plane("v_cache", v_cache), op,
-                       self._table(block_table, r), self._ints("q_start", q_start, r), self._ints("step_len", step_len, r),
-                       self._ints("key_len", key_len, r), r, q.shape[0], q.shape[0] if max_step is None else max_step, scale,
-                       _stream(stream)))
+        st = fn(self._h, qp, qs, self._plane("k_cache", k_cache), self._plane("v_cache", v_cache), op,
+                self._table(block_table, r), self._ints("q_start", q_start, r), self._ints("step_len", step_len, r),
+                self._ints("key_len", key_len, r), r, tokens, tokens if max_step is None else max_step,
+                self.geometry.default_scale if scale is None else scale, self._stream(stream))
+        if st:
+            self._check(st)
 
     def attention(self, q, k_cache, v_cache, out, block_table, q_start, step_len, total_len, max_step=None, scale=None,
                   stream=None):
