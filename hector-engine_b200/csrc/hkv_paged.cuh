@@ -2,7 +2,6 @@
 // and the kernels around attention: block tables and slot maps, release, append, any-geometry attention.
 #pragma once
 
-#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -30,6 +29,21 @@ template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
 template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));   // bf16 is the upper half of fp32
 }
+
+// ---- division by a page size ----------------------------------------------------------------------------------------
+// n / d for 0 <= n < 2^31 as a product: with l = ceil(log2 d) and m = floor(2^(31+l) / d) + 1 <= 2^32 - 1 (d > 1), m d is
+// above 2^(31+l) by at most 2^l, so n m / 2^(31+l) is above n / d by less than 1 / d.
+struct FastDiv {
+    uint32_t mul, shift;      // mul 0: d = 1
+};
+__host__ inline FastDiv fast_div(uint32_t d) {
+    if (d == 1) return FastDiv{0, 0};
+    uint32_t l = 1;
+    while ((1ull << l) < d) ++l;
+    return FastDiv{(uint32_t)((1ull << (31 + l)) / d + 1), l - 1};
+}
+__device__ __forceinline__ int div_by(const FastDiv f, int n) { return f.mul ? (int)(__umulhi((uint32_t)n, f.mul) >> f.shift) : n; }
+__device__ __forceinline__ int ceil_div_by(const FastDiv f, int n) { return n > 0 ? div_by(f, n - 1) + 1 : 0; }
 
 // ---- the packed batch -----------------------------------------------------------------------------------------------
 struct PagedBatch {
@@ -105,20 +119,21 @@ __device__ __forceinline__ long long block_scan(long long v, long long* buf, lon
 }
 
 // ---- plan -----------------------------------------------------------------------------------------------------------
-// One thread-block cluster of up to 8 CTAs. Every CTA scans all requests itself (at most four per thread: cheaper than
-// passing sums between CTAs) and leaves their starts, lengths and places on the free stack in shared memory; after the
-// cluster barrier — every CTA has read the state that the launch may update in place — each CTA writes its share of the
-// tables. A packed token finds its request by bisection over the starts, a new page by bisection over the places on the
-// stack, so both are dealt evenly and read and written in order whatever the lengths. New pages come from the stack
-// directly, so no CTA waits for another's table writes.
+// Every CTA scans all requests itself (at most four per thread: cheaper than passing sums between CTAs) and leaves their
+// starts, lengths and places on the free stack in shared memory, then writes its share of the tables. A packed token
+// finds its request by bisection over the starts, a new page by bisection over the places on the stack, so both are dealt
+// evenly and read and written in order whatever the lengths. New pages come from the stack directly, so no CTA waits for
+// another's table writes. Where lengths or count are updated in place, the CTA that finishes last writes them: every
+// other one has read them before it says that it is done.
 // Bound: latency — the launch and three dependent trips to memory (lengths, then table or stack entry, then the store).
 struct PlanArgs {
     const int32_t *past, *fresh, *free_pages, *free_count;
     int32_t *table, *total, *step, *q_start, *slots, *positions, *free_left;
+    int* done;                        // CTAs that have finished; null: nothing is updated in place
     int requests, tokens, cols, page, pages;
+    FastDiv by_page;
 };
 constexpr int kPlanThreads = 1024;
-constexpr int kPlanMaxCluster = 8;
 constexpr int kPagedMaxRequests = 4096;
 constexpr int kPlanPer = 4;           // requests per thread
 __host__ __device__ constexpr size_t plan_smem_bytes(int requests) { return (size_t)(3 * requests + 4) * 4; }
@@ -161,9 +176,9 @@ __device__ __forceinline__ void last_at_most(const int32_t* key, const int n, co
 }
 
 __global__ void __launch_bounds__(kPlanThreads, 1) hkv_paged_plan_kernel(const PlanArgs a) {
-    namespace cg = cooperative_groups;
     extern __shared__ int32_t plan_smem[];
     __shared__ uint32_t buf[2][32];
+    __shared__ int s_last;
     __shared__ uint32_t s_taken;                     // pages taken by all admitted requests
     const int R = a.requests, tid = threadIdx.x, threads = blockDim.x;
     int32_t* s_start = plan_smem;                    // [R + 1] first packed row
@@ -197,7 +212,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) hkv_paged_plan_kernel(const P
             const uint32_t end = min(at + min((uint32_t)(fresh[i] > 0 ? fresh[i] : 0), cap), cap);
             const long long len = (long long)past[i] + fresh[i];
             fits[i] = past[i] >= 0 && fresh[i] >= 0 && len <= (long long)a.cols * a.page && end <= (uint32_t)a.tokens;
-            if (fits[i]) need[i] = (uint32_t)((len + a.page - 1) / a.page - ((long long)past[i] + a.page - 1) / a.page);
+            if (fits[i]) need[i] = (uint32_t)(ceil_div_by(a.by_page, (int)len) - ceil_div_by(a.by_page, past[i]));
             need_sum += need[i];                     // at most tokens / page + requests in all
             at = end;
         }
@@ -219,29 +234,11 @@ __global__ void __launch_bounds__(kPlanThreads, 1) hkv_paged_plan_kernel(const P
         s_start[R] = (int)min(tokens_all, (uint32_t)a.tokens);
         s_take[R] = (int)need_all;
     }
-    cg::cluster_group cluster = cg::this_cluster();
-    const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
-    if (ctas > 1) cluster.sync();                    // past, new and the count are read everywhere: state may change
-    else __syncthreads();
+    __syncthreads();
 
-    const int taken = (int)s_taken, gsize = ctas * threads, g = rank * threads + tid;
-    if (rank == 0) {
-        // every thread still holds its requests' lengths
-#pragma unroll
-        for (int i = 0; i < kPlanPer; ++i) {
-            if (i < per && r0 + i < R) {
-                const int n = s_past[r0 + i] >= 0 ? fresh[i] : 0;
-                a.q_start[r0 + i] = s_start[r0 + i];
-                a.step[r0 + i] = n;
-                a.total[r0 + i] = past[i] + n;
-            }
-        }
-        if (tid == 0) {
-            a.q_start[R] = s_start[R];
-            *a.free_left = avail - taken;
-        }
-    }
-    constexpr int U = 4;
+    const int taken = (int)s_taken, gsize = (int)gridDim.x * threads, g = (int)blockIdx.x * threads + tid;
+    const int live = s_start[R];
+    constexpr int U = 2;
     // new block-table entries: the j-th page off the stack
     for (int j0 = g; j0 < taken; j0 += U * gsize) {
         int x[U], r[U], pg[U];
@@ -255,24 +252,25 @@ __global__ void __launch_bounds__(kPlanThreads, 1) hkv_paged_plan_kernel(const P
         for (int u = 0; u < U; ++u)
             if (x[u] < taken) {
                 const int p = s_past[r[u]];          // (an admitted request: only those hold places below `taken`)
-                a.table[(long long)r[u] * a.cols + (p + a.page - 1) / a.page + x[u] - s_take[r[u]]] = pg[u];
+                a.table[(long long)r[u] * a.cols + ceil_div_by(a.by_page, p) + x[u] - s_take[r[u]]] = pg[u];
             }
     }
     // slot and position of every packed token
-    const int live = s_start[R];
     for (int t0 = g; t0 < a.tokens; t0 += U * gsize) {
-        int x[U], r[U], pos[U], pg[U];
+        int x[U], r[U], pos[U], pg[U], in[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) x[u] = t0 + u * gsize;
         if (R > 0) last_at_most<U>(s_start, R, x, r);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             pos[u] = pg[u] = -1;
+            in[u] = 0;
             if (x[u] < live) {
                 const int p = s_past[r[u]];
                 if (p >= 0) {
                     pos[u] = p + x[u] - s_start[r[u]];
-                    const int j = pos[u] / a.page, held = (p + a.page - 1) / a.page;
+                    const int j = div_by(a.by_page, pos[u]), held = ceil_div_by(a.by_page, p);
+                    in[u] = pos[u] - j * a.page;
                     pg[u] = j < held ? a.table[(long long)r[u] * a.cols + j] : a.free_pages[avail - 1 - s_take[r[u]] - (j - held)];
                 }
             }
@@ -280,9 +278,34 @@ __global__ void __launch_bounds__(kPlanThreads, 1) hkv_paged_plan_kernel(const P
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (x[u] < a.tokens) {
-                a.slots[x[u]] = pg[u] >= 0 && pg[u] < a.pages ? pg[u] * a.page + pos[u] % a.page : -1;
+                a.slots[x[u]] = pg[u] >= 0 && pg[u] < a.pages ? pg[u] * a.page + in[u] : -1;
                 a.positions[x[u]] = pos[u];
             }
+    }
+    // per-request outputs: from one CTA, every thread still holds its requests' lengths
+    if (a.done) {
+        __syncthreads();
+        if (tid == 0) {
+            s_last = atomicAdd(a.done, 1) == (int)gridDim.x - 1;
+            if (s_last) *a.done = 0;
+        }
+        __syncthreads();
+        if (!s_last) return;
+    } else if (blockIdx.x != 0) {
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < kPlanPer; ++i) {
+        if (i < per && r0 + i < R) {
+            const int n = s_past[r0 + i] >= 0 ? fresh[i] : 0;
+            a.q_start[r0 + i] = s_start[r0 + i];
+            a.step[r0 + i] = n;
+            a.total[r0 + i] = past[i] + n;
+        }
+    }
+    if (tid == 0) {
+        a.q_start[R] = live;
+        *a.free_left = avail - taken;
     }
 }
 

@@ -24,6 +24,7 @@ struct hkv_paged_ctx {
     int device = -1;
     int sm_count = 0;
     int32_t* d_status = nullptr;
+    int* plan_done = nullptr;       // CTAs of a plan launch that have finished (zero between launches)
     size_t smem_optin = 0, smem_sm = 0;
     bool staged = false;            // the geometry allows the staged kernels
     // attention workspace: partial rows of cut requests, the merge kernel's entries, marks of requests to be done again
@@ -194,7 +195,7 @@ DecodeShape decode_shape(const hkv_paged_ctx* c, int cols, int requests) {
     const bool wide = g.head_dim == 256;     // its tiles need the whole shared memory
     s.groups = two / requests > 40 || wide ? 2 : 1;
     if (s.groups == 1) {
-        s.plan = paged_decode_plan(g.head_dim, cols, 4, requests, c->smem_sm / 2 - 2048);
+        s.plan = paged_decode_plan(g.head_dim, cols, 4, requests, c->smem_sm / 2 - 1024 - 2048);
         if (s.plan.stages < 2) s.groups = 2;
     }
     if (s.groups == 2) s.plan = paged_decode_plan(g.head_dim, cols, 8, requests, c->smem_optin);
@@ -439,9 +440,10 @@ int hkv_paged_create(hkv_paged_ctx** out, const hkv_paged_geometry* geometry) {
     cudaDeviceGetAttribute(&c->sm_count, cudaDevAttrMultiProcessorCount, dev);
     if (major != 10) return fail(c, HKV_ERR_NO_DEVICE, "device is not compute capability 10.x (built for sm_100a only)");
     c->device = dev;
-    e = cudaMalloc(&c->d_status, sizeof(int32_t));
+    e = cudaMalloc(&c->d_status, 2 * sizeof(int32_t));
     if (e != cudaSuccess) return fail_cuda(c, e, "cudaMalloc(status)");
-    e = cudaMemset(c->d_status, 0, sizeof(int32_t));
+    c->plan_done = c->d_status + 1;
+    e = cudaMemset(c->d_status, 0, 2 * sizeof(int32_t));
     if (e != cudaSuccess) return fail_cuda(c, e, "cudaMemset(status)");
     e = cudaFuncSetAttribute((const void*)hkv_paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              (int)plan_smem_bytes(kPagedMaxRequests));
@@ -460,14 +462,14 @@ int hkv_paged_create(hkv_paged_ctx** out, const hkv_paged_geometry* geometry) {
             for (int groups = 1; groups <= 2; ++groups) {
                 // the attribute belongs to the kernel: always the device maximum, so that contexts never lower it for each other
                 e = cudaFuncSetAttribute((const void*)pick_decode(geometry->dtype, geometry->head_dim, nt, groups),
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, optin - 1024);
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, optin - 2048);
                 if (e != cudaSuccess) return fail_cuda(c, e, "cudaFuncSetAttribute(shared memory)");
             }
-        c->smem_optin = (size_t)optin - 1024;   // (the kernels hold a few hundred bytes of their own)
+        c->smem_optin = (size_t)optin - 2048;   // (the kernels hold up to 1.3 KB of their own)
         {
             const size_t need = chunk_smem(*geometry, geometry->max_requests);
             if (need > c->smem_optin) return fail(c, HKV_ERR_TOO_LARGE, "shared memory too small for the request table");
-            e = cudaFuncSetAttribute(chunk_kernel(*geometry), cudaFuncAttributeMaxDynamicSharedMemorySize, optin - 1024);
+            e = cudaFuncSetAttribute(chunk_kernel(*geometry), cudaFuncAttributeMaxDynamicSharedMemorySize, optin - 2048);
             if (e != cudaSuccess) return fail_cuda(c, e, "cudaFuncSetAttribute(shared memory)");
             const size_t cb = chunk_part_bytes(*geometry, c->sm_count);
             if ((e = cudaMalloc(&c->chunk_part, cb)) != cudaSuccess) return fail_cuda(c, e, "cudaMalloc(partial rows)");
@@ -546,23 +548,14 @@ int hkv_paged_plan(hkv_paged_ctx* c, int32_t requests, int32_t tokens, const int
     a.cols = c->g.max_pages;
     a.page = c->g.page_size;
     a.pages = c->g.num_pages;
-    // few requests and tokens: one small block (cheaper barriers); else a cluster with about four tokens per thread
-    int threads = kPlanThreads, ctas = 1;
-    while (threads > 128 && threads / 2 * kPlanPer >= requests && threads / 2 * 4 >= tokens) threads /= 2;
-    while (ctas < kPlanMaxCluster && (long long)ctas * threads * 4 < tokens) ctas *= 2;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)ctas);
-    cfg.blockDim = dim3((unsigned)threads);
-    cfg.dynamicSmemBytes = plan_smem_bytes(requests);
-    cfg.stream = (cudaStream_t)stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)ctas;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, hkv_paged_plan_kernel, a);
-    return e == cudaSuccess ? HKV_OK : fail_cuda(c, e, "plan launch");
+    a.by_page = fast_div((uint32_t)c->g.page_size);
+    // few requests and tokens: one small block (cheaper barriers); else two tokens per thread
+    int threads = kPlanThreads;
+    while (threads > 128 && threads / 2 * kPlanPer >= requests && threads >= tokens) threads /= 2;
+    const int ctas = std::max(1, std::min((tokens + 2 * threads - 1) / (2 * threads), c->sm_count));
+    a.done = ctas > 1 && (d_total_len == d_past_len || d_free_left == d_free_count) ? c->plan_done : nullptr;
+    hkv_paged_plan_kernel<<<ctas, threads, plan_smem_bytes(requests), (cudaStream_t)stream>>>(a);
+    return launched(c, "plan launch");
 }
 
 int hkv_paged_release(hkv_paged_ctx* c, int32_t requests, const int32_t* d_finished, int32_t* d_seq_len,

@@ -28,6 +28,7 @@ namespace hkv {
 
 constexpr int kSmallCols = 16;            // query rows per KV head this kernel takes (two n8 tiles)
 constexpr int kPagedMaxStages = 8;
+constexpr int kReqCache = 64;             // requests of a span kept in shared memory
 
 __host__ __device__ constexpr int paged_chunk_width(int HD) { return HD % 64 == 0 ? 64 : 32; }
 
@@ -114,6 +115,7 @@ hkv_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     uint64_t* bars = reinterpret_cast<uint64_t*>(mrg_ml + (size_t)NCW * a.cols * 2);
     int* prefix = reinterpret_cast<int*>(bars + 2 * kPagedMaxStages);               // [R + 1]
     __shared__ long long scan_buf[33];
+    __shared__ int4 s_req[kReqCache];     // the span's first requests: {start, n, pos0, keys}
     const uint32_t smem_base = smem_u32(smem);
     const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + kPagedMaxStages);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -163,6 +165,18 @@ hkv_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         }
         r_first = lo;
     }
+    if (u1 > u0) {
+        for (int i = tid; i < kReqCache && r_first + i < R; i += blockDim.x) {
+            const PagedRequest q = paged_request(bt, r_first + i);
+            s_req[i] = make_int4(q.start, q.n, q.pos0, q.keys);
+        }
+    }
+    __syncthreads();
+    auto request = [&](int r) -> PagedRequest {
+        if (r - r_first >= kReqCache) return paged_request(bt, r);
+        const int4 x = s_req[r - r_first];
+        return PagedRequest{x.x, x.y, x.z, x.w};
+    };
     if (member == 0 && tid == 0 && span < (int)gridDim.x / GS) {
         // the request that starts in this span and goes on behind it is merged from this span's entry
         int4 cut = make_int4(0, 0, 0, 0);
@@ -186,6 +200,7 @@ hkv_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         bool ok = true;
         const int boxes = 2 * NCH * a.pieces;
         const int page_shift = 31 - __clz(bt.page);   // page sizes here are powers of two
+        const int my_piece = lane % a.pieces;         // (pieces divides 32)
         for (int kvh = member; kvh < KVH && ok; kvh += GS) {
             int r = r_first;
             for (int u = u0; u < u1 && ok; ++r) {
@@ -194,34 +209,37 @@ hkv_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                 const int off = u - prefix[r];
                 const int nt = nb - off < u1 - u ? nb - off : u1 - u;
                 u += nt;
-                const PagedRequest q = paged_request(bt, r);
+                const PagedRequest q = request(r);
                 int tile_lo, n_tiles, lo, hi, x_;
                 paged_tiles(bt, q, tile_lo, n_tiles);
                 paged_key_range(bt, q, 0, lo, x_);
                 paged_key_range(bt, q, q.n - 1, x_, hi);
                 const int32_t* table = bt.table + (long long)r * bt.cols;
+                // page of this lane's box: behind the tensor (zeros, nothing read) where no query looks
+                auto look_up = [&](int p) -> int {
+                    if (p >= hi || p + a.box_rows <= lo) return bt.pages;
+                    const int pg = __ldg(table + (p >> page_shift));
+                    if (pg >= 0 && pg < bt.pages) return pg;
+                    atomicOr(bt.status, kStatusBoundCheck);
+                    return bt.pages;
+                };
+                int pg = look_up((tile_lo + off) * kTileRows + my_piece * a.box_rows);
                 for (int t = 0; t < nt; ++t) {
+                    const int pos0 = (tile_lo + off + t) * kTileRows;
+                    const int pg_next = t + 1 < nt ? look_up(pos0 + kTileRows + my_piece * a.box_rows) : 0;   // a tile ahead
                     if (round > 0) ok = __all_sync(0xffffffffu, mbar_wait(empty0 + 8 * stage, (uint32_t)(round - 1) & 1u, bt.status));
                     if (!ok) break;
                     const uint32_t full = full0 + 8 * stage;
                     const uint32_t dst = smem_base + (uint32_t)stage * STAGE_BYTES;
                     if (lane == 0) mbar_expect_tx(full, STAGE_BYTES);
                     __syncwarp();
-                    const int pos0 = (tile_lo + off + t) * kTileRows;
-                    for (int x = lane; x < boxes; x += 32) {
-                        const int piece = x % a.pieces, c = x / a.pieces % NCH, kv = x / (a.pieces * NCH);
-                        const int p = pos0 + piece * a.box_rows;
-                        int pg = bt.pages;            // behind the tensor: zeros
-                        if (p < hi && p + a.box_rows > lo) {
-                            pg = __ldg(table + (p >> page_shift));
-                            if (pg < 0 || pg >= bt.pages) {
-                                atomicOr(bt.status, kStatusBoundCheck);
-                                pg = bt.pages;
-                            }
-                        }
-                        tma_load_4d(dst + kv * TILE_BYTES + c * CHUNK_BYTES + piece * a.box_rows * ROWB, kv ? &tm_v : &tm_k, full,
-                                    c * CW, kvh, p & (bt.page - 1), pg);
+                    for (int b0 = 0; b0 < boxes; b0 += 32) {
+                        const int x = b0 + lane, piece = x % a.pieces, c = x / a.pieces % NCH, kv = x / (a.pieces * NCH);
+                        if (x < boxes)
+                            tma_load_4d(dst + kv * TILE_BYTES + c * CHUNK_BYTES + piece * a.box_rows * ROWB, kv ? &tm_v : &tm_k, full,
+                                        c * CW, kvh, (pos0 + piece * a.box_rows) & (bt.page - 1), pg);
                     }
+                    pg = pg_next;
                     ++issued;
                     if (++stage == stages) { stage = 0; ++round; }
                 }
@@ -256,7 +274,7 @@ hkv_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         const int nt = nb - off < u1 - u ? nb - off : u1 - u;
         const bool begins = off == 0, ends = off + nt == nb;
         u += nt;
-        const PagedRequest q = paged_request(bt, r);
+        const PagedRequest q = request(r);
         const int ncol = q.n * G;
         int tile_lo, n_tiles, lo_first, hi_first, lo_last, hi_last;
         paged_tiles(bt, q, tile_lo, n_tiles);

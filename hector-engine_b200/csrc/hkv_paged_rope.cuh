@@ -90,6 +90,34 @@ __global__ void __launch_bounds__(kMropeThreads) hkv_paged_norm_rope_any_kernel(
     }
 }
 
+// Two 32-bit values in one 64-bit register: sm_100 multiplies and adds them in one instruction.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack_f2(float a, float b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack_f2(f32x2 x) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ f32x2 widen2(uint32_t w) {
+    const float2 f = unpack2<T>(w);
+    return pack_f2(f.x, f.y);
+}
+
 // The register path (host: rows 16-byte aligned, head_dim and rotary_dim multiples of 16).
 //
 // Bound: HBM for prompts (each row read once, written once); latency for a decode step. A warp works on one token at a
@@ -99,11 +127,15 @@ __global__ void __launch_bounds__(kMropeThreads) hkv_paged_norm_rope_any_kernel(
 //     8 lanes for head_dim 128, four heads per warp and round.
 //   * cos and sin of a token's pairs are computed once, two pairs per lane at head_dim 128, and shared through the warp's
 //     table in shared memory: 64-bit turns reduced to [-1/2, 1/2], then sincospi in 32 bits.
+//   * The norm weights are folded into them, per token and kind of head: with x, y the halves of a pair,
+//         x' = inv (x A + y B)   y' = inv (x C + y D)    A = w_x cos   B = -w_y sin   C = w_x sin   D = w_y cos
+//     so that an element costs three packed instructions of two elements each beside its conversions. (Unfolded and
+//     unpacked the kernel was bound by instruction issue: 245 instructions a round, 40 us for 8 192 tokens.)
 //   * U rounds' loads are issued together, in front of the angles.
 constexpr int kMropeRounds = 4;
 
 template <typename T, int LPH>
-__global__ void __launch_bounds__(kMropeThreads) hkv_paged_norm_rope_kernel(const __grid_constant__ MropeArgs a) {
+__global__ void __launch_bounds__(kMropeThreads, 2) hkv_paged_norm_rope_kernel(const __grid_constant__ MropeArgs a) {
     constexpr int HPW = 32 / LPH;                      // heads per warp and round
     constexpr int U = kMropeRounds;
     __shared__ float2 s_cs[kMropeWarps][LPH * 8];      // pairs of one token: rot/2 <= LPH * 8
@@ -111,7 +143,7 @@ __global__ void __launch_bounds__(kMropeThreads) hkv_paged_norm_rope_kernel(cons
     __shared__ uint8_t s_axis[LPH * 8];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = a.rot / 2;
     const int sub = lane / LPH, p = lane % LPH;
-    const int heads = a.H + a.KVH + (a.k_cache ? a.KVH : 0);
+    const int heads = a.H + a.KVH + (a.k_cache ? a.KVH : 0), HK = a.H + a.KVH;
     for (int i = threadIdx.x; i < half; i += kMropeThreads) { s_turns[i] = a.turns[i]; s_axis[i] = a.axis[i]; }
     const bool live = 16 * p < a.HD, turns = 16 * p < a.rot;
     // elements of this lane's two pieces
@@ -136,8 +168,7 @@ __global__ void __launch_bounds__(kMropeThreads) hkv_paged_norm_rope_kernel(cons
                 const int j = jb + u * HPW + sub;
                 x0[u] = x1[u] = make_uint4(0, 0, 0, 0);
                 if (live && j < j1 && j < heads) {
-                    const T* src = j < a.H ? qt + (long long)j * a.HD
-                                 : j < a.H + a.KVH ? kt + (long long)(j - a.H) * a.HD : vt + (long long)(j - a.H - a.KVH) * a.HD;
+                    const T* src = j < a.H ? qt + j * a.HD : j < HK ? kt + (j - a.H) * a.HD : vt + (j - HK) * a.HD;
                     x0[u] = *reinterpret_cast<const uint4*>(src + e0);
                     x1[u] = *reinterpret_cast<const uint4*>(src + e1);
                 }
@@ -148,59 +179,64 @@ __global__ void __launch_bounds__(kMropeThreads) hkv_paged_norm_rope_kernel(cons
         const bool store = slot >= 0 && (!a.k_cache || slot < a.rows);
         if (a.k_cache && slot >= a.rows && lane == 0) atomicOr(a.status, kStatusBoundCheck);
         __syncwarp();
-        float c[8], s[8];
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-            const float4 w = turns ? *reinterpret_cast<const float4*>(&s_cs[warp][8 * p + e]) : make_float4(1.0f, 0.0f, 1.0f, 0.0f);
-            c[e] = w.x; s[e] = w.y; c[e + 1] = w.z; s[e + 1] = w.w;
-        }
+        f32x2 A[4], B[4], C[4], D[4];                  // of this lane's 8 pairs, for the kind of head it is at
+        int kind = -1;                                 // 0 query, 1 key, 2 value (copied)
+        // rows of this token that are written: query rows, and key / value rows in the planes or in k_out
+        T* const q_row = (T*)a.q_out + t * a.qo_stride;
+        T* const k_row = a.k_cache ? (T*)a.k_cache + (long long)slot * a.KVH * a.HD : (T*)a.k_out + t * a.ko_stride;
+        T* const v_row = (T*)a.v_cache + (long long)slot * a.KVH * a.HD;
         for (int jb = j0; jb < j1; jb += U * HPW) {
             if (jb != j0) load(jb);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int j = jb + u * HPW + sub;
                 if (jb + u * HPW >= j1) break;         // warp-uniform
-                const bool is_q = j < a.H, is_v = j >= a.H + a.KVH;
-                float x[8], y[8];
-                const uint32_t w0[4] = {x0[u].x, x0[u].y, x0[u].z, x0[u].w}, w1[4] = {x1[u].x, x1[u].y, x1[u].z, x1[u].w};
+                const int is = j < a.H ? 0 : j < HK ? 1 : 2;
+                if (is != kind && is < 2) {
+                    const T* w = (const T*)(is == 0 ? a.q_w : a.k_w);
+                    uint4 w0 = make_uint4(0, 0, 0, 0), w1 = w0;
+                    if (w && live) { w0 = *reinterpret_cast<const uint4*>(w + e0); w1 = *reinterpret_cast<const uint4*>(w + e1); }
+                    const uint32_t v0[4] = {w0.x, w0.y, w0.z, w0.w}, v1[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float2 f = unpack2<T>(w0[e]), g = unpack2<T>(w1[e]);
-                    x[2 * e] = f.x; x[2 * e + 1] = f.y;
-                    y[2 * e] = g.x; y[2 * e + 1] = g.y;
-                }
-                if (a.q_w) {
-                    float ssq = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) ssq = fmaf(x[e], x[e], fmaf(y[e], y[e], ssq));
-#pragma unroll
-                    for (int o = LPH / 2; o > 0; o >>= 1) ssq += __shfl_xor_sync(0xffffffffu, ssq, o);
-                    const float inv = rsqrtf(fmaf(ssq, inv_hd, a.eps));
-                    const T* w = (const T*)(is_q ? a.q_w : a.k_w);
-                    if (live) {
-                        const uint4 a0 = *reinterpret_cast<const uint4*>(w + e0), a1 = *reinterpret_cast<const uint4*>(w + e1);
-                        const uint32_t u0[4] = {a0.x, a0.y, a0.z, a0.w}, u1[4] = {a1.x, a1.y, a1.z, a1.w};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float2 f = unpack2<T>(u0[e]), g = unpack2<T>(u1[e]);
-                            x[2 * e] *= inv * f.x; x[2 * e + 1] *= inv * f.y;
-                            y[2 * e] *= inv * g.x; y[2 * e + 1] *= inv * g.y;
-                        }
+                    for (int e = 0; e < 4; ++e) {
+                        const float4 cs = turns ? *reinterpret_cast<const float4*>(&s_cs[warp][8 * p + 2 * e]) : make_float4(1.0f, 0.0f, 1.0f, 0.0f);
+                        const f32x2 c = pack_f2(cs.x, cs.z), s = pack_f2(cs.y, cs.w), n = pack_f2(-cs.y, -cs.w);
+                        const f32x2 wx = w ? widen2<T>(v0[e]) : pack_f2(1.0f, 1.0f), wy = w ? widen2<T>(v1[e]) : pack_f2(1.0f, 1.0f);
+                        A[e] = mul2(wx, c); B[e] = mul2(wy, n); C[e] = mul2(wx, s); D[e] = mul2(wy, c);
                     }
                 }
-                uint32_t r0[4], r1[4];
+                kind = is;
+                uint32_t r0[4] = {x0[u].x, x0[u].y, x0[u].z, x0[u].w}, r1[4] = {x1[u].x, x1[u].y, x1[u].z, x1[u].w};
+                f32x2 x[4], y[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    r0[e] = pack2<T>(x[2 * e] * c[2 * e] - y[2 * e] * s[2 * e], x[2 * e + 1] * c[2 * e + 1] - y[2 * e + 1] * s[2 * e + 1]);
-                    r1[e] = pack2<T>(x[2 * e] * s[2 * e] + y[2 * e] * c[2 * e], x[2 * e + 1] * s[2 * e + 1] + y[2 * e + 1] * c[2 * e + 1]);
+                for (int e = 0; e < 4; ++e) { x[e] = widen2<T>(r0[e]); y[e] = widen2<T>(r1[e]); }
+                float inv = 1.0f;
+                if (a.q_w) {
+                    f32x2 q = mul2(x[0], x[0]);
+#pragma unroll
+                    for (int e = 1; e < 4; ++e) q = fma2(x[e], x[e], q);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) q = fma2(y[e], y[e], q);
+                    const float2 h = unpack_f2(q);
+                    float ssq = h.x + h.y;
+#pragma unroll
+                    for (int o = LPH / 2; o > 0; o >>= 1) ssq += __shfl_xor_sync(0xffffffffu, ssq, o);
+                    inv = rsqrtf(fmaf(ssq, inv_hd, a.eps));
                 }
-                if (!live || j >= heads || (!is_q && !store)) continue;
-                T* dst = is_q ? (T*)a.q_out + t * a.qo_stride + (long long)j * a.HD
-                       : is_v ? (T*)a.v_cache + ((long long)slot * a.KVH + (j - a.H - a.KVH)) * a.HD
-                       : a.k_cache ? (T*)a.k_cache + ((long long)slot * a.KVH + (j - a.H)) * a.HD
-                                   : (T*)a.k_out + t * a.ko_stride + (long long)(j - a.H) * a.HD;
-                *reinterpret_cast<uint4*>(dst + e0) = is_v ? x0[u] : make_uint4(r0[0], r0[1], r0[2], r0[3]);
-                *reinterpret_cast<uint4*>(dst + e1) = is_v ? x1[u] : make_uint4(r1[0], r1[1], r1[2], r1[3]);
+                if (!live || j >= heads || (is > 0 && !store)) continue;
+                if (is < 2) {
+                    const f32x2 i2 = pack_f2(inv, inv);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 f = unpack_f2(mul2(i2, fma2(x[e], A[e], mul2(y[e], B[e]))));
+                        const float2 g = unpack_f2(mul2(i2, fma2(x[e], C[e], mul2(y[e], D[e]))));
+                        r0[e] = pack2<T>(f.x, f.y);
+                        r1[e] = pack2<T>(g.x, g.y);
+                    }
+                }
+                T* dst = is == 0 ? q_row + j * a.HD : is == 1 ? k_row + (j - a.H) * a.HD : v_row + (j - HK) * a.HD;
+                *reinterpret_cast<uint4*>(dst + e0) = make_uint4(r0[0], r0[1], r0[2], r0[3]);
+                *reinterpret_cast<uint4*>(dst + e1) = make_uint4(r1[0], r1[1], r1[2], r1[3]);
             }
         }
         __syncwarp();                                  // the table is read before the next token's is written
