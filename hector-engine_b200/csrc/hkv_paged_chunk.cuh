@@ -12,8 +12,10 @@
 //     kernel's entry, 11 completes the warpgroup for setmaxnreg. A key tile is a set of boxes, one per page: the
 //     producer's lanes look up one page each, a tile ahead, and issue side by side.
 //   * Tensor memory: S_A, S_B (128 columns each; P is written over the first half of its S), O_A, O_B. Per key tile:
-//     PV_A QK_A(next) PV_B QK_B(next), so that one tile's softmax runs under the other's products. O is rescaled only
-//     when a row's maximum outgrows its reference by 2^8. P is rounded to the element type (its sum is not). 3 of 8 pairs
+//     PV_A QK_A(next) PV_B QK_B(next), so that one tile's softmax runs under the other's products; P V of the first half
+//     of a tile's keys starts while P of the second half is computed. O is rescaled only when a row's maximum outgrows
+//     its reference by 2^8. (Two threads per row halve nothing: the softmax is bound by its instructions, the exchange and
+//     the doubled bookkeeping cost a tenth.) P is rounded to the element type (its sum is not). 3 of 8 pairs
 //     take a polynomial on the FMA pipe instead of ex2, the narrowest unit.
 //   * Every wait is bounded and reports through the status word; tensor memory is freed on every path.
 #pragma once
@@ -132,6 +134,34 @@ __device__ __forceinline__ void chunk_walk(const PagedBatch& b, const PagedLine&
     }
 }
 
+// V rows [kstart, kstart + keys) of a staged tile that not every query of a block sees: rows that none attends are zeroed,
+// values that are not finite are dropped from the others (0 * NaN would reach the queries they are hidden from). `threads`
+// threads take part; true if this one dropped a value.
+template <typename T, int NCH, int threads>
+static __device__ __noinline__ bool clean_values(const PagedBatch& b, const PagedRequest q, const int i0, const int QB, const int kstart,
+                                          const int keys, uint8_t* tile, const int chunk_bytes, const int tid) {
+    int lo_first, hi_first, lo_last, hi_last;
+    paged_key_range(b, q, i0, lo_first, hi_first);
+    paged_key_range(b, q, (i0 + QB < q.n ? i0 + QB : q.n) - 1, lo_last, hi_last);
+    const int head = lo_last - kstart < 0 ? 0 : (lo_last - kstart < keys ? lo_last - kstart : keys);
+    int tail = hi_first - kstart < 0 ? 0 : (hi_first - kstart < keys ? hi_first - kstart : keys);
+    if (tail < head) tail = head;
+    bool bad = false;
+    for (int idx = tid; idx < (head + keys - tail) * 8 * NCH; idx += threads) {
+        const int k = idx / (8 * NCH), u = idx % (8 * NCH);
+        const int vr = k < head ? k : tail + k - head, pos = kstart + vr;
+        uint4* at = reinterpret_cast<uint4*>(tile + (u / 8) * chunk_bytes + vr * 128 + (u % 8) * 16);
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (pos >= lo_first && pos < hi_last) {
+            x = *at;
+            if (!drop_nonfinite<T>(x)) continue;
+            bad = true;
+        }
+        *at = x;
+    }
+    return bad;
+}
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(kCkThreads, 1)
 hkv_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -157,8 +187,8 @@ hkv_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     __shared__ long long scan_buf[33];
     const uint32_t q_smem = smem_u32(smem), k_smem = smem_u32(k_gen), v_smem = smem_u32(v_gen), bar0 = smem_u32(bars);
     const uint32_t B_QFULL = bar0, B_QEMPTY = bar0 + 8, B_KFULL = bar0 + 16, B_KEMPTY = bar0 + 32, B_VFULL = bar0 + 48,
-                   B_VEMPTY = bar0 + 64, B_SFULL = bar0 + 80, B_PFULL = bar0 + 96, B_OFULL = bar0 + 112, B_DONE = bar0 + 128,
-                   B_WF = bar0 + 144, B_WE = bar0 + 176;      // work queue: slot full [4], slot read [4]
+                   B_VEMPTY = bar0 + 64, B_SFULL = bar0 + 80, B_PFULL = bar0 + 96 /* [tile][half] */, B_OFULL = bar0 + 128,
+                   B_DONE = bar0 + 144, B_WF = bar0 + 152, B_WE = bar0 + 184;      // work queue: slot full [4], slot read [4]
     const PagedBatch& bt = a.t.b;
     const int G = a.line.G, H = a.t.H, D = a.t.HD;
 
@@ -169,8 +199,8 @@ hkv_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             mbar_init(B_KFULL + 8 * s, 1); mbar_init(B_KEMPTY + 8 * s, 1);
             mbar_init(B_VFULL + 8 * s, 1); mbar_init(B_VEMPTY + 8 * s, 1);
         }
-        for (int g = 0; g < 2; ++g) { mbar_init(B_SFULL + 8 * g, 1); mbar_init(B_PFULL + 8 * g, 128); mbar_init(B_OFULL + 8 * g, 1); }
-        for (int i = 0; i < 4; ++i) { mbar_init(B_WF + 8 * i, 1); mbar_init(B_WE + 8 * i, 9); }
+        for (int g = 0; g < 2; ++g) { mbar_init(B_SFULL + 8 * g, 1); mbar_init(B_OFULL + 8 * g, 1); }
+        for (int i = 0; i < 4; ++i) { mbar_init(B_PFULL + 8 * i, 4); mbar_init(B_WF + 8 * i, 1); mbar_init(B_WE + 8 * i, 9); }
         fence_mbar_init();
         tma_prefetch_desc(&tm_q); tma_prefetch_desc(&tm_k); tma_prefetch_desc(&tm_v);
     }
@@ -297,14 +327,17 @@ hkv_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
                 }
                 tc_commit(B_SFULL + 8 * grp);
             };
-            auto issue_pv = [&](uint32_t g, int grp, bool accumulate) {   // O_grp (+)= P_grp V(g)
+            // O_grp (+)= P_grp V(g) over one half of the tile's keys
+            auto issue_pv = [&](uint32_t g, int grp, int half, bool accumulate) {
                 const uint32_t vd = v_lo + (((g % kCkStages) * TILE_BYTES) >> 4);
                 const uint32_t pbase = tmem + COL_S + 128u * grp, d = tmem + COL_O + 128u * grp;
-                if (accumulate) tc_mma_ts_i<true>(d, pbase, vd, desc_hi, IDESC_PV);
-                else tc_mma_ts_i<false>(d, pbase, vd, desc_hi, IDESC_PV);
 #pragma unroll
-                for (int kk = 1; kk < kCkKeys / 16; ++kk)
-                    tc_mma_ts_i<true>(d, pbase + kk * 8, vd + (uint32_t)((kk * 2048) >> 4), desc_hi, IDESC_PV);
+                for (int k = 0; k < kCkKeys / 32; ++k) {
+                    const int kk = half * (kCkKeys / 32) + k;
+                    const uint32_t at = vd + (uint32_t)((kk * 2048) >> 4);
+                    if (k > 0 || accumulate) tc_mma_ts_i<true>(d, pbase + kk * 8, at, desc_hi, IDESC_PV);
+                    else tc_mma_ts_i<false>(d, pbase + kk * 8, at, desc_hi, IDESC_PV);
+                }
             };
             for (; ok; ++it) {
                 if (!queue_wait(it)) { ok = false; break; }
@@ -328,9 +361,13 @@ hkv_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 #pragma unroll
                     for (int grp = 0; grp < 2; ++grp) {
                         if (grp == 1 && !two) break;
-                        if (!mbar_wait(B_PFULL + 8 * grp, (grp ? gb : gt) & 1, bt.status)) { ok = false; break; }
+                        const uint32_t ph = (grp ? gb : gt) & 1;
+                        if (!mbar_wait(B_PFULL + 16 * grp, ph, bt.status)) { ok = false; break; }
                         tc_fence_after();
-                        issue_pv(gt, grp, t > 0);
+                        issue_pv(gt, grp, 0, t > 0);
+                        if (!mbar_wait(B_PFULL + 16 * grp + 8, ph, bt.status)) { ok = false; break; }
+                        tc_fence_after();
+                        issue_pv(gt, grp, 1, true);
                         if (!more) tc_commit(B_OFULL + 8 * grp);
                         if (grp == two) tc_commit(B_VEMPTY + 8 * vs);       // every tile has consumed V(g)
                         if (more) {
@@ -357,7 +394,7 @@ hkv_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         const uint32_t lane_sel = (uint32_t)(quad * 32) << 16;
         const uint32_t s_addr = tmem + lane_sel + COL_S + 128u * grp;
         const uint32_t o_addr = tmem + lane_sel + COL_O + 128u * grp;
-        const uint32_t b_sfull = B_SFULL + 8 * grp, b_pfull = B_PFULL + 8 * grp, b_ofull = B_OFULL + 8 * grp;
+        const uint32_t b_sfull = B_SFULL + 8 * grp, b_pfull = B_PFULL + 16 * grp, b_ofull = B_OFULL + 8 * grp;
         const int ql = row / G, g = row % G;
         uint32_t gt = 0, si = 0;   // tiles and items of this group (barrier phases); group A's tiles are the CTA's
         bool ok = true;            // kept warp-uniform: a wait that ran out for any lane stops the warp
@@ -366,22 +403,22 @@ hkv_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             if (!ok) break;
             const volatile int* d = queue + (qk & 3) * kCkDesc;
             const int r = d[0], kvh = d[1], p = d[2], kt = d[3], nt = d[4], slot = d[5], two = d[6];
-            PagedRequest q;
-            q.start = d[7]; q.n = d[8]; q.pos0 = d[9]; q.keys = d[10];
+            const PagedRequest q{d[7], d[8], d[9], d[10]};
             __syncwarp();
             if (lane == 0) mbar_arrive(B_WE + 8 * (qk & 3));
             if (r < 0) break;
             if (grp > two) continue;               // the block of queries fits tile A
-            const int i0 = p * a.line.QB;
-            const int qi = i0 + grp * a.QT + ql;
-            const bool row_valid = ql < a.QT && qi < q.n;
+            const int i0 = p * a.line.QB, qi = i0 + grp * a.QT + ql, kbase = kt * kCkKeys;
             // rows without a query take the bounds of the last one, so that they never hold up their warp
-            int lo_row, hi_row;
+            int lo_row, hi_row, head, tail;        // tiles that not every query of the item sees whole: before head, from tail on
             paged_key_range(bt, q, qi < q.n ? qi : q.n - 1, lo_row, hi_row);
-            // item-wide bounds: a tile outside them holds keys that not every query sees
-            int lo_first, hi_first, lo_last, hi_last;
-            paged_key_range(bt, q, i0, lo_first, hi_first);
-            paged_key_range(bt, q, (i0 + a.line.QB < q.n ? i0 + a.line.QB : q.n) - 1, lo_last, hi_last);
+            {
+                int x, lo_last, hi_first;
+                paged_key_range(bt, q, i0, x, hi_first);
+                paged_key_range(bt, q, (i0 + a.line.QB < q.n ? i0 + a.line.QB : q.n) - 1, lo_last, x);
+                head = lo_last > kbase ? (lo_last - kbase + kCkKeys - 1) / kCkKeys : 0;
+                tail = hi_first > kbase ? (hi_first - kbase) / kCkKeys : 0;
+            }
             float m_ref = kLow, l_run = 0.0f;      // m_ref: the reference P and O are scaled by
 
             for (int t = 0; t < nt; ++t, ++gt) {
@@ -391,39 +428,32 @@ hkv_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
                 uint32_t sv[4][32];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) tmem_ld32(sv[c], s_addr + c * 32);
-                const int kstart = (kt + t) * kCkKeys;
-                const int lo = lo_row - kstart, hi = hi_row - kstart;   // attended columns [lo, hi)
+                const int lo = lo_row - (kt + t) * kCkKeys, hi = hi_row - (kt + t) * kCkKeys;   // attended columns [lo, hi)
                 const bool all_in = __all_sync(0xffffffffu, lo <= 0 && hi >= kCkKeys);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) tc_wait_ld_dep(sv[c]);
+                if (!all_in) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (c * 32 + j < lo || c * 32 + j >= hi) sv[c][j] = 0xff800000u;   // -infinity
+                }
                 // ---- row maximum of the raw scores (the scale is positive) ----
                 float mx;
                 {
                     float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;   // independent chains
-                    if (all_in) {
 #pragma unroll
-                        for (int c = 0; c < 4; ++c)
+                    for (int c = 0; c < 4; ++c)
 #pragma unroll
-                            for (int j = 0; j < 32; j += 8) {
-                                m0 = fmax3(m0, __uint_as_float(sv[c][j]), __uint_as_float(sv[c][j + 1]));
-                                m1 = fmax3(m1, __uint_as_float(sv[c][j + 2]), __uint_as_float(sv[c][j + 3]));
-                                m2 = fmax3(m2, __uint_as_float(sv[c][j + 4]), __uint_as_float(sv[c][j + 5]));
-                                m3 = fmax3(m3, __uint_as_float(sv[c][j + 6]), __uint_as_float(sv[c][j + 7]));
-                            }
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < 4; ++c)
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                const int col = c * 32 + j;
-                                const float sc = (col >= lo && col < hi) ? __uint_as_float(sv[c][j]) : -INFINITY;
-                                sv[c][j] = __float_as_uint(sc);
-                                m0 = fmaxf(m0, sc);
-                            }
-                    }
-                    mx = fmaxf(fmax3(m0, m1, m2), m3);
+                        for (int j = 0; j < 32; j += 8) {
+                            m0 = fmax3(m0, __uint_as_float(sv[c][j]), __uint_as_float(sv[c][j + 1]));
+                            m1 = fmax3(m1, __uint_as_float(sv[c][j + 2]), __uint_as_float(sv[c][j + 3]));
+                            m2 = fmax3(m2, __uint_as_float(sv[c][j + 4]), __uint_as_float(sv[c][j + 5]));
+                            m3 = fmax3(m3, __uint_as_float(sv[c][j + 6]), __uint_as_float(sv[c][j + 7]));
+                        }
+                    mx = fmaxf(fmax3(m0, m1, m2), m3) * a.t.scale_log2;
                 }
-                mx *= a.t.scale_log2;
                 const bool move = mx > m_ref + 8.0f;
                 if (__any_sync(0xffffffffu, move)) {
                     const float m_to = move ? mx : m_ref;
@@ -433,7 +463,18 @@ hkv_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
                     l_run *= alpha;
                     m_ref = m_to;
                 }
-                // ---- p = 2^(s*scale - m_ref), row sum, P back to tensor memory ----
+                // Tiles that not every query of the item sees whole: group A cleans the V rows before its arrival, which
+                // precedes both output products.
+                if (grp == 0 && (t < head || t >= tail)) {
+                    const uint32_t vs = gt % kCkStages;
+                    ok = __all_sync(0xffffffffu, mbar_wait(B_VFULL + 8 * vs, (gt / kCkStages) & 1, bt.status));
+                    if (!ok) continue;
+                    const bool bad = clean_values<T, NCH, 128>(bt, q, i0, a.line.QB, (kt + t) * kCkKeys, kCkKeys,
+                                                               v_gen + (size_t)vs * TILE_BYTES, CHUNK_BYTES, tid);
+                    if (__any_sync(0xffffffffu, bad) && lane == 0) a.fix.push(r, p, kvh);
+                    fence_proxy_async_smem();
+                }
+                // ---- p = 2^(s*scale - m_ref), row sum, P back to tensor memory, half a tile at a time ----
                 float lsum0 = 0.0f, lsum1 = 0.0f, lsum2 = 0.0f, lsum3 = 0.0f;
                 const float neg_m = -m_ref;
 #pragma unroll
@@ -455,48 +496,26 @@ hkv_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
                         pk[j / 2 + 1] = pack2<T>(p2, p3);
                     }
                     tmem_st16(s_addr + c * 16, pk);    // over the scores, all of which are in registers
-                }
-                tc_wait_st();
-                l_run += (lsum0 + lsum1) + (lsum2 + lsum3);
-                // Tiles that not every query of the item sees whole: group A zeroes the V rows that none attends and drops
-                // values that are not finite from the others (0 * NaN), before its arrival, which precedes both output products.
-                if (grp == 0 && (kstart < lo_last || kstart + kCkKeys > hi_first)) {
-                    const uint32_t vs = gt % kCkStages;
-                    ok = __all_sync(0xffffffffu, mbar_wait(B_VFULL + 8 * vs, (gt / kCkStages) & 1, bt.status));
-                    if (!ok) continue;
-                    uint8_t* vt = v_gen + (size_t)vs * TILE_BYTES;
-                    const int head = lo_last - kstart < 0 ? 0 : (lo_last - kstart < kCkKeys ? lo_last - kstart : kCkKeys);
-                    int tail = hi_first - kstart < 0 ? 0 : (hi_first - kstart < kCkKeys ? hi_first - kstart : kCkKeys);
-                    if (tail < head) tail = head;
-                    bool bad = false;
-                    for (int idx = tid; idx < (head + kCkKeys - tail) * 8 * NCH; idx += 128) {
-                        const int k = idx / (8 * NCH), u = idx % (8 * NCH);
-                        const int vr = k < head ? k : tail + k - head, pos = kstart + vr;
-                        uint4* at = reinterpret_cast<uint4*>(vt + (u / 8) * CHUNK_BYTES + vr * 128 + (u % 8) * 16);
-                        uint4 x = make_uint4(0, 0, 0, 0);
-                        if (pos >= lo_first && pos < hi_last) {
-                            x = *at;
-                            if (!drop_nonfinite<T>(x)) continue;
-                            bad = true;
-                        }
-                        *at = x;
+                    if (c & 1) {
+                        tc_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(b_pfull + 4 * (c & 2));
                     }
-                    if (__any_sync(0xffffffffu, bad) && lane == 0) a.fix.push(r, p, kvh);
-                    fence_proxy_async_smem();
                 }
-                tc_fence_before();
-                mbar_arrive(b_pfull);
+                l_run += (lsum0 + lsum1) + (lsum2 + lsum3);
             }
             // the item's last P V of this tile, then the row goes out
             ok = __all_sync(0xffffffffu, ok && mbar_wait(b_ofull, si & 1, bt.status));
             ++si;
             if (!ok) continue;
             tc_fence_after();
+            const bool row_valid = ql < a.QT && qi < q.n;
             const float inv = l_run == 0.0f ? 0.0f : (l_run < kSumLimit ? 1.0f / l_run : NAN);
             float* prow = slot >= 0 ? a.part + ((long long)slot * (2 * kCkRows) + grp * kCkRows + row) * (D + 4) : nullptr;
             T* op = (T*)a.t.out + ((long long)(q.start + qi) * H + (long long)kvh * G + g) * D;
-#pragma unroll
-            for (int c = 0; c < HD / 32; ++c) {
+#pragma unroll 1
+            for (int c = 0; c < HD / 32; ++c) {            // (a loop: straight-line code is fetched once per item here)
                 uint32_t v[32];
                 tmem_ld32(v, o_addr + c * 32);
                 tc_wait_ld_dep(v);
