@@ -15,7 +15,7 @@
 //     PV_A QK_A(next) PV_B QK_B(next), so that one tile's softmax runs under the other's products; P V of the first half
 //     of a tile's keys starts while P of the second half is computed. O is rescaled only when a row's maximum outgrows
 //     its reference by 2^8. (Two threads per row halve nothing: the softmax is bound by its instructions, the exchange and
-//     the doubled bookkeeping cost a tenth.) P is rounded to the element type (its sum is not). 3 of 8 pairs
+//     the doubled bookkeeping cost a tenth.) P is rounded to the element type (its sum is not). 1 of 8 pairs
 //     take a polynomial on the FMA pipe instead of ex2, the narrowest unit.
 //   * Every wait is bounded and reports through the status word; tensor memory is freed on every path.
 #pragma once
@@ -31,7 +31,7 @@ namespace hkv {
 constexpr int kCkRows = 128, kCkKeys = 128;
 constexpr int kCkStages = 2;              // K tiles and V tiles in flight
 constexpr int kCkThreads = 384;
-constexpr int kCkEmuOf8 = 3;              // pairs of every 8 whose exp2 runs on the FMA pipe
+constexpr int kCkEmuOf8 = 1;              // pairs of every 8 whose exp2 runs on the FMA pipe (0, 1, 2, 3: 823, 788, 864, 915 us for 2 048 queries over 32k keys)
 constexpr int kCkDesc = 16;               // words of a work descriptor
 // A row sum beyond this comes from a score that is not a number: sums of n probabilities stay below n * 2^8.
 constexpr float kSumLimit = 1.0e30f;
@@ -218,7 +218,7 @@ hkv_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     auto queue_wait = [&](uint32_t k) -> bool { return mbar_wait(B_WF + 8 * (k & 3), (k >> 2) & 1, bt.status); };
 
     if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     if (warp == 8) {
         // ------------------------------ producer (the whole warp) ------------------------------
         uint32_t gt = 0, it = 0;
@@ -387,7 +387,7 @@ hkv_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         }
     }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         // ------------------------------ softmax / output rows ------------------------------
         const int quad = warp & 3, grp = warp >> 2;
         const int row = quad * 32 + lane;          // row of the tile = lane of tensor memory
@@ -511,6 +511,7 @@ hkv_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             if (!ok) continue;
             tc_fence_after();
             const bool row_valid = ql < a.QT && qi < q.n;
+            if (m_ref == kLow) l_run = 0.0f;       // every score was masked: what the polynomial makes of -infinity is no weight
             const float inv = l_run == 0.0f ? 0.0f : (l_run < kSumLimit ? 1.0f / l_run : NAN);
             float* prow = slot >= 0 ? a.part + ((long long)slot * (2 * kCkRows) + grp * kCkRows + row) * (D + 4) : nullptr;
             T* op = (T*)a.t.out + ((long long)(q.start + qi) * H + (long long)kvh * G + g) * D;

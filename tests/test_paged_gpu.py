@@ -291,14 +291,15 @@ def test_attention_window(hkv, cuda, heads, window):
     run_attention(hkv, cuda, heads=heads, page=64, steps=[1, 150, 300], keys=[700, 150, 901], window=window, dtype="bfloat16")
 
 
+@pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("causal", [True, False], ids=["causal", "cross"])
 @pytest.mark.parametrize("heads", [(28, 4, 128), (8, 8, 96), (16, 8, 256), (6, 2, 80)], ids=str)
-def test_attention_rows_that_attend_nothing(hkv, cuda, heads, causal):
+def test_attention_rows_that_attend_nothing(hkv, cuda, heads, causal, dtype):
     """More queries than cached positions (causal: the first ones sit before position 0), and no cached position at all:
     zero rows."""
     torch = cuda
     steps, keys = [5, 200, 1, 40, 2], [2, 150, 0, 0, 1]
-    out = run_attention(hkv, torch, heads=heads, page=16, steps=steps, keys=keys, causal=causal)
+    out = run_attention(hkv, torch, heads=heads, page=16, steps=steps, keys=keys, causal=causal, dtype=dtype)
     assert (out[206:246] == 0).all() and (out[205] == 0).all()
     if causal:
         assert (out[:3] == 0).all() and (out[5:55] == 0).all()
