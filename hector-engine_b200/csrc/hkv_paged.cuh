@@ -89,6 +89,11 @@ __device__ __forceinline__ void paged_key_range(const PagedBatch& a, const Paged
     }
 }
 
+// ---- launches that overlap --------------------------------------------------------------------------------------------
+// The dependent launch may be set up from here on; it waits for this one's end before it reads anything.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---- scans of a block -----------------------------------------------------------------------------------------------
 // Exclusive prefix sum of one value per thread over the block (at most 1024 threads); `total` gets the sum.
 // `buf` holds 33 values; ends with the block synchronised.
@@ -415,9 +420,11 @@ struct PagedAttnArgs {
 };
 constexpr int kPagedGenWarps = 4;
 constexpr float kLow = -3.3e38f;          // start of a running maximum: below every score that is finite
+// A row sum beyond this comes from a score that is not a number: sums of n probabilities stay below n * 2^8.
+constexpr float kSumLimit = 1.0e30f;
 
-// One output row: query i of request r (packed row t), head h. The whole block takes part.
-template <typename T>
+// One output row: query i of request r (packed row t), head h. The whole block of WARPS warps takes part.
+template <typename T, int WARPS>
 __device__ __forceinline__ void paged_row(const PagedAttnArgs& a, const int r, const PagedRequest& rq, const int i, const int h) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long t = rq.start + i;
@@ -434,7 +441,7 @@ __device__ __forceinline__ void paged_row(const PagedAttnArgs& a, const int r, c
     }
     float m = kLow, l = 0.0f;
     const int32_t* table = a.b.table + (long long)r * a.b.cols;
-    for (int s = k_lo + warp; s < k_hi; s += kPagedGenWarps) {
+    for (int s = k_lo + warp; s < k_hi; s += WARPS) {
         const int pg = table[s / a.b.page];
         const bool in = pg >= 0 && pg < a.b.pages;   // an entry outside the planes: rows of zeros
         if (!in && lane == 0) atomicOr(a.b.status, kStatusBoundCheck);
@@ -460,24 +467,24 @@ __device__ __forceinline__ void paged_row(const PagedAttnArgs& a, const int r, c
         }
         m = mn;
     }
-    __shared__ float s_m[kPagedGenWarps], s_l[kPagedGenWarps];
-    __shared__ float s_acc[kPagedGenWarps][512];
+    __shared__ float s_m[WARPS], s_l[WARPS];
+    __shared__ float s_acc[WARPS][512];
     if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
 #pragma unroll
     for (int e = 0; e < 16; ++e) s_acc[warp][lane + 32 * e] = acc[e];
     __syncthreads();
     float gm = s_m[0];
 #pragma unroll
-    for (int w = 1; w < kPagedGenWarps; ++w) gm = fmaxf(gm, s_m[w]);
+    for (int w = 1; w < WARPS; ++w) gm = fmaxf(gm, s_m[w]);
     float gl = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kPagedGenWarps; ++w) gl += s_l[w] * exp2f(s_m[w] - gm);
+    for (int w = 0; w < WARPS; ++w) gl += s_l[w] * exp2f(s_m[w] - gm);
     const float inv = gl > 0.0f ? 1.0f / gl : 0.0f;
     T* op = (T*)a.out + (t * a.H + h) * a.HD;
-    for (int d = threadIdx.x; d < a.HD; d += kPagedGenWarps * 32) {
+    for (int d = threadIdx.x; d < a.HD; d += WARPS * 32) {
         float o = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kPagedGenWarps; ++w) o += s_acc[w][d] * exp2f(s_m[w] - gm);
+        for (int w = 0; w < WARPS; ++w) o += s_acc[w][d] * exp2f(s_m[w] - gm);
         op[d] = from_f32<T>(o * inv);
     }
     __syncthreads();
@@ -494,7 +501,7 @@ __global__ void __launch_bounds__(kPagedGenWarps * 32) hkv_paged_generic_kernel(
     const PagedRequest rq = paged_request(a.b, lo);
     const int i = t - rq.start;
     if (i < 0 || i >= rq.n) return;                  // a row of no query
-    paged_row<T>(a, lo, rq, i, blockIdx.y);
+    paged_row<T, kPagedGenWarps>(a, lo, rq, i, blockIdx.y);
 }
 
 // Work to be done again: the staged kernels drop values of V that are not finite where only some queries of an item look
@@ -511,24 +518,32 @@ struct PagedFix {
     }
 };
 
-// The rows of those items, key by key, so that each query sees exactly its own keys. Returns at once in any other call.
-// The last CTA to finish empties the list.
-template <typename T>
-__global__ void __launch_bounds__(kPagedGenWarps * 32) hkv_paged_fix_kernel(const PagedAttnArgs a, const PagedFix fix, const int QB) {
-    const int count = *reinterpret_cast<volatile int*>(fix.head);
-    if (count == 0) return;
+// Whether an item is on the list of `count` entries.
+__device__ __forceinline__ bool paged_to_fix(const PagedFix& f, const int count, const int r, const int block, const int kvh) {
+    if (count > kFixMax) return true;
+    for (int e = 0; e < count; ++e) {
+        const int4 x = f.items[e];
+        if (x.x == r && x.y == block && x.z == kvh) return true;
+    }
+    return false;
+}
+// The rows of the listed items, key by key, so that each query sees exactly its own keys; all blocks of the grid take
+// part, the last one to finish empties the list. Blocks of WARPS warps; only called where count > 0.
+template <typename T, int WARPS>
+__device__ __noinline__ void paged_fix_rows(const PagedAttnArgs& a, const PagedFix& fix, const int count, const int QB) {
     const int G = a.H / a.KVH;
     if (count <= kFixMax) {
         for (int e = 0; e < count; ++e) {
             const int4 item = fix.items[e];
+            if (item.x >= a.b.requests) continue;    // left behind by a call whose second launch failed
             const PagedRequest rq = paged_request(a.b, item.x);
             const int i0 = item.y < 0 ? 0 : item.y * QB, i1 = item.y < 0 || i0 + QB > rq.n ? rq.n : i0 + QB;
-            for (int x = blockIdx.x; x < (i1 - i0) * G; x += gridDim.x) paged_row<T>(a, item.x, rq, i0 + x / G, item.z * G + x % G);
+            for (int x = blockIdx.x; x < (i1 - i0) * G; x += gridDim.x) paged_row<T, WARPS>(a, item.x, rq, i0 + x / G, item.z * G + x % G);
         }
     } else {
         for (int r = 0; r < a.b.requests; ++r) {
             const PagedRequest rq = paged_request(a.b, r);
-            for (long long x = blockIdx.x; x < (long long)rq.n * a.H; x += gridDim.x) paged_row<T>(a, r, rq, (int)(x / a.H), (int)(x % a.H));
+            for (long long x = blockIdx.x; x < (long long)rq.n * a.H; x += gridDim.x) paged_row<T, WARPS>(a, r, rq, (int)(x / a.H), (int)(x % a.H));
         }
     }
     __syncthreads();

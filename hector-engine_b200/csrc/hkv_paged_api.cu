@@ -14,6 +14,7 @@
 #include "hkv_paged.cuh"
 #include "hkv_paged_chunk.cuh"
 #include "hkv_paged_decode.cuh"
+#include "hkv_paged_finish.cuh"
 #include "hkv_paged_rope.cuh"
 #include "hkv_paged_wide.cuh"
 
@@ -209,7 +210,7 @@ DecodeShape decode_shape(const hkv_paged_ctx* c, int cols, int requests) {
     return s;
 }
 
-int launch_small(hkv_paged_ctx* c, const PagedAttnArgs& t, int cols, cudaStream_t st) {
+int launch_small(hkv_paged_ctx* c, const PagedAttnArgs& t, int cols, PagedFinishArgs& f, cudaStream_t st) {
     const hkv_paged_geometry& g = c->g;
     const DecodeShape s = decode_shape(c, cols, t.b.requests);
     if (s.plan.stages < 2) return fail(c, HKV_ERR_GEOMETRY, "attention: shared memory too small for two stages");
@@ -228,18 +229,10 @@ int launch_small(hkv_paged_ctx* c, const PagedAttnArgs& t, int cols, cudaStream_
     if (!e) e = encode_plane(c, t.v_cache, width, a.box_rows, &mv);
     if (e) return e;
     pick_decode(g.dtype, g.head_dim, cols > 8 ? 2 : 1, s.groups)<<<s.grid, (s.groups * 4 + 1) * 32, s.plan.bytes, st>>>(mk, mv, a, s.plan.stages);
-    PagedMergeArgs m{};
-    m.b = t.b;
-    m.part = c->part;
-    m.cuts = c->cuts;
-    m.out = t.out;
-    m.H = t.H;
-    m.KVH = t.KVH;
-    m.HD = t.HD;
-    m.cols = cols;
-    const dim3 grid((unsigned)(s.grid / s.gang), (unsigned)t.KVH, (unsigned)cols);
-    if (g.dtype == HKV_DTYPE_F16) hkv_paged_merge_kernel<__half><<<grid, 256, 0, st>>>(m);
-    else hkv_paged_merge_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(m);
+    f.small_part = c->part;
+    f.small_cuts = c->cuts;
+    f.spans = s.grid / s.gang;
+    f.cols = cols;
     return launched(c, "attention launch");
 }
 
@@ -272,7 +265,7 @@ int line_shift(const hkv_paged_geometry& g, int QB) {
     return shift;
 }
 
-int launch_chunk(hkv_paged_ctx* c, const PagedAttnArgs& t, const void* q, int small, cudaStream_t st) {
+int launch_chunk(hkv_paged_ctx* c, const PagedAttnArgs& t, const void* q, int small, PagedFinishArgs& f, cudaStream_t st) {
     const hkv_paged_geometry& g = c->g;
     const int G = g.num_heads / g.num_kv_heads;
     PagedChunkArgs a{};
@@ -308,27 +301,27 @@ int launch_chunk(hkv_paged_ctx* c, const PagedAttnArgs& t, const void* q, int sm
         if (r != CUDA_SUCCESS) return fail(c, HKV_ERR_CUDA, "cuTensorMapEncodeTiled failed (queries)");
         pick_chunk(g.dtype, g.head_dim)<<<c->sm_count, kCkThreads, smem, st>>>(mq, mk, mv, a);
     }
-    PagedChunkMergeArgs m{};
-    m.b = t.b;
-    m.part = c->chunk_part;
-    m.cuts = c->chunk_cuts;
-    m.out = t.out;
-    m.H = t.H;
-    m.KVH = t.KVH;
-    m.HD = t.HD;
-    m.QT = a.QT;
-    m.QB = a.line.QB;
-    m.tiles = wide(g) ? 1 : 2;
-    const dim3 grid((unsigned)c->sm_count, 8);
-    if (g.dtype == HKV_DTYPE_F16) hkv_paged_chunk_merge_kernel<__half><<<grid, 256, 0, st>>>(m);
-    else hkv_paged_chunk_merge_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(m);
+    f.chunk_part = c->chunk_part;
+    f.chunk_cuts = c->chunk_cuts;
+    f.ctas = c->sm_count;
+    f.tiles = wide(g) ? 1 : 2;
+    f.QT = a.QT;
     return launched(c, "attention launch");
 }
 
-int launch_fix(hkv_paged_ctx* c, const PagedAttnArgs& t, int QB, cudaStream_t st) {
-    if (c->g.dtype == HKV_DTYPE_F16) hkv_paged_fix_kernel<__half><<<c->sm_count, kPagedGenWarps * 32, 0, st>>>(t, fix_of(c), QB);
-    else hkv_paged_fix_kernel<__nv_bfloat16><<<c->sm_count, kPagedGenWarps * 32, 0, st>>>(t, fix_of(c), QB);
-    return launched(c, "attention launch");
+int launch_finish(hkv_paged_ctx* c, const PagedFinishArgs& f, cudaStream_t st) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)finish_blocks(f, c->g.num_kv_heads));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = c->g.dtype == HKV_DTYPE_F16 ? cudaLaunchKernelEx(&cfg, hkv_paged_finish_kernel<__half>, f)
+                                                       : cudaLaunchKernelEx(&cfg, hkv_paged_finish_kernel<__nv_bfloat16>, f);
+    return e == cudaSuccess ? HKV_OK : fail_cuda(c, e, "attention finish launch");
 }
 
 template <typename T>
@@ -401,13 +394,19 @@ int attention(hkv_paged_ctx* c, const void* q, int64_t q_token_stride, const voi
     if (staged && (only_small || scale > 0.0f)) {
         // Query rows per KV head of the few-token kernel: all that the call can have, or, beside the prompt kernel, as many
         // tokens as fit one n8 tile (16 rows where a single token has more than 8): with two tiles every request of the
-        // launch pays for the registers (head_dim 256: one consumer group instead of two).
-        const int small = only_small ? max_step * G : G <= 8 ? 8 / G * G : G <= kSmallCols ? G : 0;
+        // launch pays for the registers (head_dim 256: one consumer group instead of two). A call whose requests have 64
+        // tokens or more on average leaves it out: single tokens among such prompts cost the prompt kernel a fraction of
+        // them, an empty launch costs 6 us.
+        const int small = only_small ? max_step * G : tokens / 64 >= requests ? 0 : G <= 8 ? 8 / G * G : G <= kSmallCols ? G : 0;
+        PagedFinishArgs f{};
+        f.t = a;
+        f.fix = fix_of(c);
+        f.QB = block_queries(g);
+        f.may_fix = max_step > 1 ? 1 : 0;                // (nothing is hidden from a single query)
         int e = HKV_OK;
-        if (small) e = launch_small(c, a, small, st);
-        if (!e && !only_small) e = launch_chunk(c, a, q, small, st);
-        if (!e && max_step > 1) e = launch_fix(c, a, block_queries(g), st);   // (nothing is hidden from a single query)
-        return e;
+        if (small) e = launch_small(c, a, small, f, st);
+        if (!e && !only_small) e = launch_chunk(c, a, q, small, f, st);
+        return e ? e : launch_finish(c, f, st);
     }
     const dim3 grid((unsigned)tokens, (unsigned)g.num_heads);
     if (g.dtype == HKV_DTYPE_F16) hkv_paged_generic_kernel<__half><<<grid, kPagedGenWarps * 32, 0, st>>>(a);

@@ -33,8 +33,6 @@ constexpr int kCkStages = 2;              // K tiles and V tiles in flight
 constexpr int kCkThreads = 384;
 constexpr int kCkEmuOf8 = 1;              // pairs of every 8 whose exp2 runs on the FMA pipe (0, 1, 2, 3: 823, 788, 864, 915 us for 2 048 queries over 32k keys)
 constexpr int kCkDesc = 16;               // words of a work descriptor
-// A row sum beyond this comes from a score that is not a number: sums of n probabilities stay below n * 2^8.
-constexpr float kSumLimit = 1.0e30f;
 
 struct PagedChunkArgs {
     PagedAttnArgs t;
@@ -193,6 +191,7 @@ hkv_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     const int G = a.line.G, H = a.t.H, D = a.t.HD;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    launch_dependents();
     if (tid == 0) {
         mbar_init(B_QFULL, 1); mbar_init(B_QEMPTY, 1); mbar_init(B_DONE, 1);
         for (int s = 0; s < kCkStages; ++s) {
@@ -544,69 +543,6 @@ hkv_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     tc_fence_before();
     __syncthreads();
     if (warp == 9) tmem_dealloc(tmem, TMEM_COLS);
-}
-
-// ---------------------------------------------------------------------------------------------------------------------
-// Merge of the items that were cut, one warp per row: blockIdx.x = the CTA whose entry names an item, blockIdx.y = a
-// share of its rows. `tiles` tiles of 128 rows per item.
-// ---------------------------------------------------------------------------------------------------------------------
-struct PagedChunkMergeArgs {
-    PagedBatch b;
-    const float* part;
-    const int4* cuts;
-    void* out;
-    int H, KVH, HD, QT, QB, tiles;
-};
-template <typename T>
-__global__ void __launch_bounds__(256) hkv_paged_chunk_merge_kernel(const PagedChunkMergeArgs a) {
-    const int4 cut = a.cuts[blockIdx.x];
-    const int parts = cut.w;
-    if (parts <= 1) return;
-    const PagedRequest q = paged_request(a.b, cut.x);
-    const int G = a.H / a.KVH, HD = a.HD, PW = HD + 4, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int row = blockIdx.y * 8 + warp; row < a.tiles * 128; row += gridDim.y * 8) {
-        const int ql = row % 128 / G, i = cut.z * a.QB + row / 128 * a.QT + ql;
-        if (ql >= a.QT || i >= q.n) continue;
-        // part 0 sits in this CTA's second slot, the others in the first slots of the CTAs behind it
-        const float* base = a.part + (long long)row * PW;
-        const long long set = (long long)a.tiles * 128 * PW;
-        float M = kLow, L = 0.0f;
-        float2 acc[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] = make_float2(0.0f, 0.0f);
-        for (int p0 = 0; p0 < parts; p0 += 2) {
-            float2 ml[2], x[2][4];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int pt = p0 + u;
-                const float* r = base + (2ll * (blockIdx.x + pt) + (pt == 0 ? 1 : 0)) * set;
-                ml[u] = pt < parts ? *reinterpret_cast<const float2*>(r + HD) : make_float2(kLow, 0.0f);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int d = 2 * lane + 64 * e;
-                    x[u][e] = pt < parts && d < HD ? *reinterpret_cast<const float2*>(r + d) : make_float2(0.0f, 0.0f);
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const float Mn = fmaxf(M, ml[u].x), keep = exp2f(M - Mn), w = exp2f(ml[u].x - Mn);
-                L = fmaf(ml[u].y, w, L * keep);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    acc[e].x = fmaf(x[u][e].x, w, acc[e].x * keep);
-                    acc[e].y = fmaf(x[u][e].y, w, acc[e].y * keep);
-                }
-                M = Mn;
-            }
-        }
-        const float inv = L == 0.0f ? 0.0f : (L < kSumLimit ? 1.0f / L : NAN);
-        T* op = (T*)a.out + ((long long)(q.start + i) * a.H + (long long)cut.y * G + row % 128 % G) * HD;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int d = 2 * lane + 64 * e;
-            if (d < HD) *reinterpret_cast<uint32_t*>(op + d) = pack2<T>(acc[e].x * inv, acc[e].y * inv);
-        }
-    }
 }
 
 }  // namespace hkv

@@ -35,7 +35,7 @@ __host__ __device__ constexpr int paged_chunk_width(int HD) { return HD % 64 == 
 struct PagedDecodeArgs {
     PagedAttnArgs t;
     float* part;          // [2 * spans][KVH][cols][HD + 2]: o, maximum (log2 domain), sum
-    int4* cuts;           // [spans]: request that starts in this span and goes on behind it: {request, spans, -, -}; spans 0: none
+    int4* cuts;           // [spans]: request that starts in this span and goes on behind it: {request, spans, first packed row, queries}; spans 0: none
     PagedFix fix;
     int gang, cols;       // cols = query rows per KV head that the partial rows hold
     int box_rows, pieces; // rows of a box, boxes per tile and column block
@@ -120,6 +120,7 @@ hkv_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + kPagedMaxStages);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
+    launch_dependents();
     if (tid == 0) {
         for (int s = 0; s < stages; ++s) {
             mbar_init(full0 + 8 * s, 1);
@@ -187,8 +188,8 @@ hkv_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                 if (prefix[mid] <= u1 - 1) lo = mid; else hi = mid - 1;
             }
             if (prefix[lo] >= u0 && prefix[lo + 1] > u1) {
-                cut.x = lo;
-                cut.y = span_owner(prefix[lo + 1] - 1, W, NS) - span + 1;
+                const PagedRequest q = paged_request(bt, lo);
+                cut = make_int4(lo, span_owner(prefix[lo + 1] - 1, W, NS) - span + 1, q.start, q.n);
             }
         }
         a.cuts[span] = cut;
@@ -481,87 +482,6 @@ hkv_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
             }
         }
         named_bar_sync(1, NCW * 32);
-    }
-}
-
-// ---------------------------------------------------------------------------------------------------------------------
-// Merge of the requests that were cut: o = sum 2^(m_c - M) o_c / sum 2^(m_c - M) l_c. A CTA per (span whose entry names a
-// request, KV head, query row); eight warps deal the parts among them, a lane holds the dimensions 2*lane, 2*lane+64, ...
-// ---------------------------------------------------------------------------------------------------------------------
-struct PagedMergeArgs {
-    PagedBatch b;
-    const float* part;
-    const int4* cuts;
-    void* out;
-    int H, KVH, HD, cols;
-};
-template <typename T>
-__global__ void __launch_bounds__(256) hkv_paged_merge_kernel(const PagedMergeArgs a) {
-    const int4 cut = a.cuts[blockIdx.x];
-    if (cut.y <= 1) return;
-    const int G = a.H / a.KVH, kvh = blockIdx.y, HD = a.HD;
-    const PagedRequest q = paged_request(a.b, cut.x);
-    const int ncol = q.n * G;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, parts = cut.y;
-    __shared__ float s_o[8][256];
-    __shared__ float s_m[8], s_l[8];
-    for (int c = blockIdx.z; c < ncol; c += gridDim.z) {
-        float M = kLow, L = 0.0f;
-        float2 acc[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = make_float2(0.0f, 0.0f);
-        for (int p0 = warp; p0 < parts; p0 += 16) {
-            float2 ml[2], x[2][4];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int p = p0 + 8 * u;
-                const int slot = 2 * (blockIdx.x + p) + (p == 0 ? 1 : 0);
-                const float* row = a.part + (((long long)slot * a.KVH + kvh) * a.cols + c) * (HD + 2);
-                ml[u] = make_float2(kLow, 0.0f);
-                if (p < parts) ml[u] = *reinterpret_cast<const float2*>(row + HD);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int d = 2 * lane + 64 * i;
-                    x[u][i] = p < parts && d < HD ? *reinterpret_cast<const float2*>(row + d) : make_float2(0.0f, 0.0f);
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const float Mn = fmaxf(M, ml[u].x), keep = exp2f(M - Mn), w = exp2f(ml[u].x - Mn);
-                L = fmaf(ml[u].y, w, L * keep);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    acc[i].x = fmaf(x[u][i].x, w, acc[i].x * keep);
-                    acc[i].y = fmaf(x[u][i].y, w, acc[i].y * keep);
-                }
-                M = Mn;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int d = 2 * lane + 64 * i;
-            if (d < HD) *reinterpret_cast<float2*>(&s_o[warp][d]) = acc[i];
-        }
-        if (lane == 0) { s_m[warp] = M; s_l[warp] = L; }
-        __syncthreads();
-        float Mx = s_m[0];
-#pragma unroll
-        for (int w = 1; w < 8; ++w) Mx = fmaxf(Mx, s_m[w]);
-        float f[8], Lx = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 8; ++w) {
-            f[w] = exp2f(s_m[w] - Mx);
-            Lx = fmaf(s_l[w], f[w], Lx);
-        }
-        const float inv = Lx > 0.0f ? 1.0f / Lx : 0.0f;
-        T* op = (T*)a.out + ((long long)(q.start + c / G) * a.H + (long long)kvh * G + c % G) * HD;
-        for (int d = threadIdx.x; d < HD; d += 256) {
-            float o = 0.0f;
-#pragma unroll
-            for (int w = 0; w < 8; ++w) o = fmaf(s_o[w][d], f[w], o);
-            op[d] = from_f32<T>(o * inv);
-        }
-        __syncthreads();
     }
 }
 

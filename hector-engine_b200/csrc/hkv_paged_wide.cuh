@@ -51,6 +51,7 @@ hkv_paged_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
     const int G = a.line.G, H = a.t.H;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    launch_dependents();
     if (tid == 0) {
         mbar_init(B_QFULL, 256); mbar_init(B_PFULL, 256); mbar_init(B_PV, 1); mbar_init(B_OFULL, 1); mbar_init(B_DONE, 1);
         mbar_init(B_XCH, 256);
@@ -232,10 +233,10 @@ hkv_paged_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                 tc_fence_before();
                 mbar_arrive(B_QFULL);
             }
-            int lo_row, hi_row, lo_first, hi_first, lo_last, hi_last;
+            int lo_row, hi_row, lo_last, hi_first, x;
             paged_key_range(bt, q, qi < q.n ? qi : q.n - 1, lo_row, hi_row);
-            paged_key_range(bt, q, i0, lo_first, hi_first);
-            paged_key_range(bt, q, (i0 + a.line.QB < q.n ? i0 + a.line.QB : q.n) - 1, lo_last, hi_last);
+            paged_key_range(bt, q, i0, x, hi_first);
+            paged_key_range(bt, q, (i0 + a.line.QB < q.n ? i0 + a.line.QB : q.n) - 1, lo_last, x);
             float m_ref = kLow, l_run = 0.0f;
 
             for (int t = 0; t < nt; ++t, ++gt) {
@@ -310,23 +311,8 @@ hkv_paged_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                     const uint32_t vs = gt % kWdStages;
                     ok = __all_sync(0xffffffffu, mbar_wait(B_VFULL + 8 * vs, (gt / kWdStages) & 1, bt.status));
                     if (!ok) continue;
-                    uint8_t* vt = v_gen + (size_t)vs * TILE_BYTES;
-                    const int head = lo_last - kstart < 0 ? 0 : (lo_last - kstart < kWdKeys ? lo_last - kstart : kWdKeys);
-                    int tail = hi_first - kstart < 0 ? 0 : (hi_first - kstart < kWdKeys ? hi_first - kstart : kWdKeys);
-                    if (tail < head) tail = head;
-                    bool bad = false;
-                    for (int idx = tid; idx < (head + kWdKeys - tail) * 8 * NCH; idx += 256) {
-                        const int k = idx / (8 * NCH), u = idx % (8 * NCH);
-                        const int vr = k < head ? k : tail + k - head, pos = kstart + vr;
-                        uint4* at = reinterpret_cast<uint4*>(vt + (u / 8) * CHUNK_BYTES + vr * 128 + (u % 8) * 16);
-                        uint4 x = make_uint4(0, 0, 0, 0);
-                        if (pos >= lo_first && pos < hi_last) {
-                            x = *at;
-                            if (!drop_nonfinite<T>(x)) continue;
-                            bad = true;
-                        }
-                        *at = x;
-                    }
+                    const bool bad = clean_values<T, NCH, 256>(bt, q, i0, a.line.QB, kstart, kWdKeys, v_gen + (size_t)vs * TILE_BYTES,
+                                                               CHUNK_BYTES, tid);
                     if (__any_sync(0xffffffffu, bad) && lane == 0) a.fix.push(r, p, kvh);
                     fence_proxy_async_smem();
                 }
