@@ -44,18 +44,20 @@ hkv_paged_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
     uint32_t* pre = reinterpret_cast<uint32_t*>(xch + 6 * kCkRows);            // [requests + 1]
     __shared__ long long scan_buf[33];
     const uint32_t k_smem = smem_u32(smem), v_smem = smem_u32(v_gen), bar0 = smem_u32(bars);
-    const uint32_t B_QFULL = bar0, B_PFULL = bar0 + 8, B_PV = bar0 + 16, B_OFULL = bar0 + 24, B_DONE = bar0 + 32, B_XCH = bar0 + 40,
+    const uint32_t B_QFULL = bar0, B_PV = bar0 + 16, B_OFULL = bar0 + 24, B_DONE = bar0 + 32, B_XCH = bar0 + 40,
                    B_SFULL = bar0 + 48 /* [2] */, B_KFULL = bar0 + 64 /* [3] */, B_KEMPTY = bar0 + 88, B_VFULL = bar0 + 112,
-                   B_VEMPTY = bar0 + 136, B_WF = bar0 + 160 /* [4] */, B_WE = bar0 + 192;
+                   B_VEMPTY = bar0 + 136, B_WF = bar0 + 160 /* [4] */, B_WE = bar0 + 192,
+                   // one per score buffer: P(t+1) may be complete before the issuer, held up by V(t), looks for P(t)
+                   B_PFULL = bar0 + 224 /* [2] */;
     const PagedBatch& bt = a.t.b;
     const int G = a.line.G, H = a.t.H;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     launch_dependents();
     if (tid == 0) {
-        mbar_init(B_QFULL, 256); mbar_init(B_PFULL, 256); mbar_init(B_PV, 1); mbar_init(B_OFULL, 1); mbar_init(B_DONE, 1);
+        mbar_init(B_QFULL, 256); mbar_init(B_PV, 1); mbar_init(B_OFULL, 1); mbar_init(B_DONE, 1);
         mbar_init(B_XCH, 256);
-        for (int s = 0; s < 2; ++s) mbar_init(B_SFULL + 8 * s, 1);
+        for (int s = 0; s < 2; ++s) { mbar_init(B_SFULL + 8 * s, 1); mbar_init(B_PFULL + 8 * s, 256); }
         for (int s = 0; s < kWdStages; ++s) {
             mbar_init(B_KFULL + 8 * s, 1); mbar_init(B_KEMPTY + 8 * s, 1);
             mbar_init(B_VFULL + 8 * s, 1); mbar_init(B_VEMPTY + 8 * s, 1);
@@ -177,7 +179,7 @@ hkv_paged_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                 if (!issue_qk(gt) || (nt > 1 && !issue_qk(gt + 1))) { ok = false; break; }
                 for (int t = 0; t < nt; ++t, ++gt) {
                     const uint32_t s = gt % kWdStages;
-                    if (!mbar_wait(B_VFULL + 8 * s, (gt / kWdStages) & 1, bt.status) || !mbar_wait(B_PFULL, gt & 1, bt.status)) { ok = false; break; }
+                    if (!mbar_wait(B_VFULL + 8 * s, (gt / kWdStages) & 1, bt.status) || !mbar_wait(B_PFULL + 8 * (gt & 1), (gt >> 1) & 1, bt.status)) { ok = false; break; }
                     tc_fence_after();
                     const uint32_t vd = v_lo + ((s * TILE_BYTES) >> 4), pbase = tmem + COL_S + 64u * (gt & 1), o = tmem + COL_O;
                     if (t > 0) tc_mma_ts_i<true>(o, pbase, vd, desc_hi, IDESC_PV);
@@ -317,7 +319,7 @@ hkv_paged_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                     fence_proxy_async_smem();
                 }
                 tc_fence_before();
-                mbar_arrive(B_PFULL);
+                mbar_arrive(B_PFULL + 8 * sb);
             }
             float l_tot = l_run;
             if (ok) {                              // sum of both halves (same reference)

@@ -492,3 +492,191 @@ def test_empty_calls_do_nothing(hkv, cuda):
     for t in (kc, vc, out):
         assert (t == 7).all()
     ctx.close()
+
+
+# ---- the operators together -------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("heads,dtype,window", [((28, 4, 128), "float16", 0), ((14, 2, 64), "bfloat16", 40), ((16, 8, 256), "bfloat16", 0),
+                                                ((6, 2, 80), "float16", 0)], ids=str)
+def test_serving_steps_captured_and_replayed(hkv, cuda, heads, dtype, window):
+    """A serving loop of two layers: plan, norm + rotary positions into the pages, attention, all captured once on a side
+    stream and replayed with other lengths every step (joins, chunks, single tokens, requests that do not fit), releases
+    in between. Every step's tables, cache rows and outputs are held against the models."""
+    torch = cuda
+    H, KVH, HD = heads
+    D = dt(torch, dtype)
+    R, page, cols, num_pages, T, layers, most = 11, 16, 20, 90, 160, 2, 64
+    rot, sections = HD // 2 // 16 * 32, None
+    sections = [rot // 2 - 2 * (rot // 8), rot // 8, rot // 8]
+    gen = torch.Generator().manual_seed(HD)
+    rng = np.random.default_rng(HD)
+    ctx = hkv.PagedContext(hkv.PagedGeometry(num_heads=H, num_kv_heads=KVH, head_dim=HD, page_size=page, num_pages=num_pages,
+                                             max_requests=R, max_pages=cols, max_tokens=T, window_size=window, dtype=dtype))
+    step = ctx.new_step(R, T)
+    z = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")
+    lens, new, gone, pos3 = z(R), z(R), z(R), z(3, T)
+    table, free, count = z(R, cols) - 1, torch.arange(num_pages, dtype=torch.int32, device="cuda"), i32(torch, [num_pages])
+    qkv = [torch.zeros(T, (H + 2 * KVH) * HD, dtype=D, device="cuda") for _ in range(layers)]
+    planes = [[torch.zeros(num_pages, page, KVH, HD, dtype=D, device="cuda") for _ in range(2)] for _ in range(layers)]
+    turned = [torch.zeros(T, H, HD, dtype=D, device="cuda") for _ in range(layers)]
+    outs = [torch.zeros(T, H, HD, dtype=D, device="cuda") for _ in range(layers)]
+    qw, kw = ((1 + 0.2 * torch.randn(HD, generator=gen)).to(D).cuda() for _ in range(2))
+    offsets = i32(torch, [[0], [5], [9]])
+    rope = dict(q_norm_w=qw, k_norm_w=kw, sections=sections, rotary_dim=rot, theta=1e6)
+
+    def one_step():
+        ctx.plan(lens, new, table, free, count, step, total_len=lens, free_left=count)
+        torch.add(step.positions, offsets, out=pos3)
+        for n in range(layers):
+            q, k, v = (x.unflatten(1, (-1, HD)) for x in qkv[n].split([H * HD, KVH * HD, KVH * HD], 1))
+            ctx.norm_rope(q, k, v, pos3, slots=step.slots, k_cache=planes[n][0], v_cache=planes[n][1], q_out=turned[n], **rope)
+            ctx.attention(turned[n], planes[n][0], planes[n][1], outs[n], table, step.q_start, step.step_len, lens, max_step=most)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        one_step()                                       # no tokens yet: nothing happens
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            one_step()
+    torch.cuda.current_stream().wait_stream(side)
+    for it in range(9):
+        fresh = rng.choice([0, 1, 1, 1, 2, 3, 40] if it % 3 else [1, 20, 64], R)
+        new.copy_(i32(torch, fresh))
+        for x in qkv:
+            x.copy_(torch.randn(x.shape, generator=gen))
+        before = [[x.clone() for x in pl] for pl in planes]
+        n_lens, n_table, n_free, n_count = lens.cpu().numpy(), table.cpu().numpy(), free.cpu().numpy(), int(count)
+        ref = P.plan_model(n_lens, fresh, n_table, n_free, n_count, page, T)
+        for x in outs:
+            x.fill_(77.0)
+        graph.replay()
+        for name, got in (("table", table), ("q_start", step.q_start), ("step_len", step.step_len), ("total_len", lens),
+                          ("slots", step.slots), ("positions", step.positions)):
+            assert np.array_equal(got.cpu().numpy(), ref[name]), (it, name)
+        assert int(count) == ref["free_left"]
+        keep = step.slots >= 0
+        at = step.slots[keep].long()
+        for n in range(layers):
+            q, k, v = (x.unflatten(1, (-1, HD)) for x in qkv[n].split([H * HD, KVH * HD, KVH * HD], 1))
+            for x, w, got, pick in ((q, qw, turned[n], slice(None)), (k, kw, planes[n][0].view(-1, KVH, HD)[at], keep)):
+                want, size = P.rope_model(torch, x, pos3, w, rot, 3, sections, False, 1e-6, 1e6, 1.0)
+                assert ((got.double() - want[pick]).abs() <= rope_tolerance(torch, D, size[pick])).all(), (it, n)
+            for plane, old in zip(planes[n], before[n]):
+                rest = torch.ones(num_pages * page, dtype=torch.bool, device="cuda")
+                rest[at] = False
+                assert torch.equal(plane.view(-1, KVH, HD)[rest], old.view(-1, KVH, HD)[rest])
+            assert torch.equal(planes[n][1].view(-1, KVH, HD)[at], v[keep])
+            want, tol, live = P.attend_model(torch, turned[n], *planes[n], table, ref["q_start"], ref["step_len"], ref["total_len"],
+                                             ctx.geometry.default_scale, page, window)
+            assert (outs[n][~live] == 77.0).all() and ((outs[n].double() - want).abs() <= tol)[live].all(), (it, n)
+        if it % 2:
+            gone.copy_(i32(torch, rng.random(R) < 0.4))
+            ctx.release(gone, lens, table, free, count)
+    assert ctx.device_status() == 0
+    del graph
+    ctx.close()
+
+
+@pytest.mark.parametrize("heads", [(16, 8, 256), (28, 4, 128), (14, 2, 64)], ids=str)
+def test_attention_many_passes(hkv, cuda, heads):
+    """Hundreds of passes over a ragged windowed batch from two contexts in turn: no wait inside the kernels ever runs out
+    (the order in which copies land differs from pass to pass), and every pass gives the same bits."""
+    torch = cuda
+    H, KVH, HD = heads
+    gen = torch.Generator().manual_seed(2)
+    page, steps = 32, [1, 1, 400, 1, 1, 1, 1, 250] * 4
+    keys = [int(x) for x in torch.randint(2000, 6000, (len(steps),), generator=gen)]
+    cols = max(-(-k // page) for k in keys)
+    num_pages = sum(-(-k // page) for k in keys)
+    kc, vc, table = P.make_pages(torch, gen, keys, page, num_pages, cols, KVH, HD, torch.float16)
+    T = sum(steps)
+    q = torch.randn(T, H, HD, generator=gen).half().cuda()
+    starts = np.concatenate([[0], np.cumsum(steps)])
+    args = (table, i32(torch, starts), i32(torch, steps), i32(torch, keys))
+    ctxs = [hkv.PagedContext(hkv.PagedGeometry(num_heads=H, num_kv_heads=KVH, head_dim=HD, page_size=page, num_pages=num_pages,
+                                               max_requests=len(steps), max_pages=cols, max_tokens=T, window_size=1024)) for _ in range(2)]
+    first, out = torch.empty_like(q), torch.empty_like(q)
+    ctxs[0].attention(q, kc, vc, first, *args, max_step=400)
+    differ = torch.zeros((), dtype=torch.int64, device="cuda")
+    for it in range(300):
+        ctxs[it % 2].attention(q, kc, vc, out, *args, max_step=400)
+        if it % 10 == 9:
+            differ += (out != first).sum()
+    assert [c.device_status() for c in ctxs] == [0, 0]
+    assert int(differ) == 0
+    for c in ctxs:
+        c.close()
+
+
+def test_planes_beyond_2_to_31_elements(hkv, cuda):
+    """Pages at the far end of planes of 2.2e9 elements: append, rotary positions, single tokens and a chunk."""
+    torch = cuda
+    KVH, HD, H, page = 8, 128, 16, 64
+    num_pages = (2_200_000_000 // (KVH * HD * page)) + 1
+    kc, vc = (torch.empty(num_pages, page, KVH, HD, dtype=torch.float16, device="cuda") for _ in range(2))
+    gen = torch.Generator().manual_seed(4)
+    keys, steps = [130, 333], [1, 200]
+    need = [3, 6]
+    ids = torch.cat([torch.arange(num_pages - 8, num_pages), torch.tensor([0])])[torch.randperm(9, generator=gen)].to(torch.int32)
+    table = torch.full((2, 8), -1, dtype=torch.int32)
+    table[0, :3], table[1, :6] = ids[:3], ids[3:]
+    for r in range(2):
+        for j in range(need[r]):
+            for plane in (kc, vc):
+                plane[int(table[r, j])] = torch.randn(page, KVH, HD, generator=gen).half().cuda()
+    T = sum(steps)
+    q, k, v = (torch.randn(T, h, HD, generator=gen).half().cuda() for h in (H, KVH, KVH))
+    slots = i32(torch, [int(table[r, p // page]) * page + p % page for r in range(2) for p in range(keys[r] - steps[r], keys[r])])
+    pos = i32(torch, [p for r in range(2) for p in range(keys[r] - steps[r], keys[r])])
+    for kernel in (0, 1):
+        ctx = hkv.PagedContext(hkv.PagedGeometry(num_heads=H, num_kv_heads=KVH, head_dim=HD, page_size=page, num_pages=num_pages,
+                                                 max_requests=2, max_pages=8, max_tokens=T, kernel_select=kernel))
+        ctx.append(k, v, kc, vc, slots)
+        at = slots.long()
+        assert torch.equal(kc.view(-1, KVH, HD)[at], k) and torch.equal(vc.view(-1, KVH, HD)[at], v)
+        turned = torch.empty_like(q)
+        ctx.norm_rope(q, k, v, pos, slots=slots, k_cache=kc, v_cache=vc, q_out=turned)
+        want, size = P.rope_model(torch, k, pos, None, HD, 1, None, False, 1e-6, 1e4, 1.0)
+        assert ((kc.view(-1, KVH, HD)[at].double() - want).abs() <= rope_tolerance(torch, torch.float16, size)).all()
+        out = torch.empty_like(q)
+        ctx.attention(turned, kc, vc, out, table.cuda(), i32(torch, [0, 1]), i32(torch, steps), i32(torch, keys), max_step=200)
+        ref, tol, live = P.attend_model(torch, turned, kc, vc, table.cuda(), [0, 1], steps, keys, ctx.geometry.default_scale, page)
+        assert live.all() and ((out.double() - ref).abs() <= tol).all()
+        assert ctx.device_status() == 0
+        ctx.close()
+
+
+@pytest.mark.parametrize("steps", [[1], [70]], ids=["token", "chunk"])
+def test_attention_over_a_very_long_request(hkv, cuda, steps):
+    run_attention(hkv, cuda, heads=(14, 2, 64), page=16, steps=steps, keys=[200_003], dtype="bfloat16", poison=False)
+
+
+def test_two_streams_take_two_contexts(hkv, cuda):
+    """Two contexts at work on two streams at once, inputs made on the same streams: both give what one alone gives."""
+    torch = cuda
+    H, KVH, HD, page, steps, keys = 28, 4, 128, 16, [1, 1, 90], [5000, 3000, 4000]
+    gen = torch.Generator().manual_seed(6)
+    cols, num_pages, T = 320, 760, sum(steps)
+    kc, vc, table = P.make_pages(torch, gen, keys, page, num_pages, cols, KVH, HD, torch.float16)
+    q = torch.randn(T, H, HD, generator=gen).half().cuda()
+    args = (table, i32(torch, [0, 1, 2]), i32(torch, steps), i32(torch, keys))
+    make = lambda: hkv.PagedContext(hkv.PagedGeometry(num_heads=H, num_kv_heads=KVH, head_dim=HD, page_size=page, num_pages=num_pages,
+                                                      max_requests=3, max_pages=cols, max_tokens=T))
+    ctxs, streams = [make(), make()], [torch.cuda.Stream(), torch.cuda.Stream()]
+    want = torch.empty_like(q)
+    ctxs[0].attention(q, kc, vc, want, *args, max_step=90)
+    want2 = torch.empty_like(q)
+    ctxs[0].attention(q * 2, kc, vc, want2, *args, max_step=90)
+    torch.cuda.synchronize()
+    outs = [torch.empty_like(q) for _ in range(2)]
+    for _ in range(20):
+        for n, (ctx, st) in enumerate(zip(ctxs, streams)):
+            with torch.cuda.stream(st):
+                outs[n].zero_()
+                ctx.attention(q * (n + 1), kc, vc, outs[n], *args, max_step=90)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want) and torch.equal(outs[1], want2)
+    for ctx, st in zip(ctxs, streams):
+        with torch.cuda.stream(st):
+            assert ctx.device_status() == 0
+        ctx.close()
