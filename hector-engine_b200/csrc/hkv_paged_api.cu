@@ -146,6 +146,23 @@ int encode_plane(hkv_paged_ctx* c, const void* base, int width, int rows, CUtens
     return fail(c, HKV_ERR_CUDA, buf);
 }
 
+// A launch configuration; `early`: it may be set up (and run, up to its own wait) while the launch before it still runs.
+struct Launch {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    Launch(unsigned blocks, unsigned threads, size_t smem, cudaStream_t st, bool early) {
+        cfg.gridDim = dim3(blocks);
+        cfg.blockDim = dim3(threads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = st;
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = early ? 1 : 0;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+    }
+    Launch(const Launch&) = delete;
+};
+
 PagedFix fix_of(const hkv_paged_ctx* c) { return PagedFix{reinterpret_cast<int*>(c->fix), c->fix + 1}; }
 
 typedef void (*DecodeKernel)(const CUtensorMap, const CUtensorMap, const PagedDecodeArgs, const int);
@@ -254,7 +271,7 @@ const void* chunk_kernel(const hkv_paged_geometry& g) {
     if (wide(g)) return g.dtype == HKV_DTYPE_F16 ? (const void*)hkv_paged_wide_kernel<__half> : (const void*)hkv_paged_wide_kernel<__nv_bfloat16>;
     return (const void*)pick_chunk(g.dtype, g.head_dim);
 }
-size_t chunk_part_bytes(const hkv_paged_geometry& g, int sm_count) { return 2ull * sm_count * (wide(g) ? 1 : 2) * kCkRows * (g.head_dim + 4) * sizeof(float); }
+size_t chunk_part_bytes(const hkv_paged_geometry& g, int sm_count) { return 2ull * sm_count * partial_floats((wide(g) ? 1 : 2) * kCkRows, g.head_dim) * sizeof(float); }
 
 // The line's table counts units of 128 << shift keys; the shift keeps the largest batch the context allows inside 31 bits.
 int line_shift(const hkv_paged_geometry& g, int QB) {
@@ -287,9 +304,12 @@ int launch_chunk(hkv_paged_ctx* c, const PagedAttnArgs& t, const void* q, int sm
     if (!e) e = encode_plane(c, t.v_cache, 64, a.box_rows, &mv);
     if (e) return e;
     const size_t smem = chunk_smem(g, t.b.requests);
+    // behind a few-token launch this one starts where that one's CTAs leave room (neither reads what the other writes)
+    const Launch l((unsigned)c->sm_count, wide(g) ? kWdThreads : kCkThreads, smem, st, small > 0);
+    cudaError_t le;
     if (wide(g)) {
-        if (g.dtype == HKV_DTYPE_F16) hkv_paged_wide_kernel<__half><<<c->sm_count, kWdThreads, smem, st>>>(mk, mv, a);
-        else hkv_paged_wide_kernel<__nv_bfloat16><<<c->sm_count, kWdThreads, smem, st>>>(mk, mv, a);
+        le = g.dtype == HKV_DTYPE_F16 ? cudaLaunchKernelEx(&l.cfg, hkv_paged_wide_kernel<__half>, mk, mv, a)
+                                      : cudaLaunchKernelEx(&l.cfg, hkv_paged_wide_kernel<__nv_bfloat16>, mk, mv, a);
     } else {
         const cuuint64_t dims[3] = {(cuuint64_t)g.head_dim, (cuuint64_t)g.num_heads, (cuuint64_t)t.b.tokens};
         const cuuint64_t strides[2] = {(cuuint64_t)g.head_dim * 2, (cuuint64_t)t.q_stride * 2};
@@ -299,28 +319,21 @@ int launch_chunk(hkv_paged_ctx* c, const PagedAttnArgs& t, const void* q, int sm
             dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
         if (r != CUDA_SUCCESS) return fail(c, HKV_ERR_CUDA, "cuTensorMapEncodeTiled failed (queries)");
-        pick_chunk(g.dtype, g.head_dim)<<<c->sm_count, kCkThreads, smem, st>>>(mq, mk, mv, a);
+        le = cudaLaunchKernelEx(&l.cfg, pick_chunk(g.dtype, g.head_dim), mq, mk, mv, a);
     }
+    if (le != cudaSuccess) return fail_cuda(c, le, "attention launch");
     f.chunk_part = c->chunk_part;
     f.chunk_cuts = c->chunk_cuts;
     f.ctas = c->sm_count;
     f.tiles = wide(g) ? 1 : 2;
     f.QT = a.QT;
-    return launched(c, "attention launch");
+    return HKV_OK;
 }
 
 int launch_finish(hkv_paged_ctx* c, const PagedFinishArgs& f, cudaStream_t st) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)finish_blocks(f, c->g.num_kv_heads));
-    cfg.blockDim = dim3(256);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = c->g.dtype == HKV_DTYPE_F16 ? cudaLaunchKernelEx(&cfg, hkv_paged_finish_kernel<__half>, f)
-                                                       : cudaLaunchKernelEx(&cfg, hkv_paged_finish_kernel<__nv_bfloat16>, f);
+    const Launch l((unsigned)finish_blocks(f, c->g.num_kv_heads), 256, 0, st, true);
+    const cudaError_t e = c->g.dtype == HKV_DTYPE_F16 ? cudaLaunchKernelEx(&l.cfg, hkv_paged_finish_kernel<__half>, f)
+                                                       : cudaLaunchKernelEx(&l.cfg, hkv_paged_finish_kernel<__nv_bfloat16>, f);
     return e == cudaSuccess ? HKV_OK : fail_cuda(c, e, "attention finish launch");
 }
 

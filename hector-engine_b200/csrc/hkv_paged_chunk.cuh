@@ -37,7 +37,7 @@ constexpr int kCkDesc = 16;               // words of a work descriptor
 struct PagedChunkArgs {
     PagedAttnArgs t;
     PagedLine line;           // `pre` is filled in by the kernel
-    float* part;              // [2 * grid][rows per item][HD + 4]: o, maximum (log2 domain), sum
+    float* part;              // [2 * grid] sets of partial rows, see store_partial
     int4* cuts;               // [grid]: the item that starts in a CTA's span and goes on behind it: {request, kv head, block, parts}
     PagedFix fix;
     int QT;                   // queries per 128-row tile
@@ -132,6 +132,53 @@ __device__ __forceinline__ void chunk_walk(const PagedBatch& b, const PagedLine&
     }
 }
 
+// ---- rows out of tensor memory ----------------------------------------------------------------------------------------
+// A thread holds a row, but 32 stores of 16 bytes at 32 rows are 32 half-used sectors: a warp's 4 KB then takes a quarter
+// of a microsecond of the store path, 3.2 us an item. So the four lanes of a quad swap 16-byte pieces (a 4 x 4 transpose)
+// and each store writes 64 contiguous bytes of 8 rows.
+__device__ __forceinline__ void quad_transpose(uint32_t (&w)[16]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int bit = 1; bit <= 2; bit <<= 1) {
+        const bool up = lane & bit;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            if (b & bit) continue;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                uint32_t &x = w[4 * b + e], &y = w[4 * (b | bit) + e];
+                const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? x : y, bit);
+                if (up) x = got; else y = got;
+            }
+        }
+    }
+}
+// Element offsets of the four rows of this lane's quad; -1: a row that is not written.
+__device__ __forceinline__ void quad_rows(const long long mine, long long (&rows)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) rows[i] = __shfl_sync(0xffffffffu, mine, (threadIdx.x & 28) + i);
+}
+// 32 columns of a row per thread, scaled and rounded, to the quad's rows. Whole warps.
+template <typename T>
+__device__ __forceinline__ void store_rows32(T* out, const long long (&rows)[4], const int col, const uint32_t (&v)[32], const float inv) {
+    uint32_t w[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) w[j] = pack2<T>(__uint_as_float(v[2 * j]) * inv, __uint_as_float(v[2 * j + 1]) * inv);
+    quad_transpose(w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (rows[i] >= 0)
+            *reinterpret_cast<uint4*>(out + rows[i] + col + (threadIdx.x & 3) * 8) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+}
+// A set of partial rows: [head_dim / 4][rows] float4 of o, then [rows] {maximum (log2 domain), sum}: a warp writes its rows
+// side by side, and the finishing kernel reads them so.
+__host__ __device__ constexpr long long partial_floats(int rows, int hd) { return (long long)rows * (hd + 2); }
+__device__ __forceinline__ void store_partial32(float* set, const int rows, const int row, const int col, const uint32_t (&v)[32]) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 4)
+        *reinterpret_cast<uint4*>(set + ((long long)((col + j) / 4) * rows + row) * 4) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+}
+
 // V rows [kstart, kstart + keys) of a staged tile that not every query of a block sees: rows that none attends are zeroed,
 // values that are not finite are dropped from the others (0 * NaN would reach the queries they are hidden from). `threads`
 // threads take part; true if this one dropped a value.
@@ -145,17 +192,28 @@ static __device__ __noinline__ bool clean_values(const PagedBatch& b, const Page
     int tail = hi_first - kstart < 0 ? 0 : (hi_first - kstart < keys ? hi_first - kstart : keys);
     if (tail < head) tail = head;
     bool bad = false;
-    for (int idx = tid; idx < (head + keys - tail) * 8 * NCH; idx += threads) {
-        const int k = idx / (8 * NCH), u = idx % (8 * NCH);
-        const int vr = k < head ? k : tail + k - head, pos = kstart + vr;
-        uint4* at = reinterpret_cast<uint4*>(tile + (u / 8) * chunk_bytes + vr * 128 + (u % 8) * 16);
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (pos >= lo_first && pos < hi_last) {
-            x = *at;
-            if (!drop_nonfinite<T>(x)) continue;
-            bad = true;
+    // a thread keeps its 16-byte column and steps over rows, four loads in flight
+    constexpr int kStep = threads / (8 * NCH);
+    const int u = tid % (8 * NCH), rows = head + keys - tail;
+    uint8_t* col = tile + (u / 8) * chunk_bytes + (u % 8) * 16;
+    for (int k0 = tid / (8 * NCH); k0 < rows; k0 += 4 * kStep) {
+        uint4 x[4];
+        uint4* at[4];
+        bool seen[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int k = k0 + e * kStep, vr = k < head ? k : tail + k - head, pos = kstart + vr;
+            at[e] = k < rows ? reinterpret_cast<uint4*>(col + vr * 128) : nullptr;
+            seen[e] = pos >= lo_first && pos < hi_last;
+            x[e] = make_uint4(0, 0, 0, 0);
+            if (at[e] && seen[e]) x[e] = *at[e];
         }
-        *at = x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const bool drop = at[e] && seen[e] && drop_nonfinite<T>(x[e]);
+            bad |= drop;
+            if (at[e] && (drop || !seen[e])) *at[e] = x[e];
+        }
     }
     return bad;
 }
@@ -512,34 +570,23 @@ hkv_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             const bool row_valid = ql < a.QT && qi < q.n;
             if (m_ref == kLow) l_run = 0.0f;       // every score was masked: what the polynomial makes of -infinity is no weight
             const float inv = l_run == 0.0f ? 0.0f : (l_run < kSumLimit ? 1.0f / l_run : NAN);
-            float* prow = slot >= 0 ? a.part + ((long long)slot * (2 * kCkRows) + grp * kCkRows + row) * (D + 4) : nullptr;
-            T* op = (T*)a.t.out + ((long long)(q.start + qi) * H + (long long)kvh * G + g) * D;
+            float* set = slot >= 0 ? a.part + slot * partial_floats(2 * kCkRows, D) : nullptr;
+            long long rows[4];
+            quad_rows(row_valid ? ((long long)(q.start + qi) * H + (long long)kvh * G + g) * D : -1, rows);
 #pragma unroll 1
             for (int c = 0; c < HD / 32; ++c) {            // (a loop: straight-line code is fetched once per item here)
                 uint32_t v[32];
                 tmem_ld32(v, o_addr + c * 32);
                 tc_wait_ld_dep(v);
-                if (c * 32 >= D || !row_valid) continue;   // columns of zeros (head_dim 96); rows without a query
-                if (prow) {
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4)
-                        *reinterpret_cast<uint4*>(prow + c * 32 + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; j += 8) {
-                        uint4 w;
-                        w.x = pack2<T>(__uint_as_float(v[j]) * inv, __uint_as_float(v[j + 1]) * inv);
-                        w.y = pack2<T>(__uint_as_float(v[j + 2]) * inv, __uint_as_float(v[j + 3]) * inv);
-                        w.z = pack2<T>(__uint_as_float(v[j + 4]) * inv, __uint_as_float(v[j + 5]) * inv);
-                        w.w = pack2<T>(__uint_as_float(v[j + 6]) * inv, __uint_as_float(v[j + 7]) * inv);
-                        *reinterpret_cast<uint4*>(op + c * 32 + j) = w;
-                    }
-                }
+                if (c * 32 >= D) continue;                 // columns of zeros (head_dim 96)
+                if (set) store_partial32(set, 2 * kCkRows, grp * kCkRows + row, c * 32, v);
+                else store_rows32<T>((T*)a.t.out, rows, c * 32, v, inv);
             }
-            if (prow && row_valid) *reinterpret_cast<float2*>(prow + D) = make_float2(m_ref, l_run);
+            if (set) *reinterpret_cast<float2*>(set + (2 * kCkRows) * D + 2 * (grp * kCkRows + row)) = make_float2(m_ref, l_run);
             tc_fence_before();
         }
     }
+    if (tid == 0) wait_for_previous();         // the few-token kernel of the call, where it ran ahead: this launch ends behind it
     tc_fence_before();
     __syncthreads();
     if (warp == 9) tmem_dealloc(tmem, TMEM_COLS);

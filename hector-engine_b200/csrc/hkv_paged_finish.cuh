@@ -2,12 +2,11 @@
 //     o = sum 2^(m_c - M) o_c / sum 2^(m_c - M) l_c,   M = max m_c,
 // and does again what they left on the list of items with hidden values that are not finite. Blocks of 256 threads:
 // first those of the few-token kernel (a block per span, KV head and query row: few rows, up to hundreds of parts, so
-// eight warps deal the parts of a row among them), then those of the prompt kernel (eight per CTA of that launch: many
-// rows of mostly two parts, a warp each). It is launched while the kernel before it still runs and waits for its end on
+// eight warps deal the parts of a row among them), then those of the prompt kernel (many rows of mostly two parts). It is launched while the kernel before it still runs and waits for its end on
 // the GPU. Bound: launch latency; the partial rows (39 MB at most) come out of the L2.
 #pragma once
 
-#include "hkv_paged.cuh"
+#include "hkv_paged_chunk.cuh"
 
 namespace hkv {
 
@@ -16,14 +15,14 @@ struct PagedFinishArgs {
     PagedFix fix;
     const float* small_part;      // [2 * spans][KVH][cols][HD + 2]
     const int4* small_cuts;       // [spans]
-    const float* chunk_part;      // [2 * ctas][tiles * 128][HD + 4]
+    const float* chunk_part;      // [2 * ctas] sets of tiles * 128 rows
     const int4* chunk_cuts;       // [ctas]
     int spans, cols;              // spans 0: no few-token launch
     int ctas, tiles, QT, QB;      // ctas 0: no prompt launch
     int may_fix;                  // 0: a single query per request, nothing can be on the list
 };
-constexpr int kFinishPerCta = 8;  // blocks per CTA of the prompt launch
-__host__ __device__ inline int finish_blocks(const PagedFinishArgs& a, int KVH) { return a.spans * KVH * a.cols + a.ctas * kFinishPerCta; }
+// (blocks of 32 rows behind those of the few-token kernel)
+__host__ __device__ inline int finish_blocks(const PagedFinishArgs& a, int KVH) { return a.spans * KVH * a.cols + a.ctas * a.tiles * 4; }
 
 template <typename T>
 __device__ __forceinline__ void finish_small(const PagedFinishArgs& a, const int block, const int fix_count) {
@@ -91,64 +90,58 @@ __device__ __forceinline__ void finish_small(const PagedFinishArgs& a, const int
     }
 }
 
+// 32 rows per block: a warp takes 8 rows and every eighth group of 4 x 4 columns, so that it reads whole lines of a set and
+// writes whole sectors of a row; the loads of two parts are in flight together, nothing in front of them but the entry.
 template <typename T>
 __device__ __forceinline__ void finish_chunk(const PagedFinishArgs& a, const int block, const int fix_count) {
-    const int cta = block / kFinishPerCta, share = block % kFinishPerCta;
+    const int rows = a.tiles * 128, shares = rows / 32;
+    const int cta = block / shares, share = block % shares;
     const int4 cut = a.chunk_cuts[cta];
     const int parts = cut.w;
     if (parts <= 1) return;
     if (fix_count && paged_to_fix(a.fix, fix_count, cut.x, cut.z, cut.y)) return;
+    const int G = a.t.H / a.t.KVH, HD = a.t.HD, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int row = share * 32 + (warp & 3) * 8 + (lane & 7), cb = (warp >> 2) * 4 + (lane >> 3);
+    const int ql = row % 128 / G, i = cut.z * a.QB + row / 128 * a.QT + ql;
     const PagedRequest q = paged_request(a.t.b, cut.x);
-    const int G = a.t.H / a.t.KVH, HD = a.t.HD, PW = HD + 4, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long long set = (long long)a.tiles * 128 * PW;
+    if (ql >= a.QT || i >= q.n) return;
+    const long long set = partial_floats(rows, HD);
     // part 0 sits in this CTA's second slot, the others in the first slots of the CTAs behind it
-    const float* first = a.chunk_part + (2ll * cta + 1) * set;
-    const float* rest = a.chunk_part + 2ll * (cta + 1) * set;
-    for (int row = share * 8 + warp; row < a.tiles * 128; row += kFinishPerCta * 8) {
-        const int ql = row % 128 / G, i = cut.z * a.QB + row / 128 * a.QT + ql;
-        if (ql >= a.QT || i >= q.n) continue;
-        auto at = [&](int p) { return (p == 0 ? first : rest + 2ll * (p - 1) * set) + (long long)row * PW; };
-        // maxima and sums of up to 32 parts at a time, one per lane; then the rows, four floats per lane
-        float M = kLow, L = 0.0f;
-        float4 acc[2] = {make_float4(0.0f, 0.0f, 0.0f, 0.0f), make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
-        for (int p0 = 0; p0 < parts; p0 += 32) {
-            const int n = parts - p0 < 32 ? parts - p0 : 32;
-            const float2 ml = lane < n ? *reinterpret_cast<const float2*>(at(p0 + lane) + HD) : make_float2(kLow, 0.0f);
-            float Mn = ml.x;
+    const float* base = a.chunk_part + 2ll * cta * set;
+    float M = kLow, L = 0.0f;
+    float4 acc[8];
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) Mn = fmaxf(Mn, __shfl_xor_sync(0xffffffffu, Mn, o));
-            Mn = fmaxf(Mn, M);
-            const float keep = exp2f(M - Mn), w = lane < n ? exp2f(ml.x - Mn) : 0.0f;
-            float l = ml.y * w;
+    for (int e = 0; e < 8; ++e) acc[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int p0 = 0; p0 < parts; p0 += 2) {
+        float2 ml[2];
+        float4 x[2][8];
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-            L = fmaf(L, keep, l);
+        for (int u = 0; u < 2; ++u) {
+            const int p = p0 + u;
+            const float* s = base + (2ll * p + (p == 0 ? 1 : 0)) * set;
+            ml[u] = p < parts ? *reinterpret_cast<const float2*>(s + (long long)rows * HD + 2 * row) : make_float2(kLow, 0.0f);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) { acc[e].x *= keep; acc[e].y *= keep; acc[e].z *= keep; acc[e].w *= keep; }
-#pragma unroll 4
-            for (int p = 0; p < n; ++p) {
-                const float wp = __shfl_sync(0xffffffffu, w, p);
-                const float* r = at(p0 + p);
+            for (int e = 0; e < 8; ++e)
+                x[u][e] = p < parts && 32 * e < HD ? *reinterpret_cast<const float4*>(s + ((long long)(cb + 8 * e) * rows + row) * 4)
+                                                   : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int d = 4 * lane + 128 * e;
-                    if (d < HD) {
-                        const float4 x = *reinterpret_cast<const float4*>(r + d);
-                        acc[e].x = fmaf(x.x, wp, acc[e].x); acc[e].y = fmaf(x.y, wp, acc[e].y);
-                        acc[e].z = fmaf(x.z, wp, acc[e].z); acc[e].w = fmaf(x.w, wp, acc[e].w);
-                    }
-                }
+        for (int u = 0; u < 2; ++u) {
+            const float Mn = fmaxf(M, ml[u].x), keep = exp2f(M - Mn), w = exp2f(ml[u].x - Mn);
+            L = fmaf(ml[u].y, w, L * keep);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                acc[e].x = fmaf(x[u][e].x, w, acc[e].x * keep); acc[e].y = fmaf(x[u][e].y, w, acc[e].y * keep);
+                acc[e].z = fmaf(x[u][e].z, w, acc[e].z * keep); acc[e].w = fmaf(x[u][e].w, w, acc[e].w * keep);
             }
             M = Mn;
         }
-        const float inv = L == 0.0f ? 0.0f : (L < kSumLimit ? 1.0f / L : NAN);
-        T* op = (T*)a.t.out + ((long long)(q.start + i) * a.t.H + (long long)cut.y * G + row % 128 % G) * HD;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int d = 4 * lane + 128 * e;
-            if (d < HD) *reinterpret_cast<uint2*>(op + d) = make_uint2(pack2<T>(acc[e].x * inv, acc[e].y * inv), pack2<T>(acc[e].z * inv, acc[e].w * inv));
-        }
     }
+    const float inv = L == 0.0f ? 0.0f : (L < kSumLimit ? 1.0f / L : NAN);
+    T* op = (T*)a.t.out + ((long long)(q.start + i) * a.t.H + (long long)cut.y * G + row % 128 % G) * HD + 4 * cb;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (32 * e < HD) *reinterpret_cast<uint2*>(op + 32 * e) = make_uint2(pack2<T>(acc[e].x * inv, acc[e].y * inv), pack2<T>(acc[e].z * inv, acc[e].w * inv));
 }
 
 template <typename T>

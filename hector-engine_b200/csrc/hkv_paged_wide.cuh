@@ -334,35 +334,23 @@ hkv_paged_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
             if (!ok) continue;
             tc_fence_after();
             const float inv = l_tot == 0.0f ? 0.0f : (l_tot < kSumLimit ? 1.0f / l_tot : NAN);
-            float* prow = slot >= 0 ? a.part + ((long long)slot * kCkRows + row) * (HD + 4) : nullptr;
-            T* op = (T*)a.t.out + ((long long)(q.start + qi) * H + (long long)kvh * G + g) * HD;
-#pragma unroll
+            float* set = slot >= 0 ? a.part + slot * partial_floats(kCkRows, HD) : nullptr;
+            long long rows[4];
+            quad_rows(row_valid ? ((long long)(q.start + qi) * H + (long long)kvh * G + g) * HD : -1, rows);
+#pragma unroll 1
             for (int c = 0; c < HH / 32; ++c) {
                 const int d0 = half * HH + c * 32;
                 uint32_t v[32];
                 tmem_ld32(v, tmem + lane_sel + COL_O + d0);
                 tc_wait_ld_dep(v);
-                if (!row_valid) continue;
-                if (prow) {
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4)
-                        *reinterpret_cast<uint4*>(prow + d0 + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; j += 8) {
-                        uint4 w;
-                        w.x = pack2<T>(__uint_as_float(v[j]) * inv, __uint_as_float(v[j + 1]) * inv);
-                        w.y = pack2<T>(__uint_as_float(v[j + 2]) * inv, __uint_as_float(v[j + 3]) * inv);
-                        w.z = pack2<T>(__uint_as_float(v[j + 4]) * inv, __uint_as_float(v[j + 5]) * inv);
-                        w.w = pack2<T>(__uint_as_float(v[j + 6]) * inv, __uint_as_float(v[j + 7]) * inv);
-                        *reinterpret_cast<uint4*>(op + d0 + j) = w;
-                    }
-                }
+                if (set) store_partial32(set, kCkRows, row, d0, v);
+                else store_rows32<T>((T*)a.t.out, rows, d0, v, inv);
             }
-            if (prow && row_valid && half == 0) *reinterpret_cast<float2*>(prow + HD) = make_float2(m_ref, l_tot);
+            if (set && half == 0) *reinterpret_cast<float2*>(set + kCkRows * HD + 2 * row) = make_float2(m_ref, l_tot);
             tc_fence_before();
         }
     }
+    if (tid == 0) wait_for_previous();         // the few-token kernel of the call, where it ran ahead: this launch ends behind it
     tc_fence_before();
     __syncthreads();
     if (warp == 9) tmem_dealloc(tmem, TMEM_COLS);
