@@ -146,6 +146,29 @@ int encode_plane(hkv_paged_ctx* c, const void* base, int width, int rows, CUtens
     return fail(c, HKV_ERR_CUDA, buf);
 }
 
+// Map of a plane for the prompt kernels: rows in groups of 8, [group of the pool][column block of 64][row][64 elements], so
+// that one box holds `rows` rows of one KV head and lands as whole swizzle groups; its blocks are the unit of the third
+// coordinate. head_dim 96, whose rows are not a whole number of blocks: the third coordinate counts heads and a box is one
+// block, the second of them half outside (zeros).
+int encode_tiles(hkv_paged_ctx* c, const void* base, int rows, CUtensorMap* out) {
+    const hkv_paged_geometry& g = c->g;
+    const bool whole = g.head_dim % 64 == 0;
+    const int blocks = whole ? g.head_dim / 64 : 1;
+    const cuuint64_t row = (cuuint64_t)g.num_kv_heads * g.head_dim * 2;
+    const cuuint64_t dims[4] = {whole ? 64u : (cuuint64_t)g.head_dim, 8u, (cuuint64_t)g.num_kv_heads * blocks,
+                                (cuuint64_t)g.num_pages * g.page_size / 8};
+    const cuuint64_t strides[3] = {row, whole ? 128u : (cuuint64_t)g.head_dim * 2, row * 8};
+    const cuuint32_t box[4] = {64u, 8u, (cuuint32_t)blocks, (cuuint32_t)rows / 8}, one[4] = {1u, 1u, 1u, 1u};
+    const CUresult r = encode_tiled_fn()(
+        out, g.dtype == HKV_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+        const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r == CUDA_SUCCESS) return HKV_OK;
+    char buf[96];
+    snprintf(buf, sizeof buf, "cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
+    return fail(c, HKV_ERR_CUDA, buf);
+}
+
 // A launch configuration; `early`: it may be set up (and run, up to its own wait) while the launch before it still runs.
 struct Launch {
     cudaLaunchConfig_t cfg{};
@@ -263,9 +286,12 @@ size_t chunk_smem(const hkv_paged_geometry& g, int requests) {
 }
 
 typedef void (*ChunkKernel)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const PagedChunkArgs);
+template <typename T>
+ChunkKernel pick_chunk_t(int hd) {
+    return hd == 64 ? hkv_paged_chunk_kernel<T, 64, true> : hd == 128 ? hkv_paged_chunk_kernel<T, 128, true> : hkv_paged_chunk_kernel<T, 128, false>;
+}
 ChunkKernel pick_chunk(int dtype, int hd) {
-    if (dtype == HKV_DTYPE_F16) return staged_hd(hd) == 64 ? hkv_paged_chunk_kernel<__half, 64> : hkv_paged_chunk_kernel<__half, 128>;
-    return staged_hd(hd) == 64 ? hkv_paged_chunk_kernel<__nv_bfloat16, 64> : hkv_paged_chunk_kernel<__nv_bfloat16, 128>;
+    return dtype == HKV_DTYPE_F16 ? pick_chunk_t<__half>(hd) : pick_chunk_t<__nv_bfloat16>(hd);
 }
 const void* chunk_kernel(const hkv_paged_geometry& g) {
     if (wide(g)) return g.dtype == HKV_DTYPE_F16 ? (const void*)hkv_paged_wide_kernel<__half> : (const void*)hkv_paged_wide_kernel<__nv_bfloat16>;
@@ -300,8 +326,8 @@ int launch_chunk(hkv_paged_ctx* c, const PagedAttnArgs& t, const void* q, int sm
     a.pieces = a.line.keys / a.box_rows;
     a.small = small;
     CUtensorMap mq, mk, mv;
-    int e = encode_plane(c, t.k_cache, 64, a.box_rows, &mk);
-    if (!e) e = encode_plane(c, t.v_cache, 64, a.box_rows, &mv);
+    int e = encode_tiles(c, t.k_cache, a.box_rows, &mk);
+    if (!e) e = encode_tiles(c, t.v_cache, a.box_rows, &mv);
     if (e) return e;
     const size_t smem = chunk_smem(g, t.b.requests);
     // behind a few-token launch this one starts where that one's CTAs leave room (neither reads what the other writes)

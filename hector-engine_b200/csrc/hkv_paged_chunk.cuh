@@ -41,7 +41,7 @@ struct PagedChunkArgs {
     int4* cuts;               // [grid]: the item that starts in a CTA's span and goes on behind it: {request, kv head, block, parts}
     PagedFix fix;
     int QT;                   // queries per 128-row tile
-    int box_rows, pieces;     // rows of a box; boxes per tile and column block
+    int box_rows, pieces;     // rows of a box; pages per tile
     int small;                // query rows per KV head up to which the few-token kernel takes a request; 0: none
 };
 __host__ __device__ constexpr size_t chunk_smem_bytes(int HD /*staged*/, int requests) {
@@ -184,7 +184,7 @@ __device__ __forceinline__ void store_partial32(float* set, const int rows, cons
 // threads take part; true if this one dropped a value.
 template <typename T, int NCH, int threads>
 static __device__ __noinline__ bool clean_values(const PagedBatch& b, const PagedRequest q, const int i0, const int QB, const int kstart,
-                                          const int keys, uint8_t* tile, const int chunk_bytes, const int tid) {
+                                                 const int keys, uint8_t* tile, const int chunk_off, const int group_off, const int tid) {
     int lo_first, hi_first, lo_last, hi_last;
     paged_key_range(b, q, i0, lo_first, hi_first);
     paged_key_range(b, q, (i0 + QB < q.n ? i0 + QB : q.n) - 1, lo_last, hi_last);
@@ -195,7 +195,7 @@ static __device__ __noinline__ bool clean_values(const PagedBatch& b, const Page
     // a thread keeps its 16-byte column and steps over rows, four loads in flight
     constexpr int kStep = threads / (8 * NCH);
     const int u = tid % (8 * NCH), rows = head + keys - tail;
-    uint8_t* col = tile + (u / 8) * chunk_bytes + (u % 8) * 16;
+    uint8_t* col = tile + (u / 8) * chunk_off + (u % 8) * 16;
     for (int k0 = tid / (8 * NCH); k0 < rows; k0 += 4 * kStep) {
         uint4 x[4];
         uint4* at[4];
@@ -203,7 +203,7 @@ static __device__ __noinline__ bool clean_values(const PagedBatch& b, const Page
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int k = k0 + e * kStep, vr = k < head ? k : tail + k - head, pos = kstart + vr;
-            at[e] = k < rows ? reinterpret_cast<uint4*>(col + vr * 128) : nullptr;
+            at[e] = k < rows ? reinterpret_cast<uint4*>(col + (vr >> 3) * group_off + (vr & 7) * 128) : nullptr;
             seen[e] = pos >= lo_first && pos < hi_last;
             x[e] = make_uint4(0, 0, 0, 0);
             if (at[e] && seen[e]) x[e] = *at[e];
@@ -218,7 +218,9 @@ static __device__ __noinline__ bool clean_values(const PagedBatch& b, const Page
     return bad;
 }
 
-template <typename T, int HD>
+// WHOLE: one box brings all column blocks of its rows, a staged K or V tile is [8-row group][column block][8 rows of 128
+// bytes]. Otherwise (head_dim 96) a box per block, [column block][8-row group], so that the columns behind it are zeros.
+template <typename T, int HD, bool WHOLE>
 __global__ void __launch_bounds__(kCkThreads, 1)
 hkv_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, const PagedChunkArgs a) {
@@ -226,6 +228,8 @@ hkv_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     constexpr int NCH = HD / 64;                       // 64-element column blocks
     constexpr int CHUNK_BYTES = kCkRows * 128;
     constexpr int TILE_BYTES = kCkRows * HD * 2;
+    constexpr int CHUNK_OFF = WHOLE ? 1024 : CHUNK_BYTES, GROUP_OFF = WHOLE ? NCH * 1024 : 1024;
+    constexpr int COL_BOXES = WHOLE ? 1 : NCH, HEAD_STEP = WHOLE ? NCH : 1;   // boxes per piece; coordinate step of a KV head
     constexpr uint32_t TMEM_COLS = 512;
     constexpr uint32_t COL_S = 0, COL_O = 256;         // + 128 * group
     constexpr uint32_t FMT = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);   // operand type of the MMA
@@ -335,11 +339,10 @@ hkv_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
                     if (lane == 0) mbar_expect_tx(full, TILE_BYTES);
                     __syncwarp();
                     const uint32_t dst = (kv ? v_smem : k_smem) + s * TILE_BYTES;
-                    for (int b0 = 0; b0 < NCH * a.pieces; b0 += 32) {
-                        const int bx = b0 + lane, piece = bx % a.pieces, c = bx / a.pieces;
-                        if (bx < NCH * a.pieces)
-                            tma_load_4d(dst + c * CHUNK_BYTES + piece * a.box_rows * 128, kv ? &tm_v : &tm_k, full, c * 64, kvh,
-                                        (pos0 + piece * a.box_rows) & (bt.page - 1), pg);
+                    if (lane < COL_BOXES * a.pieces) {             // (at most 32)
+                        const int c = COL_BOXES > 1 ? lane / a.pieces : 0, at = my_piece * a.box_rows;
+                        tma_load_4d(dst + c * CHUNK_OFF + (at >> 3) * GROUP_OFF, kv ? &tm_v : &tm_k, full, c * 64, 0, kvh * HEAD_STEP,
+                                    (pg << (page_shift - 3)) + (((pos0 + at) & (bt.page - 1)) >> 3));
                     }
                 }
                 pg = pg_next;
@@ -367,9 +370,9 @@ hkv_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         if (elect_one()) {
             uint32_t gt = 0, it = 0, gb = 0;               // tiles; items; tiles of tile B
             bool ok = true;
-            const uint64_t qdesc0 = umma_desc_sw128(q_smem, 16), kdesc0 = umma_desc_sw128(k_smem, 16);
-            const uint64_t vdesc0 = umma_desc_sw128(v_smem, CHUNK_BYTES);
-            const uint32_t desc_hi = (uint32_t)(qdesc0 >> 32);
+            const uint64_t qdesc0 = umma_desc_sw128(q_smem, 16), kdesc0 = umma_desc_sw128(k_smem, 16, GROUP_OFF);
+            const uint64_t vdesc0 = umma_desc_sw128(v_smem, CHUNK_OFF, GROUP_OFF);
+            const uint32_t q_hi = (uint32_t)(qdesc0 >> 32), kv_hi = (uint32_t)(kdesc0 >> 32);
             const uint32_t q_lo = (uint32_t)qdesc0, k_lo = (uint32_t)kdesc0, v_lo = (uint32_t)vdesc0;
             const int ksteps = (D + 15) / 16;              // zero-filled k-steps are skipped
             auto issue_qk = [&](uint32_t g, int grp) {     // S_grp = Q_grp K(g)^T
@@ -378,9 +381,9 @@ hkv_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
                 const uint32_t d = tmem + COL_S + 128u * grp;
 #pragma unroll
                 for (int kk = 0; kk < HD / 16; ++kk) {
-                    const uint32_t off = (uint32_t)(((kk / 4) * CHUNK_BYTES + (kk % 4) * 32) >> 4);
-                    if (kk == 0) tc_mma_ss_i<false>(d, qd + off, kd + off, desc_hi, IDESC_QK);
-                    else if (kk < ksteps) tc_mma_ss_i<true>(d, qd + off, kd + off, desc_hi, IDESC_QK);
+                    const uint32_t qo = (uint32_t)(((kk / 4) * CHUNK_BYTES + (kk % 4) * 32) >> 4), ko = (uint32_t)(((kk / 4) * CHUNK_OFF + (kk % 4) * 32) >> 4);
+                    if (kk == 0) tc_mma_ss_ii<false>(d, qd + qo, q_hi, kd + ko, kv_hi, IDESC_QK);
+                    else if (kk < ksteps) tc_mma_ss_ii<true>(d, qd + qo, q_hi, kd + ko, kv_hi, IDESC_QK);
                 }
                 tc_commit(B_SFULL + 8 * grp);
             };
@@ -391,9 +394,9 @@ hkv_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 #pragma unroll
                 for (int k = 0; k < kCkKeys / 32; ++k) {
                     const int kk = half * (kCkKeys / 32) + k;
-                    const uint32_t at = vd + (uint32_t)((kk * 2048) >> 4);
-                    if (k > 0 || accumulate) tc_mma_ts_i<true>(d, pbase + kk * 8, at, desc_hi, IDESC_PV);
-                    else tc_mma_ts_i<false>(d, pbase + kk * 8, at, desc_hi, IDESC_PV);
+                    const uint32_t at = vd + (uint32_t)((kk * 2 * GROUP_OFF) >> 4);
+                    if (k > 0 || accumulate) tc_mma_ts_i<true>(d, pbase + kk * 8, at, kv_hi, IDESC_PV);
+                    else tc_mma_ts_i<false>(d, pbase + kk * 8, at, kv_hi, IDESC_PV);
                 }
             };
             for (; ok; ++it) {
@@ -527,7 +530,7 @@ hkv_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
                     ok = __all_sync(0xffffffffu, mbar_wait(B_VFULL + 8 * vs, (gt / kCkStages) & 1, bt.status));
                     if (!ok) continue;
                     const bool bad = clean_values<T, NCH, 128>(bt, q, i0, a.line.QB, (kt + t) * kCkKeys, kCkKeys,
-                                                               v_gen + (size_t)vs * TILE_BYTES, CHUNK_BYTES, tid);
+                                                               v_gen + (size_t)vs * TILE_BYTES, CHUNK_OFF, GROUP_OFF, tid);
                     if (__any_sync(0xffffffffu, bad) && lane == 0) a.fix.push(r, p, kvh);
                     fence_proxy_async_smem();
                 }

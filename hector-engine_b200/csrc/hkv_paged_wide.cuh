@@ -27,7 +27,8 @@ template <typename T>
 __global__ void __launch_bounds__(kWdThreads, 1)
 hkv_paged_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const PagedChunkArgs a) {
     constexpr int HD = kWdHD, NCH = HD / 64;
-    constexpr int CHUNK_BYTES = kWdKeys * 128, TILE_BYTES = kWdKeys * HD * 2;
+    constexpr int TILE_BYTES = kWdKeys * HD * 2;
+    constexpr int CHUNK_OFF = 1024, GROUP_OFF = NCH * 1024;   // staged tiles: [8-row group][column block][8 rows of 128 bytes]
     constexpr uint32_t TMEM_COLS = 512, COL_O = 0, COL_Q = 256, COL_S = 384;   // S: + 64 * (tile & 1)
     constexpr int KH = kWdKeys / 2, HH = HD / 2;           // score columns, output dimensions per thread
     constexpr uint32_t FMT = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
@@ -125,11 +126,10 @@ hkv_paged_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                     if (lane == 0) mbar_expect_tx(full, TILE_BYTES);
                     __syncwarp();
                     const uint32_t dst = (kv ? v_smem : k_smem) + s * TILE_BYTES;
-                    for (int b0 = 0; b0 < NCH * a.pieces; b0 += 32) {
-                        const int bx = b0 + lane, piece = bx % a.pieces, c = bx / a.pieces;
-                        if (bx < NCH * a.pieces)
-                            tma_load_4d(dst + c * CHUNK_BYTES + piece * a.box_rows * 128, kv ? &tm_v : &tm_k, full, c * 64, kvh,
-                                        (pos0 + piece * a.box_rows) & (bt.page - 1), pg);
+                    if (lane < a.pieces) {             // one box per page, all column blocks
+                        const int at = lane * a.box_rows;
+                        tma_load_4d(dst + (at >> 3) * GROUP_OFF, kv ? &tm_v : &tm_k, full, 0, 0, kvh * NCH,
+                                    (pg << (page_shift - 3)) + (((pos0 + at) & (bt.page - 1)) >> 3));
                     }
                 }
                 pg = pg_next;
@@ -151,7 +151,7 @@ hkv_paged_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
         if (elect_one()) {
             uint32_t gt = 0, it = 0;
             bool ok = true;
-            const uint64_t kdesc0 = umma_desc_sw128(k_smem, 16), vdesc0 = umma_desc_sw128(v_smem, CHUNK_BYTES);
+            const uint64_t kdesc0 = umma_desc_sw128(k_smem, 16, GROUP_OFF), vdesc0 = umma_desc_sw128(v_smem, CHUNK_OFF, GROUP_OFF);
             const uint32_t desc_hi = (uint32_t)(kdesc0 >> 32), k_lo = (uint32_t)kdesc0, v_lo = (uint32_t)vdesc0;
             auto issue_qk = [&](uint32_t g) -> bool {      // S_(g&1) = Q K(g)^T
                 const uint32_t s = g % kWdStages;
@@ -160,7 +160,7 @@ hkv_paged_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                 const uint32_t kd = k_lo + ((s * TILE_BYTES) >> 4), d = tmem + COL_S + 64u * (g & 1), qa = tmem + COL_Q;
 #pragma unroll
                 for (int kk = 0; kk < HD / 16; ++kk) {
-                    const uint32_t off = (uint32_t)(((kk / 4) * CHUNK_BYTES + (kk % 4) * 32) >> 4);
+                    const uint32_t off = (uint32_t)(((kk / 4) * CHUNK_OFF + (kk % 4) * 32) >> 4);
                     if (kk == 0) tc_mma_ts_i<false>(d, qa + kk * 8, kd + off, desc_hi, IDESC_QK);
                     else tc_mma_ts_i<true>(d, qa + kk * 8, kd + off, desc_hi, IDESC_QK);
                 }
@@ -186,7 +186,7 @@ hkv_paged_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                     else tc_mma_ts_i<false>(o, pbase, vd, desc_hi, IDESC_PV);
 #pragma unroll
                     for (int kk = 1; kk < kWdKeys / 16; ++kk)
-                        tc_mma_ts_i<true>(o, pbase + kk * 8, vd + (uint32_t)((kk * 2048) >> 4), desc_hi, IDESC_PV);
+                        tc_mma_ts_i<true>(o, pbase + kk * 8, vd + (uint32_t)((kk * 2 * GROUP_OFF) >> 4), desc_hi, IDESC_PV);
                     tc_commit(B_PV);
                     if (t + 1 == nt) tc_commit(B_OFULL);
                     tc_commit(B_VEMPTY + 8 * s);
@@ -314,7 +314,7 @@ hkv_paged_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                     ok = __all_sync(0xffffffffu, mbar_wait(B_VFULL + 8 * vs, (gt / kWdStages) & 1, bt.status));
                     if (!ok) continue;
                     const bool bad = clean_values<T, NCH, 256>(bt, q, i0, a.line.QB, kstart, kWdKeys, v_gen + (size_t)vs * TILE_BYTES,
-                                                               CHUNK_BYTES, tid);
+                                                               CHUNK_OFF, GROUP_OFF, tid);
                     if (__any_sync(0xffffffffu, bad) && lane == 0) a.fix.push(r, p, kvh);
                     fence_proxy_async_smem();
                 }

@@ -63,14 +63,14 @@ __device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint
         ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// Shared-memory matrix descriptor, 128-byte swizzle, 8-row groups 1024 bytes apart.
+// Shared-memory matrix descriptor, 128-byte swizzle, 8-row groups `group_bytes` apart.
 // K-major operands ignore the leading-dimension offset; MN-major operands use it as the
 // distance between 64-element column blocks.
-__device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t smem_addr, uint32_t lbo_bytes) {
+__device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t smem_addr, uint32_t lbo_bytes, uint32_t group_bytes = 1024u) {
     uint64_t d = 0;
     d |= (uint64_t)((smem_addr >> 4) & 0x3FFF);
     d |= (uint64_t)((lbo_bytes >> 4) & 0x3FFF) << 16;
-    d |= (uint64_t)((1024u >> 4) & 0x3FFF) << 32;
+    d |= (uint64_t)((group_bytes >> 4) & 0x3FFF) << 32;
     d |= (uint64_t)1 << 46;  // descriptor version for sm_100
     d |= (uint64_t)2 << 61;  // SWIZZLE_128B
     return d;
@@ -191,6 +191,16 @@ __device__ __forceinline__ void tc_mma_ss_i(uint32_t d_tmem, uint32_t a_lo, uint
         "mov.b64 da, {%1, %3};\n\tmov.b64 db, {%2, %3};\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t}"
         ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "n"(ACC ? 1 : 0)
+        : "memory");
+}
+// The same with a high word per operand (tiles whose 8-row groups lie apart differently).
+template <bool ACC>
+__device__ __forceinline__ void tc_mma_ss_ii(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "mov.b64 da, {%1, %3};\n\tmov.b64 db, {%2, %4};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(a_hi), "r"(b_hi), "r"(idesc), "n"(ACC ? 1 : 0)
         : "memory");
 }
 template <bool ACC>
