@@ -128,17 +128,18 @@ bool staged_geometry(const hkv_paged_geometry& g) {
     return hd && G <= 128 && g.page_size >= 8 && (g.page_size & (g.page_size - 1)) == 0;
 }
 
-// Map of a plane as [page][row][kv head][head_dim], boxes of `rows` rows of one head, `width` elements wide.
-int encode_plane(hkv_paged_ctx* c, const void* base, int width, int rows, CUtensorMap* out) {
+// Map of a plane as [page][row][kv head][head_dim], boxes of `rows` rows of one head, 32 elements wide: head_dim 96 in the
+// few-token kernel.
+int encode_rows(hkv_paged_ctx* c, const void* base, int rows, CUtensorMap* out) {
     const hkv_paged_geometry& g = c->g;
     const cuuint64_t dims[4] = {(cuuint64_t)g.head_dim, (cuuint64_t)g.num_kv_heads, (cuuint64_t)g.page_size, (cuuint64_t)g.num_pages};
     const cuuint64_t row = (cuuint64_t)g.num_kv_heads * g.head_dim * 2;
     const cuuint64_t strides[3] = {(cuuint64_t)g.head_dim * 2, row, row * g.page_size};
-    const cuuint32_t box[4] = {(cuuint32_t)width, 1u, (cuuint32_t)rows, 1u}, one[4] = {1u, 1u, 1u, 1u};
+    const cuuint32_t box[4] = {32u, 1u, (cuuint32_t)rows, 1u}, one[4] = {1u, 1u, 1u, 1u};
     const CUresult r = encode_tiled_fn()(
         out, g.dtype == HKV_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
         const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-        width == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+        CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r == CUDA_SUCCESS) return HKV_OK;
     char buf[96];
@@ -146,9 +147,9 @@ int encode_plane(hkv_paged_ctx* c, const void* base, int width, int rows, CUtens
     return fail(c, HKV_ERR_CUDA, buf);
 }
 
-// Map of a plane for the prompt kernels: rows in groups of 8, [group of the pool][column block of 64][row][64 elements], so
+// Map of a plane with its rows in groups of 8, [group of the pool][column block of 64][row][64 elements], so
 // that one box holds `rows` rows of one KV head and lands as whole swizzle groups; its blocks are the unit of the third
-// coordinate. head_dim 96, whose rows are not a whole number of blocks: the third coordinate counts heads and a box is one
+// coordinate. head_dim 96 in the prompt kernel, its rows not a whole number of blocks: the third coordinate counts heads and a box is one
 // block, the second of them half outside (zeros).
 int encode_tiles(hkv_paged_ctx* c, const void* base, int rows, CUtensorMap* out) {
     const hkv_paged_geometry& g = c->g;
@@ -264,9 +265,9 @@ int launch_small(hkv_paged_ctx* c, const PagedAttnArgs& t, int cols, PagedFinish
     a.cols = cols;
     a.box_rows = std::min(g.page_size, kTileRows);
     a.pieces = kTileRows / a.box_rows;
-    const int width = paged_chunk_width(g.head_dim);
-    int e = encode_plane(c, t.k_cache, width, a.box_rows, &mk);
-    if (!e) e = encode_plane(c, t.v_cache, width, a.box_rows, &mv);
+    const auto encode = g.head_dim % 64 == 0 ? encode_tiles : encode_rows;
+    int e = encode(c, t.k_cache, a.box_rows, &mk);
+    if (!e) e = encode(c, t.v_cache, a.box_rows, &mv);
     if (e) return e;
     pick_decode(g.dtype, g.head_dim, cols > 8 ? 2 : 1, s.groups)<<<s.grid, (s.groups * 4 + 1) * 32, s.plan.bytes, st>>>(mk, mv, a, s.plan.stages);
     f.small_part = c->part;

@@ -101,6 +101,11 @@ hkv_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     constexpr int ROWB = CW * 2;
     constexpr int CHUNK_BYTES = kTileRows * ROWB;
     constexpr int TILE_BYTES = kTileRows * HD * 2;
+    // A staged tile: whole 128-byte column blocks as [8-row group][column block][8 rows], so that one box brings all of
+    // them; head_dim 96 as [column block of 64 bytes][row].
+    constexpr bool WHOLE = CW == 64;
+    constexpr int CHUNK_OFF = WHOLE ? 1024 : CHUNK_BYTES;
+    auto row_off = [](int row) { return WHOLE ? (row >> 3) * (NCH * 1024) + (row & 7) * 128 : row * ROWB; };
     constexpr int STAGE_BYTES = 2 * TILE_BYTES;
     constexpr int NCW = NGROUPS * 4;
     constexpr int KS = HD / 16;
@@ -199,7 +204,7 @@ hkv_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         // ------------------------------ producer (the whole warp) ------------------------------
         int stage = 0, round = 0, issued = 0;
         bool ok = true;
-        const int boxes = 2 * NCH * a.pieces;
+        const int boxes = 2 * (WHOLE ? 1 : NCH) * a.pieces;
         const int page_shift = 31 - __clz(bt.page);   // page sizes here are powers of two
         const int my_piece = lane % a.pieces;         // (pieces divides 32)
         for (int kvh = member; kvh < KVH && ok; kvh += GS) {
@@ -235,7 +240,16 @@ hkv_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                     if (lane == 0) mbar_expect_tx(full, STAGE_BYTES);
                     __syncwarp();
                     for (int b0 = 0; b0 < boxes; b0 += 32) {
-                        const int x = b0 + lane, piece = x % a.pieces, c = x / a.pieces % NCH, kv = x / (a.pieces * NCH);
+                        const int x = b0 + lane, piece = x % a.pieces;
+                        if constexpr (WHOLE) {
+                            if (x < boxes) {
+                                const int kv = x >= a.pieces, at = piece * a.box_rows;
+                                tma_load_4d(dst + kv * TILE_BYTES + row_off(at), kv ? &tm_v : &tm_k, full, 0, 0, kvh * NCH,
+                                            (pg << (page_shift - 3)) + (((pos0 + at) & (bt.page - 1)) >> 3));
+                            }
+                            continue;
+                        }
+                        const int c = x / a.pieces % NCH, kv = x / (a.pieces * NCH);
                         if (x < boxes)
                             tma_load_4d(dst + kv * TILE_BYTES + c * CHUNK_BYTES + piece * a.box_rows * ROWB, kv ? &tm_v : &tm_k, full,
                                         c * CW, kvh, (pos0 + piece * a.box_rows) & (bt.page - 1), pg);
@@ -264,6 +278,8 @@ hkv_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     const int v_sel = (lane >> 3) & 1;                                 // V^T: matrices 1,3 are d+8
     const int k_swz = (CW == 64) ? (k_row & 7) : ((k_row >> 1) & 3);
     const int v_swz = (CW == 64) ? (v_row & 7) : ((v_row >> 1) & 3);
+
+    const int k_off = row_off(k_row), v_off = row_off(v_row);
 
     int stage = 0, round = 0, tile_seq = 0;
     bool ok = true;
@@ -337,7 +353,7 @@ hkv_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                         const int swz = (CW == 64) ? (tr & 7) : ((tr >> 1) & 3);
                         for (int e = lane; e < HD / 8; e += 32) {
                             const int c = (e * 8) / CW, uu = (e * 8 % CW) / 8;
-                            uint4* at = reinterpret_cast<uint4*>(vgen + c * CHUNK_BYTES + tr * ROWB + ((uu ^ swz) << 4));
+                            uint4* at = reinterpret_cast<uint4*>(vgen + c * CHUNK_OFF + row_off(tr) + ((uu ^ swz) << 4));
                             uint4 x = none ? make_uint4(0, 0, 0, 0) : *at;
                             if (!none) {
                                 if (!drop_nonfinite<T>(x)) continue;
@@ -363,7 +379,7 @@ hkv_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                     const int d0 = ks * 16 + k_sel * 8;
                     const int c = d0 / CW, uu = (d0 % CW) / 8;
                     uint32_t a0, a1, a2, a3;
-                    ldsm_x4(kbase + c * CHUNK_BYTES + k_row * ROWB + ((uu ^ k_swz) << 4), a0, a1, a2, a3);
+                    ldsm_x4(kbase + c * CHUNK_OFF + k_off + ((uu ^ k_swz) << 4), a0, a1, a2, a3);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) mma_16816_t<T>(sc[n][ks & 1], a0, a1, a2, a3, qb[n][ks][0], qb[n][ks][1]);
                 }
@@ -414,7 +430,7 @@ hkv_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                     const int d0 = mt * 16 + v_sel * 8;
                     const int c = d0 / CW, uu = (d0 % CW) / 8;
                     uint32_t a0, a1, a2, a3;
-                    ldsm_x4_t(vbase + c * CHUNK_BYTES + v_row * ROWB + ((uu ^ v_swz) << 4), a0, a1, a2, a3);
+                    ldsm_x4_t(vbase + c * CHUNK_OFF + v_off + ((uu ^ v_swz) << 4), a0, a1, a2, a3);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) mma_16816_t<T>(o_acc[n][mt], a0, a1, a2, a3, pb[n][0], pb[n][1]);
                 }
