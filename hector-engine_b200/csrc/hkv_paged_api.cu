@@ -128,42 +128,22 @@ bool staged_geometry(const hkv_paged_geometry& g) {
     return hd && G <= 128 && g.page_size >= 8 && (g.page_size & (g.page_size - 1)) == 0;
 }
 
-// Map of a plane as [page][row][kv head][head_dim], boxes of `rows` rows of one head, 32 elements wide: head_dim 96 in the
-// few-token kernel.
-int encode_rows(hkv_paged_ctx* c, const void* base, int rows, CUtensorMap* out) {
+// Map of a plane with its rows in groups of 8, [group of the pool][column block][row][width elements], so that one box holds
+// `rows` rows of one KV head and lands as whole swizzle groups; the third coordinate counts column blocks. Where head_dim is
+// not a whole number of blocks (96 in blocks of 64) it counts heads and a box is one block, the last one half outside (zeros).
+int encode_tiles(hkv_paged_ctx* c, const void* base, int width, int rows, CUtensorMap* out) {
     const hkv_paged_geometry& g = c->g;
-    const cuuint64_t dims[4] = {(cuuint64_t)g.head_dim, (cuuint64_t)g.num_kv_heads, (cuuint64_t)g.page_size, (cuuint64_t)g.num_pages};
+    const bool whole = g.head_dim % width == 0;
+    const int blocks = whole ? g.head_dim / width : 1;
     const cuuint64_t row = (cuuint64_t)g.num_kv_heads * g.head_dim * 2;
-    const cuuint64_t strides[3] = {(cuuint64_t)g.head_dim * 2, row, row * g.page_size};
-    const cuuint32_t box[4] = {32u, 1u, (cuuint32_t)rows, 1u}, one[4] = {1u, 1u, 1u, 1u};
+    const cuuint64_t dims[4] = {(cuuint64_t)(whole ? width : g.head_dim), 8u, (cuuint64_t)g.num_kv_heads * blocks,
+                                (cuuint64_t)g.num_pages * g.page_size / 8};
+    const cuuint64_t strides[3] = {row, (cuuint64_t)(whole ? width : g.head_dim) * 2, row * 8};
+    const cuuint32_t box[4] = {(cuuint32_t)width, 8u, (cuuint32_t)blocks, (cuuint32_t)rows / 8}, one[4] = {1u, 1u, 1u, 1u};
     const CUresult r = encode_tiled_fn()(
         out, g.dtype == HKV_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
         const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-        CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r == CUDA_SUCCESS) return HKV_OK;
-    char buf[96];
-    snprintf(buf, sizeof buf, "cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
-    return fail(c, HKV_ERR_CUDA, buf);
-}
-
-// Map of a plane with its rows in groups of 8, [group of the pool][column block of 64][row][64 elements], so
-// that one box holds `rows` rows of one KV head and lands as whole swizzle groups; its blocks are the unit of the third
-// coordinate. head_dim 96 in the prompt kernel, its rows not a whole number of blocks: the third coordinate counts heads and a box is one
-// block, the second of them half outside (zeros).
-int encode_tiles(hkv_paged_ctx* c, const void* base, int rows, CUtensorMap* out) {
-    const hkv_paged_geometry& g = c->g;
-    const bool whole = g.head_dim % 64 == 0;
-    const int blocks = whole ? g.head_dim / 64 : 1;
-    const cuuint64_t row = (cuuint64_t)g.num_kv_heads * g.head_dim * 2;
-    const cuuint64_t dims[4] = {whole ? 64u : (cuuint64_t)g.head_dim, 8u, (cuuint64_t)g.num_kv_heads * blocks,
-                                (cuuint64_t)g.num_pages * g.page_size / 8};
-    const cuuint64_t strides[3] = {row, whole ? 128u : (cuuint64_t)g.head_dim * 2, row * 8};
-    const cuuint32_t box[4] = {64u, 8u, (cuuint32_t)blocks, (cuuint32_t)rows / 8}, one[4] = {1u, 1u, 1u, 1u};
-    const CUresult r = encode_tiled_fn()(
-        out, g.dtype == HKV_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
-        const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        width == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r == CUDA_SUCCESS) return HKV_OK;
     char buf[96];
     snprintf(buf, sizeof buf, "cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
@@ -265,9 +245,8 @@ int launch_small(hkv_paged_ctx* c, const PagedAttnArgs& t, int cols, PagedFinish
     a.cols = cols;
     a.box_rows = std::min(g.page_size, kTileRows);
     a.pieces = kTileRows / a.box_rows;
-    const auto encode = g.head_dim % 64 == 0 ? encode_tiles : encode_rows;
-    int e = encode(c, t.k_cache, a.box_rows, &mk);
-    if (!e) e = encode(c, t.v_cache, a.box_rows, &mv);
+    int e = encode_tiles(c, t.k_cache, paged_chunk_width(g.head_dim), a.box_rows, &mk);
+    if (!e) e = encode_tiles(c, t.v_cache, paged_chunk_width(g.head_dim), a.box_rows, &mv);
     if (e) return e;
     pick_decode(g.dtype, g.head_dim, cols > 8 ? 2 : 1, s.groups)<<<s.grid, (s.groups * 4 + 1) * 32, s.plan.bytes, st>>>(mk, mv, a, s.plan.stages);
     f.small_part = c->part;
@@ -327,8 +306,8 @@ int launch_chunk(hkv_paged_ctx* c, const PagedAttnArgs& t, const void* q, int sm
     a.pieces = a.line.keys / a.box_rows;
     a.small = small;
     CUtensorMap mq, mk, mv;
-    int e = encode_tiles(c, t.k_cache, a.box_rows, &mk);
-    if (!e) e = encode_tiles(c, t.v_cache, a.box_rows, &mv);
+    int e = encode_tiles(c, t.k_cache, 64, a.box_rows, &mk);
+    if (!e) e = encode_tiles(c, t.v_cache, 64, a.box_rows, &mv);
     if (e) return e;
     const size_t smem = chunk_smem(g, t.b.requests);
     // behind a few-token launch this one starts where that one's CTAs leave room (neither reads what the other writes)

@@ -99,13 +99,10 @@ hkv_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
     constexpr int CW = paged_chunk_width(HD);
     constexpr int NCH = HD / CW;
     constexpr int ROWB = CW * 2;
-    constexpr int CHUNK_BYTES = kTileRows * ROWB;
     constexpr int TILE_BYTES = kTileRows * HD * 2;
-    // A staged tile: whole 128-byte column blocks as [8-row group][column block][8 rows], so that one box brings all of
-    // them; head_dim 96 as [column block of 64 bytes][row].
-    constexpr bool WHOLE = CW == 64;
-    constexpr int CHUNK_OFF = WHOLE ? 1024 : CHUNK_BYTES;
-    auto row_off = [](int row) { return WHOLE ? (row >> 3) * (NCH * 1024) + (row & 7) * 128 : row * ROWB; };
+    // A staged tile: [8-row group][column block][8 rows], so that one box brings all column blocks of a page's rows.
+    constexpr int CHUNK_OFF = 8 * ROWB;
+    auto row_off = [](int row) { return (row >> 3) * (NCH * CHUNK_OFF) + (row & 7) * ROWB; };
     constexpr int STAGE_BYTES = 2 * TILE_BYTES;
     constexpr int NCW = NGROUPS * 4;
     constexpr int KS = HD / 16;
@@ -204,7 +201,6 @@ hkv_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         // ------------------------------ producer (the whole warp) ------------------------------
         int stage = 0, round = 0, issued = 0;
         bool ok = true;
-        const int boxes = 2 * (WHOLE ? 1 : NCH) * a.pieces;
         const int page_shift = 31 - __clz(bt.page);   // page sizes here are powers of two
         const int my_piece = lane % a.pieces;         // (pieces divides 32)
         for (int kvh = member; kvh < KVH && ok; kvh += GS) {
@@ -239,20 +235,10 @@ hkv_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                     const uint32_t dst = smem_base + (uint32_t)stage * STAGE_BYTES;
                     if (lane == 0) mbar_expect_tx(full, STAGE_BYTES);
                     __syncwarp();
-                    for (int b0 = 0; b0 < boxes; b0 += 32) {
-                        const int x = b0 + lane, piece = x % a.pieces;
-                        if constexpr (WHOLE) {
-                            if (x < boxes) {
-                                const int kv = x >= a.pieces, at = piece * a.box_rows;
-                                tma_load_4d(dst + kv * TILE_BYTES + row_off(at), kv ? &tm_v : &tm_k, full, 0, 0, kvh * NCH,
-                                            (pg << (page_shift - 3)) + (((pos0 + at) & (bt.page - 1)) >> 3));
-                            }
-                            continue;
-                        }
-                        const int c = x / a.pieces % NCH, kv = x / (a.pieces * NCH);
-                        if (x < boxes)
-                            tma_load_4d(dst + kv * TILE_BYTES + c * CHUNK_BYTES + piece * a.box_rows * ROWB, kv ? &tm_v : &tm_k, full,
-                                        c * CW, kvh, (pos0 + piece * a.box_rows) & (bt.page - 1), pg);
+                    if (lane < 2 * a.pieces) {             // one box per page and operand (at most 16), all column blocks
+                        const int kv = lane >= a.pieces, at = my_piece * a.box_rows;
+                        tma_load_4d(dst + kv * TILE_BYTES + row_off(at), kv ? &tm_v : &tm_k, full, 0, 0, kvh * NCH,
+                                    (pg << (page_shift - 3)) + (((pos0 + at) & (bt.page - 1)) >> 3));
                     }
                     pg = pg_next;
                     ++issued;
