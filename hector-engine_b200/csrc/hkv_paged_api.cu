@@ -28,7 +28,7 @@ struct hkv_paged_ctx {
     int* plan_done = nullptr;       // CTAs of a plan launch that have finished (zero between launches)
     size_t smem_optin = 0, smem_sm = 0;
     bool staged = false;            // the geometry allows the staged kernels
-    // attention workspace: partial rows of cut requests, the merge kernel's entries, marks of requests to be done again
+    // attention workspace: partial rows of cut requests and where they are, items to be done again
     float *part = nullptr, *chunk_part = nullptr;
     int4 *cuts = nullptr, *chunk_cuts = nullptr;
     int4* fix = nullptr;            // [1 + kFixMax], the count in the first
@@ -381,6 +381,8 @@ int attention(hkv_paged_ctx* c, const void* q, int64_t q_token_stride, const voi
         !aligned(d_q_start, 4) || !aligned(d_step_len, 4) || !aligned(d_key_len, 4))
         return fail(c, HKV_ERR_ALIGNMENT, "attention: a tensor is not aligned to its element size");
     if (requests == 0 || tokens == 0 || max_step == 0) return HKV_OK;
+    // (rows that are done again read their queries after others of the call have been written)
+    if (out == q) return fail(c, HKV_ERR_INVALID_ARG, "attention: out must not be q");
     a.b.table = d_block_table;
     a.b.q_start = d_q_start;
     a.b.step_len = d_step_len;

@@ -7,9 +7,9 @@
 //     contracted with the same staged K and V tiles of 128 positions. A block of queries that fits one tile leaves B out.
 //   * The items of the batch form a line that is cut into equal spans, one per CTA (hkv_paged_line.cuh): a batch of any
 //     mix keeps every SM busy to the end, and one short chunk over a long request is spread over all of them. An item that
-//     is cut leaves partial rows, two sets per CTA at most, which the merge kernel joins.
-//   * Warps: 0-3 softmax of tile A, 4-7 of tile B (one thread per row), 8 producer, 9 MMA issuer, 10 writes the merge
-//     kernel's entry, 11 completes the warpgroup for setmaxnreg. A key tile is a set of boxes, one per page: the
+//     is cut leaves partial rows, two sets per CTA at most, which the finishing kernel joins.
+//   * Warps: 0-3 softmax of tile A, 4-7 of tile B (one thread per row), 8 producer, 9 MMA issuer, 10 writes the
+//     finishing kernel's entry, 11 completes the warpgroup for setmaxnreg. A key tile is a set of boxes, one per page: the
 //     producer's lanes look up one page each, a tile ahead, and issue side by side.
 //   * Tensor memory: S_A, S_B (128 columns each; P is written over the first half of its S), O_A, O_B. Per key tile:
 //     PV_A QK_A(next) PV_B QK_B(next), so that one tile's softmax runs under the other's products; P V of the first half
@@ -17,6 +17,11 @@
 //     its reference by 2^8. (Two threads per row halve nothing: the softmax is bound by its instructions, the exchange and
 //     the doubled bookkeeping cost a tenth.) P is rounded to the element type (its sum is not). 1 of 8 pairs
 //     take a polynomial on the FMA pipe instead of ex2, the narrowest unit.
+//   * Measured (B200, one launch and the finishing one): 2 048 queries over 32k keys, 28 heads of 4, 128 wide: 727 us alone
+//     (1 282 TFLOP/s), 820 us back to back under the power limit; 8 x 448 queries over 2k to 4k keys 150 us. A pair of query
+//     tiles takes 2.0 us per 128 keys against 1.5 us of products at the library's rate. A call costs 10 us until its first
+//     scores are there, an item 2 us of output; a tile on the diagonal takes 3.8 us. A rehearsal of the tile code in front
+//     of the first tile, to warm the instruction caches, made every tile 7 % slower.
 //   * Every wait is bounded and reports through the status word; tensor memory is freed on every path.
 #pragma once
 
@@ -76,7 +81,7 @@ __device__ __forceinline__ uint32_t chunk_line(const Args& a, uint32_t* pre, lon
     return (uint32_t)all;
 }
 
-// The merge kernel's entry of CTA `cta`, by one warp: the item that starts in its span and goes on behind it.
+// The finishing kernel's entry of CTA `cta`, by one warp: the item that starts in its span and goes on behind it.
 __device__ __forceinline__ void chunk_cut_entry(const PagedBatch& b, const PagedLine& l, const uint32_t W, const int ctas, const int cta,
                                                 int4* cuts) {
     const int lane = threadIdx.x & 31;

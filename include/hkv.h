@@ -391,7 +391,7 @@ int32_t hkv_preferred_prefill_chunk(const hkv_geometry* geometry, int32_t sm_cou
  *   k/v plane      [num_pages, page_size, num_kv_heads, head_dim]   binary16 or bfloat16 (`dtype`)
  *   block table    [max_requests][max_pages] int32, entries 0 .. num_pages-1, -1 = not assigned
  *   packed batch   the new tokens of all requests back to back: request r owns the rows
- *                  q_start[r] .. q_start[r] + step_len[r] - 1 of q, k_new, v_new, out
+ *                  q_start[r] .. q_start[r] + step_len[r] - 1 of q, k_new, v_new, out; q_start ascends
  *   slot           page * page_size + row; -1 = the token is not stored
  *
  * One step of a serving loop: hkv_paged_plan (block tables and slot maps from the request lengths),
@@ -507,7 +507,8 @@ int hkv_paged_norm_rope(hkv_paged_ctx* ctx, const hkv_paged_rope* args, void* st
 /* Attention of the new tokens of every request over its pages, their own rows included (append first):
  * query i of request r sits at position total_len[r] - step_len[r] + i and attends the positions up to
  * its own, the last window_size of them with a window. From single tokens to whole prompts, mixed in
- * one call. q [tokens][H][head_dim] with q_token_stride elements between tokens (0 = dense); out dense.
+ * one call. q [tokens][H][head_dim] with q_token_stride elements between tokens (0 = dense); out dense
+ * and apart from q.
  * Rows of `out` that belong to no query are left as they were; a query that attends nothing gets zeros.
  * max_step: upper bound of step_len (queries beyond it are left out); with max_step * H / KVH <= 16 only
  * the single-token kernel is launched. */

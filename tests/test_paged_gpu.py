@@ -680,3 +680,15 @@ def test_two_streams_take_two_contexts(hkv, cuda):
         with torch.cuda.stream(st):
             assert ctx.device_status() == 0
         ctx.close()
+
+
+def test_out_must_not_be_q(hkv, cuda):
+    torch = cuda
+    ctx = hkv.PagedContext(hkv.PagedGeometry(num_heads=4, num_kv_heads=2, head_dim=64, page_size=16, num_pages=8, max_requests=1,
+                                             max_pages=4, max_tokens=20))
+    q, kc = torch.zeros(5, 4, 64, dtype=torch.float16, device="cuda"), torch.zeros(8, 16, 2, 64, dtype=torch.float16, device="cuda")
+    z = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")
+    with pytest.raises(hkv.HkvError) as e:
+        ctx.attention(q, kc, kc, q, z(1, 4), z(1), z(1) + 5, z(1) + 5)
+    assert e.value.status == 1
+    ctx.close()
