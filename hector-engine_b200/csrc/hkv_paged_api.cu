@@ -125,7 +125,9 @@ EncodeTiledFn encode_tiled_fn() {
 bool staged_geometry(const hkv_paged_geometry& g) {
     const int G = g.num_heads / g.num_kv_heads;
     const bool hd = g.head_dim == 64 || g.head_dim == 96 || g.head_dim == 128 || g.head_dim == 256;
-    return hd && G <= 128 && g.page_size >= 8 && (g.page_size & (g.page_size - 1)) == 0;
+    // (the few-token kernel counts the tiles of all requests in 31 bits)
+    const bool count = (double)g.max_requests * ((double)g.max_pages * g.page_size / kTileRows + 1.0) < 2.0e9;
+    return hd && count && G <= 128 && g.page_size >= 8 && (g.page_size & (g.page_size - 1)) == 0;
 }
 
 // Map of a plane with its rows in groups of 8, [group of the pool][column block][row][width elements], so that one box holds
@@ -475,7 +477,7 @@ int hkv_paged_create(hkv_paged_ctx** out, const hkv_paged_geometry* geometry) {
     c->smem_sm = (size_t)per_sm;
     c->staged = staged_geometry(*geometry) && geometry->kernel_select != HKV_KERNEL_GENERIC;
     if (geometry->kernel_select == HKV_KERNEL_TMA && !c->staged)
-        return fail(c, HKV_ERR_GEOMETRY, "the staged kernels need head_dim in {64,96,128,256}, group <= 128, page_size a power of two >= 8");
+        return fail(c, HKV_ERR_GEOMETRY, "the staged kernels need head_dim in {64,96,128,256}, group <= 128, page_size a power of two >= 8, and max_requests * max_pages * page_size below 1.28e11");
     if (c->staged && !(geometry->flags & HKV_FLAG_APPEND_ONLY)) {
         if (!encode_tiled_fn()) return fail(c, HKV_ERR_CUDA, "cuTensorMapEncodeTiled entry point not available");
         for (int nt = 1; nt <= 2; ++nt)

@@ -61,12 +61,12 @@ __device__ __forceinline__ long long line_units(const PagedBatch& b, const Paged
     return (s + unit - 1) / unit;
 }
 
-// floor(x / d) for a quotient below 2^22: a 64-bit division costs a hundred instructions in front of a CTA's first load,
-// the 32-bit estimate is off by one at most.
+// floor(x / d): a 64-bit division costs a hundred instructions in front of a CTA's first load; the 32-bit estimate is off by
+// one at most below 2^22 and by a few at the largest quotients (2^24 tiles).
 __host__ __device__ __forceinline__ int line_div(const long long x, const long long d) {
     long long q = (long long)((float)x / (float)d);
-    if (q * d > x) --q;
-    else if ((q + 1) * d <= x) ++q;
+    while (q * d > x) --q;
+    while ((q + 1) * d <= x) ++q;
     return (int)q;
 }
 

@@ -692,3 +692,13 @@ def test_out_must_not_be_q(hkv, cuda):
         ctx.attention(q, kc, kc, q, z(1, 4), z(1), z(1) + 5, z(1) + 5)
     assert e.value.status == 1
     ctx.close()
+
+
+def test_block_tables_beyond_31_bits_of_tiles_are_not_staged(hkv, cuda):
+    """4 096 requests of up to 2^31 positions: more tiles than the few-token kernel counts."""
+    g = dict(num_heads=4, num_kv_heads=2, head_dim=64, page_size=64, num_pages=8, max_requests=4096, max_pages=2**25 - 1, max_tokens=8)
+    with pytest.raises(hkv.HkvError) as e:
+        hkv.PagedContext(hkv.PagedGeometry(**g, kernel_select=2))
+    assert e.value.status == 2
+    hkv.PagedContext(hkv.PagedGeometry(**g)).close()
+    hkv.PagedContext(hkv.PagedGeometry(**{**g, "max_pages": 2**14}, kernel_select=2)).close()
