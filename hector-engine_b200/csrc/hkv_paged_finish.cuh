@@ -4,7 +4,7 @@
 // first those of the few-token kernel (a block per span, KV head and query row: few rows, up to hundreds of parts, so
 // eight warps deal the parts of a row among them), then those of the prompt kernel (many rows of mostly two parts). It is launched while the kernel before it still runs and waits for its end on
 // the GPU. Bound: launch latency; the partial rows (39 MB at most) come out of the L2:
-// 4 us for a few-token call, 12 to 18 us where every CTA of a prompt launch cut an item.
+// 4 us for a few-token call, 10 to 16 us where every CTA of a prompt launch cut an item.
 #pragma once
 
 #include "hkv_paged_chunk.cuh"
@@ -23,7 +23,8 @@ struct PagedFinishArgs {
     int may_fix;                  // 0: a single query per request, nothing can be on the list
 };
 // (blocks of 32 rows behind those of the few-token kernel)
-__host__ __device__ inline int finish_blocks(const PagedFinishArgs& a, int KVH) { return a.spans * KVH * a.cols + a.ctas * a.tiles * 4; }
+__host__ __device__ inline int finish_parts(int HD) { return HD > 128 ? 2 : 1; }     // blocks per 32 rows: 128 columns each
+__host__ __device__ inline int finish_blocks(const PagedFinishArgs& a, int KVH) { return a.spans * KVH * a.cols + a.ctas * a.tiles * 4 * finish_parts(a.t.HD); }
 
 template <typename T>
 __device__ __forceinline__ void finish_small(const PagedFinishArgs& a, const int block, const int fix_count) {
@@ -91,18 +92,20 @@ __device__ __forceinline__ void finish_small(const PagedFinishArgs& a, const int
     }
 }
 
-// 32 rows per block: a warp takes 8 rows and every eighth group of 4 x 4 columns, so that it reads whole lines of a set and
-// writes whole sectors of a row; the loads of two parts are in flight together, nothing in front of them but the entry.
+// 32 rows and 128 columns per block (80 registers, three blocks per SM; with whole rows of head_dim 256 two blocks, and calls that cut
+// much took 2 to 5 us longer). A warp takes 8 rows and every eighth group of 4 x 4 columns, so that it reads whole lines of
+// a set and writes whole sectors of a row; the loads of two parts are in flight together, nothing in front of them but the entry.
 template <typename T>
 __device__ __forceinline__ void finish_chunk(const PagedFinishArgs& a, const int block, const int fix_count) {
-    const int rows = a.tiles * 128, shares = rows / 32;
-    const int cta = block / shares, share = block % shares;
+    const int rows = a.tiles * 128, wide = finish_parts(a.t.HD), shares = rows / 32 * wide;
+    const int cta = block / shares, share = block % shares / wide;
     const int4 cut = a.chunk_cuts[cta];
     const int parts = cut.w;
     if (parts <= 1) return;
     if (fix_count && paged_to_fix(a.fix, fix_count, cut.x, cut.z, cut.y)) return;
     const int G = a.t.H / a.t.KVH, HD = a.t.HD, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int row = share * 32 + (warp & 3) * 8 + (lane & 7), cb = (warp >> 2) * 4 + (lane >> 3);
+    const int cols = HD < 128 ? HD : 128;
+    const int row = share * 32 + (warp & 3) * 8 + (lane & 7), cb = block % wide * 32 + (warp >> 2) * 4 + (lane >> 3);
     const int ql = row % 128 / G, i = cut.z * a.QB + row / 128 * a.QT + ql;
     const PagedRequest q = paged_request(a.t.b, cut.x);
     if (ql >= a.QT || i >= q.n) return;
@@ -110,20 +113,20 @@ __device__ __forceinline__ void finish_chunk(const PagedFinishArgs& a, const int
     // part 0 sits in this CTA's second slot, the others in the first slots of the CTAs behind it
     const float* base = a.chunk_part + 2ll * cta * set;
     float M = kLow, L = 0.0f;
-    float4 acc[8];
+    float4 acc[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int e = 0; e < 4; ++e) acc[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int p0 = 0; p0 < parts; p0 += 2) {
         float2 ml[2];
-        float4 x[2][8];
+        float4 x[2][4];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const int p = p0 + u;
             const float* s = base + (2ll * p + (p == 0 ? 1 : 0)) * set;
             ml[u] = p < parts ? *reinterpret_cast<const float2*>(s + (long long)rows * HD + 2 * row) : make_float2(kLow, 0.0f);
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                x[u][e] = p < parts && 32 * e < HD ? *reinterpret_cast<const float4*>(s + ((long long)(cb + 8 * e) * rows + row) * 4)
+            for (int e = 0; e < 4; ++e)
+                x[u][e] = p < parts && 32 * e < cols ? *reinterpret_cast<const float4*>(s + ((long long)(cb + 8 * e) * rows + row) * 4)
                                                    : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
 #pragma unroll
@@ -131,7 +134,7 @@ __device__ __forceinline__ void finish_chunk(const PagedFinishArgs& a, const int
             const float Mn = fmaxf(M, ml[u].x), keep = exp2f(M - Mn), w = exp2f(ml[u].x - Mn);
             L = fmaf(ml[u].y, w, L * keep);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
+            for (int e = 0; e < 4; ++e) {
                 acc[e].x = fmaf(x[u][e].x, w, acc[e].x * keep); acc[e].y = fmaf(x[u][e].y, w, acc[e].y * keep);
                 acc[e].z = fmaf(x[u][e].z, w, acc[e].z * keep); acc[e].w = fmaf(x[u][e].w, w, acc[e].w * keep);
             }
@@ -141,12 +144,12 @@ __device__ __forceinline__ void finish_chunk(const PagedFinishArgs& a, const int
     const float inv = L == 0.0f ? 0.0f : (L < kSumLimit ? 1.0f / L : NAN);
     T* op = (T*)a.t.out + ((long long)(q.start + i) * a.t.H + (long long)cut.y * G + row % 128 % G) * HD + 4 * cb;
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-        if (32 * e < HD) *reinterpret_cast<uint2*>(op + 32 * e) = make_uint2(pack2<T>(acc[e].x * inv, acc[e].y * inv), pack2<T>(acc[e].z * inv, acc[e].w * inv));
+    for (int e = 0; e < 4; ++e)
+        if (32 * e < cols) *reinterpret_cast<uint2*>(op + 32 * e) = make_uint2(pack2<T>(acc[e].x * inv, acc[e].y * inv), pack2<T>(acc[e].z * inv, acc[e].w * inv));
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) hkv_paged_finish_kernel(const __grid_constant__ PagedFinishArgs a) {
+__global__ void __launch_bounds__(256, 3) hkv_paged_finish_kernel(const __grid_constant__ PagedFinishArgs a) {
     wait_for_previous();
     const int count = a.may_fix ? *reinterpret_cast<volatile int*>(a.fix.head) : 0;
     const int small = a.spans * a.t.KVH * a.cols;
