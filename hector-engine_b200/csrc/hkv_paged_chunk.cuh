@@ -15,8 +15,8 @@
 //     PV_A QK_A(next) PV_B QK_B(next), so that one tile's softmax runs under the other's products; P V of the first half
 //     of a tile's keys starts while P of the second half is computed. O is rescaled only when a row's maximum outgrows
 //     its reference by 2^8. (Two threads per row halve nothing: the softmax is bound by its instructions, the exchange and
-//     the doubled bookkeeping cost a tenth.) P is rounded to the element type (its sum is not). 1 of 8 pairs
-//     take a polynomial on the FMA pipe instead of ex2, the narrowest unit.
+//     the doubled bookkeeping cost a tenth.) P is rounded to the element type (its sum is not). In fp16 1 of
+//     8 pairs take a polynomial on the FMA pipe instead of ex2, the narrowest unit; bf16 takes none (kCkEmuOf8).
 //   * Measured (B200, one launch and the finishing one): 2 048 queries over 32k keys, 28 heads of 4, 128 wide: 727 us alone
 //     (1 282 TFLOP/s), 820 us back to back under the power limit; 8 x 448 queries over 2k to 4k keys 150 us. A pair of query
 //     tiles takes 2.0 us per 128 keys against 1.5 us of products at the library's rate. A call costs 10 us until its first
@@ -36,7 +36,11 @@ namespace hkv {
 constexpr int kCkRows = 128, kCkKeys = 128;
 constexpr int kCkStages = 2;              // K tiles and V tiles in flight
 constexpr int kCkThreads = 384;
-constexpr int kCkEmuOf8 = 1;              // pairs of every 8 whose exp2 runs on the FMA pipe (0, 1, 2, 3: 823, 788, 864, 915 us for 2 048 queries over 32k keys)
+// Pairs of every 8 whose exp2 runs on the FMA pipe, fp16 only. The polynomial ends at 2^-100, for a hidden key too: fp16
+// rounds that to zero, but bf16 carries it to the second product, where 2^-100 times a large hidden value is not nothing.
+// (2 048 queries over 32k keys, with and without in turn: head_dim 128 713 to 739 us against 721 to 747; head_dim 64 330
+// against 319. 8 x 448 queries over 4k keys 145 against 147. 2 and 3 of 8: 10 and 16 % slower than 1.)
+constexpr int kCkEmuOf8 = 1;
 constexpr int kCkDesc = 16;               // words of a work descriptor
 
 struct PagedChunkArgs {
@@ -235,6 +239,7 @@ hkv_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     constexpr int TILE_BYTES = kCkRows * HD * 2;
     constexpr int CHUNK_OFF = WHOLE ? 1024 : CHUNK_BYTES, GROUP_OFF = WHOLE ? NCH * 1024 : 1024;
     constexpr int COL_BOXES = WHOLE ? 1 : NCH, HEAD_STEP = WHOLE ? NCH : 1;   // boxes per piece; coordinate step of a KV head
+    constexpr int EMU = std::is_same<T, __half>::value ? kCkEmuOf8 : 0;
     constexpr uint32_t TMEM_COLS = 512;
     constexpr uint32_t COL_S = 0, COL_O = 256;         // + 128 * group
     constexpr uint32_t FMT = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);   // operand type of the MMA
@@ -551,9 +556,9 @@ hkv_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
                         ffma2_bcast(x0, x1, __uint_as_float(sv[c][j]), __uint_as_float(sv[c][j + 1]), a.t.scale_log2, neg_m);
                         ffma2_bcast(x2, x3, __uint_as_float(sv[c][j + 2]), __uint_as_float(sv[c][j + 3]), a.t.scale_log2, neg_m);
                         float p0, p1, p2, p3;
-                        if (((j / 4) * 2) % 8 < kCkEmuOf8) ex2_emu2_nan(p0, p1, x0, x1);
+                        if (((j / 4) * 2) % 8 < EMU) ex2_emu2_nan(p0, p1, x0, x1);
                         else { p0 = ex2_approx(x0); p1 = ex2_approx(x1); }
-                        if (((j / 4) * 2 + 1) % 8 < kCkEmuOf8) ex2_emu2_nan(p2, p3, x2, x3);
+                        if (((j / 4) * 2 + 1) % 8 < EMU) ex2_emu2_nan(p2, p3, x2, x3);
                         else { p2 = ex2_approx(x2); p3 = ex2_approx(x3); }
                         fadd2_acc(lsum0, lsum1, p0, p1);
                         fadd2_acc(lsum2, lsum3, p2, p3);

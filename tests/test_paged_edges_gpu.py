@@ -1,0 +1,100 @@
+"""GPU tests of the paged cache at the edges of what its documentation promises: values that a mask or a vanishing weight
+hides, in both types. Models and tolerances: tests/_paged.py."""
+import math
+
+import numpy as np
+import pytest
+
+import _paged as P
+
+pytestmark = pytest.mark.gpu
+
+DT = ["float16", "bfloat16"]
+STAGED = [(28, 4, 128), (14, 2, 64), (8, 8, 96), (16, 8, 256)]
+
+
+def dt(torch, name):
+    return getattr(torch, name)
+
+
+def i32(torch, a):
+    return torch.as_tensor(np.asarray(a), dtype=torch.int32).cuda()
+
+
+# ---- values that must not reach a row ---------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("kind", ["large", "nan", "inf"])
+@pytest.mark.parametrize("heads", STAGED + [(6, 2, 80)], ids=str)
+@pytest.mark.parametrize("steps", [[2, 1, 2], [2, 70, 300]], ids=["tokens", "chunks"])
+def test_hidden_values_of_both_types(hkv, cuda, heads, steps, kind, dtype):
+    """A large finite value, NaN or infinity in each of the newest rows of a chunk in turn (16 of them: the kernels treat the
+    columns of a tile in patterns of up to 16) and in a row that only its first queries' window reaches. A finite one leaves every row that does not look at it bit for bit as it was (its weight is zero, not small);
+    the others send the item to be done again, so those rows are held against the 64-bit model."""
+    torch = cuda
+    H, KVH, HD = heads
+    D = dt(torch, dtype)
+    value = {"nan": math.nan, "inf": math.inf, "large": 1e30 if dtype == "bfloat16" else 6e4}[kind]
+    gen = torch.Generator().manual_seed(13)
+    keys, page, window = [40, 333, 700], 16, 150
+    kc, vc, table = P.make_pages(torch, gen, keys, page, 70, 50, KVH, HD, D)
+    q = torch.randn(sum(steps), H, HD, generator=gen).to(D).cuda()
+    ctx = hkv.PagedContext(hkv.PagedGeometry(num_heads=H, num_kv_heads=KVH, head_dim=HD, page_size=page, num_pages=70, max_requests=3,
+                                             max_pages=50, max_tokens=sum(steps), window_size=window, dtype=dtype))
+    starts = np.concatenate([[0], np.cumsum(steps)])
+    args = (table, i32(torch, starts), i32(torch, steps), i32(torch, keys))
+    clean, got = torch.empty_like(q), torch.empty_like(q)
+    ctx.attention(q, kc, vc, clean, *args, max_step=max(steps))
+    ref, tol, live = P.attend_model(torch, q, kc, vc, table, starts, steps, keys, ctx.geometry.default_scale, page, window)
+    assert live.all()
+    for r in range(3):
+        newest = range(keys[r] - min(16, steps[r]), keys[r])
+        for j in {*newest, max(0, keys[r] - steps[r] + 1 - window)}:
+            for plane in (vc, kc):
+                pg, row = int(table[r, j // page]), j % page
+                old = plane[pg, row].clone()
+                plane[pg, row, 0, 3] = value
+                ctx.attention(q, kc, vc, got, *args, max_step=max(steps))
+                plane[pg, row] = old
+                pos = keys[r] - steps[r] + torch.arange(steps[r], device="cuda")
+                blind = torch.ones(q.shape[0], dtype=torch.bool, device="cuda")
+                blind[starts[r]:starts[r] + steps[r]] = (pos < j) | (pos >= j + window)
+                if kind == "large":
+                    assert torch.equal(got[blind], clean[blind]), f"{int((got[blind] != clean[blind]).sum())} elements moved"
+                else:
+                    assert ((got[blind].double() - ref[blind]).abs() <= tol[blind]).all()
+    assert ctx.device_status() == 0
+    ctx.close()
+
+
+@pytest.mark.parametrize("heads", STAGED + [(6, 2, 80)], ids=str)
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "cross"])
+def test_vanishing_weights_are_zero(hkv, cuda, heads, causal):
+    """One key's score stands 640 above all others (weights of 2^-923, which is zero in 32 bits), the others' values are
+    1e30: every row is that key's value. Tolerance: half a step for its weight, half a step for the result, and 2e-4 for the
+    error of exp2 in weight and sum."""
+    torch = cuda
+    H, KVH, HD = heads
+    G = H // KVH
+    gen = torch.Generator().manual_seed(17)
+    steps, keys, page = [1, 200, 3], [300, 500, 77], 16
+    kc, vc, table = P.make_pages(torch, gen, keys, page, 70, 40, KVH, HD, torch.bfloat16)
+    kc, vc = torch.zeros_like(kc), torch.full_like(vc, 1e30)
+    want = []
+    for r in range(3):
+        at = int(table[r, 0])
+        kc[at, 0, :, 0] = 40.0
+        vc[at, 0] = torch.randn(KVH, HD, generator=gen).bfloat16().cuda()
+        want.append(vc[at, 0].double().repeat_interleave(G, 0).expand(steps[r], H, HD))
+    want = torch.cat(want)
+    T = sum(steps)
+    q = torch.zeros(T, H, HD, dtype=torch.bfloat16, device="cuda")
+    q[..., 0] = 16.0
+    out = torch.empty_like(q)
+    ctx = hkv.PagedContext(hkv.PagedGeometry(num_heads=H, num_kv_heads=KVH, head_dim=HD, page_size=page, num_pages=70, max_requests=3,
+                                             max_pages=40, max_tokens=T, dtype="bfloat16"))
+    call = ctx.attention if causal else ctx.cross_attention
+    call(q, kc, vc, out, table, i32(torch, [0, 1, 201]), i32(torch, steps), i32(torch, keys), max_step=200, scale=1.0)
+    off = (out.double() - want).abs()
+    assert (off <= (2 * P.unit(torch, torch.bfloat16) + 2e-4) * want.abs()).all(), f"{off.max().item():.3e}"
+    assert ctx.device_status() == 0
+    ctx.close()
