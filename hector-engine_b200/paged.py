@@ -142,6 +142,8 @@ class PagedContext:
         s = t.stride()
         if (hd > 1 and s[2] != 1) or (heads > 1 and s[1] != hd):
             raise HkvError(2, f"{name}: heads and head_dim must be contiguous, strides {s}")
+        if tokens > 1 and s[0] < heads * hd:                # (a broadcast token's stride of 0 would mean "dense" below)
+            raise HkvError(2, f"{name}: tokens overlap, strides {s}: expand()ed rows have to be copied first")
         return t.data_ptr(), (s[0] if tokens > 1 else 0)
 
     def _plane(self, name, t):

@@ -58,3 +58,29 @@ def test_plan_model_keeps_every_page_once():
         assert sorted(held + list(free[:count])) == list(range(num_pages))
         live = out["slots"][out["slots"] >= 0]
         assert len(set(live)) == len(live)
+
+
+def rows_of(hkv, heads, head_dim, dtype):
+    """PagedContext's check of [tokens, heads, head_dim] tensors without a device: the context of a CPU tensor's device index."""
+    import torch
+    ctx = object.__new__(hkv.PagedContext)
+    ctx._h, ctx._hd, ctx._dtype, ctx._index = None, head_dim, getattr(torch, dtype), torch.zeros(0).get_device()
+    return lambda t, tokens: ctx._rows("x", t, heads, tokens)
+
+
+@pytest.mark.parametrize("heads,head_dim", [(4, 64), (1, 64), (3, 1), (1, 1)])
+def test_token_strides_that_are_passed_on(hkv, heads, head_dim):
+    """0 means dense in the library, so a broadcast token (stride 0) must never get there, nor tokens that overlap."""
+    import torch
+    rows, row = rows_of(hkv, heads, head_dim, "float16"), heads * head_dim
+    h = lambda *s: torch.zeros(*s, dtype=torch.float16)
+    assert rows(h(5, heads, head_dim), 5)[1] == 0
+    assert rows(h(5, row + 8)[:, :row].unflatten(1, (heads, head_dim)), 5)[1] == row + 8
+    assert rows(h(1, heads, head_dim).expand(1, heads, head_dim), 1)[1] == 0
+    assert rows(h(0, heads, head_dim), 0)[1] == 0
+    one = h(1, heads, head_dim)
+    for t in (one.expand(5, heads, head_dim), torch.as_strided(h(5 * row + 8), (2, heads, head_dim), (0, head_dim, 1)),
+              *([torch.as_strided(h(5 * row), (5, heads, head_dim), (row - 1, head_dim, 1))] if row > 1 else [])):
+        with pytest.raises(hkv.HkvError) as e:
+            rows(t, t.shape[0])
+        assert e.value.status == 2, e.value

@@ -98,3 +98,29 @@ def test_vanishing_weights_are_zero(hkv, cuda, heads, causal):
     assert (off <= (2 * P.unit(torch, torch.bfloat16) + 2e-4) * want.abs()).all(), f"{off.max().item():.3e}"
     assert ctx.device_status() == 0
     ctx.close()
+
+
+# ---- tensors whose tokens lie on top of each other ----------------------------------------------------------------------
+def test_broadcast_rows_are_refused(hkv, cuda):
+    """expand()ed rows have a token stride of 0, which the library reads as dense: refused in every place they can come in."""
+    torch = cuda
+    ctx = hkv.PagedContext(hkv.PagedGeometry(num_heads=4, num_kv_heads=2, head_dim=64, page_size=16, num_pages=8, max_requests=3,
+                                             max_pages=4, max_tokens=20))
+    h = lambda *s: torch.zeros(*s, dtype=torch.float16, device="cuda")
+    z = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")
+    q, k, v, out, kc, vc = h(5, 4, 64), h(5, 2, 64), h(5, 2, 64), h(5, 4, 64), h(8, 16, 2, 64), h(8, 16, 2, 64)
+    wide_q, wide_k = h(1, 4, 64).expand(5, 4, 64), h(1, 2, 64).expand(5, 2, 64)
+    att = lambda **o: ctx.attention(o.get("q", q), kc, vc, o.get("out", out), z(3, 4), z(4), z(3), z(3), max_step=1)
+    cross = lambda **o: ctx.cross_attention(o.get("q", q), kc, vc, o.get("out", out), z(3, 4), z(4), z(3), z(3), max_step=1)
+    rope = lambda **o: ctx.norm_rope(o.get("q", q), o.get("k", k), None, z(5), q_out=o.get("q_out"), k_out=o.get("k_out"))
+    paged = lambda **o: ctx.norm_rope(q, o.get("k", k), o.get("v", v), z(5), slots=z(5) - 1, k_cache=kc, v_cache=vc)
+    for call in (lambda: att(q=wide_q), lambda: att(out=wide_q), lambda: cross(q=wide_q), lambda: cross(out=wide_q),
+                 lambda: ctx.append(wide_k, wide_k, kc, vc, z(5) - 1), lambda: ctx.append(k, wide_k, kc, vc, z(5) - 1),
+                 lambda: rope(q=wide_q), lambda: rope(k=wide_k), lambda: rope(q_out=wide_q), lambda: rope(k_out=wide_k),
+                 lambda: paged(k=wide_k), lambda: paged(v=wide_k)):
+        with pytest.raises(hkv.HkvError) as e:
+            call()
+        assert e.value.status == 2, e.value
+    att(), cross(), rope(), paged()
+    assert ctx.device_status() == 0
+    ctx.close()
