@@ -26,6 +26,7 @@ DIST_LIB = os.path.join(PKG_DIR, "libhkv_dist.so")
 HOST_TESTS = os.path.join(REPO, "tests", "cpp", "hkv_host_tests")
 WATCH_TESTS = os.path.join(REPO, "tests", "cpp", "hkv_watch_tests")
 SEQSPLIT_TESTS = os.path.join(REPO, "tests", "cpp", "hkv_seqsplit_tests")
+SCHEDULE_TESTS = os.path.join(REPO, "tests", "cpp", "hkv_paged_schedule_tests")
 GEMMA4_TESTS = os.path.join(REPO, "tests", "cpp", "hkv_gemma4_tests")
 
 LIB_SOURCES = ["hkv_api.cu", "hkv_paged_api.cu"]
@@ -124,6 +125,17 @@ def build_watch_tests(force: bool = False) -> str | None:
     return WATCH_TESTS
 
 
+def build_schedule_tests(force: bool = False) -> str | None:
+    """CPU-only tests of the paged kernels' host-callable schedule arithmetic (no device call is made)."""
+    main = os.path.join(REPO, "tests", "cpp", "hkv_paged_schedule_tests.cu")
+    if not os.path.exists(main):
+        return None
+    if not force and _newer(SCHEDULE_TESTS, _sources(CSRC) + [main]):
+        return SCHEDULE_TESTS
+    subprocess.run([_nvcc(), *ARCH, "-O2", "-std=c++17", "-o", SCHEDULE_TESTS, main, "-I", CSRC], check=True)
+    return SCHEDULE_TESTS
+
+
 def build_seqsplit_tests(force: bool = False) -> str | None:
     """C++ test of SeqSplitDecoder: one process per GPU, NCCL id handed over through a file."""
     main = os.path.join(REPO, "tests", "cpp", "hkv_seqsplit_tests.cpp")
@@ -174,6 +186,7 @@ def build_all(force: bool = False) -> None:
     build_oracle()
     build_host_tests(force=force)
     build_watch_tests(force=force)
+    build_schedule_tests(force=force)
     build_seqsplit_tests(force=force)
     build_gemma4_tests(force=force)
     build_dropin()

@@ -65,7 +65,7 @@ struct PagedRequest {
     int pos0;          // position of query 0 (causal); may be negative: such queries attend nothing
     int keys;          // positions held, at most cols * page
 };
-__device__ __forceinline__ PagedRequest paged_request(const PagedBatch& a, int r) {
+__host__ __device__ __forceinline__ PagedRequest paged_request(const PagedBatch& a, int r) {
     PagedRequest q;
     q.start = a.q_start[r];
     const int step = a.step_len[r], len = a.key_len[r];
@@ -78,16 +78,25 @@ __device__ __forceinline__ PagedRequest paged_request(const PagedBatch& a, int r
     q.pos0 = q.keys - (step > 0 ? step : 0);
     return q;
 }
-// Keys [lo, hi) that query i of a request attends; hi <= lo: none.
-__device__ __forceinline__ void paged_key_range(const PagedBatch& a, const PagedRequest& q, int i, int& lo, int& hi) {
+// Keys [lo, hi) that query i of a request attends, 0 <= lo; hi <= lo: none. Lengths may come up to the end of 31 bits
+// (whatever the arrays hold, and with max_pages * page_size near it also in earnest), so a bound is never added to: tiles
+// are counted as (hi - 1) / rows + 1, and what lies behind a tile or box is asked by a difference.
+__host__ __device__ __forceinline__ void paged_key_range(const PagedBatch& a, const PagedRequest& q, int i, int& lo, int& hi) {
     lo = 0;
     hi = q.keys;
     if (a.causal) {
         const int p = q.pos0 + i;
-        if (p + 1 < hi) hi = p + 1;
-        if (a.window > 0 && p + 1 - a.window > 0) lo = p + 1 - a.window;
+        if (p + 1 < hi) hi = p >= 0 ? p + 1 : 0;
+        if (a.window > 0 && p >= a.window) lo = p - a.window + 1;
     }
 }
+// Whether a tile of `rows` positions from `row0` on holds one that not all of a run of queries attend (their lower bounds
+// up to lo_last, their upper ones from hi_first on).
+__host__ __device__ __forceinline__ bool paged_tile_masked(int row0, int rows, int lo_last, int hi_first) {
+    return row0 < lo_last || hi_first - row0 < rows;
+}
+// Whether none of `rows` positions from p on is in [lo, hi).
+__host__ __device__ __forceinline__ bool paged_box_hidden(int p, int rows, int lo, int hi) { return p >= hi || lo - p >= rows; }
 
 // ---- launches that overlap --------------------------------------------------------------------------------------------
 // The dependent launch may be set up from here on; it waits for this one's end before it reads anything.
@@ -441,11 +450,11 @@ __device__ __forceinline__ void paged_row(const PagedAttnArgs& a, const int r, c
     }
     float m = kLow, l = 0.0f;
     const int32_t* table = a.b.table + (long long)r * a.b.cols;
-    for (int s = k_lo + warp; s < k_hi; s += WARPS) {
-        const int pg = table[s / a.b.page];
+    for (uint32_t s = (uint32_t)k_lo + warp; s < (uint32_t)k_hi; s += WARPS) {
+        const int pg = table[s / (uint32_t)a.b.page];
         const bool in = pg >= 0 && pg < a.b.pages;   // an entry outside the planes: rows of zeros
         if (!in && lane == 0) atomicOr(a.b.status, kStatusBoundCheck);
-        const long long row = (((long long)(in ? pg : 0) * a.b.page + s % a.b.page) * a.KVH + kvh) * a.HD;
+        const long long row = (((long long)(in ? pg : 0) * a.b.page + s % (uint32_t)a.b.page) * a.KVH + kvh) * a.HD;
         const T* kr = (const T*)a.k_cache + row;
         const T* vr = (const T*)a.v_cache + row;
         float dot = 0.0f;

@@ -328,7 +328,7 @@ hkv_paged_chunk_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
             const int32_t* table = bt.table + (long long)r * bt.cols;
             // page of a box: behind the tensor (zeros, nothing read) where no query of the item looks
             auto look_up = [&](int pos) -> int {
-                if (pos >= hi || pos + a.box_rows <= lo) return bt.pages;
+                if (paged_box_hidden(pos, a.box_rows, lo, hi)) return bt.pages;
                 const int pg = __ldg(table + (pos >> page_shift));
                 if (pg >= 0 && pg < bt.pages) return pg;
                 atomicOr(bt.status, kStatusBoundCheck);

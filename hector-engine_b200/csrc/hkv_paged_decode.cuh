@@ -47,15 +47,15 @@ struct PagedDecodeArgs {
 
 // Tiles of a request on the line: at least one for every request with queries, so that rows that attend nothing are
 // written too.
-__device__ __forceinline__ void paged_tiles(const PagedBatch& b, const PagedRequest& q, int& tile_lo, int& n_tiles) {
+__host__ __device__ __forceinline__ void paged_tiles(const PagedBatch& b, const PagedRequest& q, int& tile_lo, int& n_tiles) {
     int lo, hi, lo2, hi2;
     paged_key_range(b, q, 0, lo, hi);
     paged_key_range(b, q, q.n - 1, lo2, hi2);
     tile_lo = lo / kTileRows;
-    n_tiles = hi2 > lo ? (hi2 + kTileRows - 1) / kTileRows - tile_lo : 1;
+    n_tiles = hi2 > lo ? (hi2 - 1) / kTileRows + 1 - tile_lo : 1;
 }
 // Whether the few-token kernel (this file) takes a request: at most `limit` query rows per KV head.
-__device__ __forceinline__ bool paged_is_small(const PagedRequest& q, int G, int limit) { return q.n > 0 && (long long)q.n * G <= limit; }
+__host__ __device__ __forceinline__ bool paged_is_small(const PagedRequest& q, int G, int limit) { return q.n > 0 && (long long)q.n * G <= limit; }
 
 template <typename T>
 __device__ __forceinline__ void mma_16816_t(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
@@ -223,7 +223,7 @@ hkv_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                 const int32_t* table = bt.table + (long long)r * bt.cols;
                 // page of this lane's box: behind the tensor (zeros, nothing read) where no query looks
                 auto look_up = [&](int p) -> int {
-                    if (p >= hi || p + a.box_rows <= lo) return bt.pages;
+                    if (paged_box_hidden(p, a.box_rows, lo, hi)) return bt.pages;
                     const int pg = __ldg(table + (p >> page_shift));
                     if (pg >= 0 && pg < bt.pages) return pg;
                     atomicOr(bt.status, kStatusBoundCheck);
@@ -330,7 +330,7 @@ hkv_paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                 const uint32_t vbase = kbase + TILE_BYTES;
                 uint8_t* vgen = smem + (size_t)stage * STAGE_BYTES + TILE_BYTES;
                 const int row0 = (t0 + t) * kTileRows;
-                const bool masked = row0 < lo_last || row0 + kTileRows > hi_first;
+                const bool masked = paged_tile_masked(row0, kTileRows, lo_last, hi_first);
                 if (masked) {
                     // V rows that no query attends are zeroed; values that are not finite in rows that only some attend are
                     // dropped and the request is marked, because 0 * NaN would reach the queries they are hidden from.

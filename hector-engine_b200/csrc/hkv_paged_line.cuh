@@ -45,17 +45,17 @@ __host__ __device__ inline long long line_prefix(const PagedLine& l, int window,
 }
 
 // Key tiles of a block: at least one, so that rows that attend nothing are written too.
-__device__ __forceinline__ void line_tiles(const PagedBatch& b, const PagedLine& l, const PagedRequest& q, int p, int& kt0, int& nt) {
+__host__ __device__ __forceinline__ void line_tiles(const PagedBatch& b, const PagedLine& l, const PagedRequest& q, int p, int& kt0, int& nt) {
     int lo, hi, lo2, hi2;
     const int i0 = p * l.QB, i1 = (i0 + l.QB < q.n ? i0 + l.QB : q.n) - 1;
     paged_key_range(b, q, i0, lo, hi);
     paged_key_range(b, q, i1, lo2, hi2);
     kt0 = lo / l.keys;
-    nt = hi2 > lo ? (hi2 + l.keys - 1) / l.keys - kt0 : 1;
+    nt = hi2 > lo ? (hi2 - 1) / l.keys + 1 - kt0 : 1;
 }
 
 // Units of a request on the line, all KV heads.
-__device__ __forceinline__ long long line_units(const PagedBatch& b, const PagedLine& l, const PagedRequest& q) {
+__host__ __device__ __forceinline__ long long line_units(const PagedBatch& b, const PagedLine& l, const PagedRequest& q) {
     const long long s = line_prefix(l, b.window, b.causal, q.pos0, q.keys, line_blocks(q.n, l.QB)) * l.KVH;
     const long long unit = (long long)kLineUnit << l.shift;
     return (s + unit - 1) / unit;
@@ -72,7 +72,7 @@ __host__ __device__ __forceinline__ int line_div(const long long x, const long l
 
 // The cut at unit u of the line (W units in all). A cut that would fall behind an item's last tile is the start of the
 // next item; u = W is the cut behind everything ({requests, 0, 0, 0}).
-__device__ __forceinline__ LineCut line_locate(const PagedBatch& b, const PagedLine& l, const uint32_t u, const uint32_t W) {
+__host__ __device__ __forceinline__ LineCut line_locate(const PagedBatch& b, const PagedLine& l, const uint32_t u, const uint32_t W) {
     LineCut c{b.requests, 0, 0, 0};
     if (u >= W) return c;
     int lo = 0, hi = b.requests - 1;      // the last request that starts at or before u
@@ -108,8 +108,8 @@ __device__ __forceinline__ LineCut line_locate(const PagedBatch& b, const PagedL
     }
     return c;
 }
-__device__ __forceinline__ bool line_same_item(const LineCut& a, const LineCut& b) { return a.r == b.r && a.kvh == b.kvh && a.p == b.p; }
-__device__ __forceinline__ bool line_before(const LineCut& a, const LineCut& b) {
+__host__ __device__ __forceinline__ bool line_same_item(const LineCut& a, const LineCut& b) { return a.r == b.r && a.kvh == b.kvh && a.p == b.p; }
+__host__ __device__ __forceinline__ bool line_before(const LineCut& a, const LineCut& b) {
     if (a.r != b.r) return a.r < b.r;
     if (a.kvh != b.kvh) return a.kvh < b.kvh;
     if (a.p != b.p) return a.p < b.p;

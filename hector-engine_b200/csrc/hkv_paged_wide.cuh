@@ -108,7 +108,7 @@ hkv_paged_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
             paged_key_range(bt, q, i1, x, hi);
             const int32_t* table = bt.table + (long long)r * bt.cols;
             auto look_up = [&](int pos) -> int {       // behind the tensor (zeros) where no query of the item looks
-                if (pos >= hi || pos + a.box_rows <= lo) return bt.pages;
+                if (paged_box_hidden(pos, a.box_rows, lo, hi)) return bt.pages;
                 const int pg = __ldg(table + (pos >> page_shift));
                 if (pg >= 0 && pg < bt.pages) return pg;
                 atomicOr(bt.status, kStatusBoundCheck);
@@ -312,7 +312,7 @@ hkv_paged_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_con
                 tc_wait_st();
                 l_run += lsum0 + lsum1;
                 // tiles that not every query of the item sees whole: rows that none attends and values that are not finite
-                if (kstart < lo_last || kstart + kWdKeys > hi_first) {
+                if (paged_tile_masked(kstart, kWdKeys, lo_last, hi_first)) {
                     const uint32_t vs = gt % kWdStages;
                     ok = __all_sync(0xffffffffu, mbar_wait(B_VFULL + 8 * vs, (gt / kWdStages) & 1, bt.status));
                     if (!ok) continue;

@@ -84,3 +84,13 @@ def test_token_strides_that_are_passed_on(hkv, heads, head_dim):
         with pytest.raises(hkv.HkvError) as e:
             rows(t, t.shape[0])
         assert e.value.status == 2, e.value
+
+
+def test_schedule_arithmetic():
+    """tests/cpp/hkv_paged_schedule_tests.cu: the kernels' host-callable schedule arithmetic, run on the CPU."""
+    import importlib
+    import subprocess
+    binary = importlib.import_module("hector-engine_b200.build").build_schedule_tests()
+    res = subprocess.run([binary], capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0, res.stdout + res.stderr
+    assert res.stdout.count("PASS:") == 2 and "ALL PASSED" in res.stdout
