@@ -31,7 +31,7 @@ __host__ __device__ inline int line_blocks(int n, int QB) { return (n + QB - 1) 
 
 // Sum of the costs of the first p blocks of a request and KV head.
 __host__ __device__ inline long long line_prefix(const PagedLine& l, int window, int causal, const int pos0, const int keys, const int p) {
-    if (!causal) return (long long)p * (keys + kLineOverhead);
+    if (!causal) return p * ((long long)keys + kLineOverhead);
     // blocks that end before position 0 attend nothing; then base + (i + 1) * QB keys, up to the cap
     const long long none = pos0 < 0 ? (-(long long)pos0 / l.QB < p ? -(long long)pos0 / l.QB : p) : 0;
     const long long base = pos0 + none * l.QB, rest = p - none;

@@ -110,6 +110,11 @@ static void test_far_lengths() {
                             if (end > 0)
                                 REQUIRE(tile == first / tk && (int64_t)(tile + (int64_t)n) * tk >= end && (int64_t)(tile + (int64_t)n - 1) * tk < end,
                                         "tiles %d + %d for keys %lld..%lld", tile, n, (long long)first, (long long)end);
+                            // a block costs its keys and a constant, and not more than the constant, a block and the keys
+                            const long long cost = line_prefix(l, h.b.window, h.b.causal, q.pos0, q.keys, p + 1) - line_prefix(l, h.b.window, h.b.causal, q.pos0, q.keys, p);
+                            REQUIRE(cost >= kLineOverhead + std::max<int64_t>(0, end - first) - l.QB &&
+                                        cost <= kLineOverhead + (int64_t)l.QB + kLineUnit + std::min<int64_t>(k, causal && window ? (int64_t)window : k),
+                                    "cost %lld of block %d (keys %d step %d window %d)", cost, p, k, step, window);
                         }
                     }
                 }
