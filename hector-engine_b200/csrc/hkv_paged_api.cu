@@ -281,15 +281,6 @@ const void* chunk_kernel(const hkv_paged_geometry& g) {
 }
 size_t chunk_part_bytes(const hkv_paged_geometry& g, int sm_count) { return 2ull * sm_count * partial_floats((wide(g) ? 1 : 2) * kCkRows, g.head_dim) * sizeof(float); }
 
-// The line's table counts units of 128 << shift keys; the shift keeps the largest batch the context allows inside 31 bits.
-int line_shift(const hkv_paged_geometry& g, int QB) {
-    const double keys = (double)g.max_pages * g.page_size + kLineOverhead + QB;
-    const double units = ((double)g.max_tokens / QB + g.max_requests) * g.num_kv_heads * (keys / kLineUnit + 1.0);
-    int shift = 0;
-    while (units / (double)(1ll << shift) > 1.0e9) ++shift;
-    return shift;
-}
-
 int launch_chunk(hkv_paged_ctx* c, const PagedAttnArgs& t, const void* q, int small, PagedFinishArgs& f, cudaStream_t st) {
     const hkv_paged_geometry& g = c->g;
     const int G = g.num_heads / g.num_kv_heads;
@@ -300,7 +291,7 @@ int launch_chunk(hkv_paged_ctx* c, const PagedAttnArgs& t, const void* q, int sm
     a.line.KVH = g.num_kv_heads;
     a.line.QB = block_queries(g);
     a.line.keys = wide(g) ? kWdKeys : kCkKeys;
-    a.line.shift = line_shift(g, a.line.QB);
+    a.line.shift = line_shift((double)g.max_pages * g.page_size, g.max_tokens, g.max_requests, g.num_kv_heads, a.line.QB);
     a.part = c->chunk_part;
     a.cuts = c->chunk_cuts;
     a.fix = fix_of(c);

@@ -60,7 +60,8 @@ __device__ __forceinline__ bool chunk_takes(const PagedChunkArgs& a, const Paged
     return q.n > 0 && !paged_is_small(q, a.line.G, a.small);
 }
 
-// Units before each request, over the block; returns the units of all. `pre` [requests + 1] in shared memory.
+// Units before each request, over the block; returns the units of all, 0 (and the status bit) where they do not fit.
+// `pre` [requests + 1] in shared memory.
 template <typename Args>
 __device__ __forceinline__ uint32_t chunk_line(const Args& a, uint32_t* pre, long long* buf) {
     const PagedBatch& b = a.t.b;
@@ -82,6 +83,10 @@ __device__ __forceinline__ uint32_t chunk_line(const Args& a, uint32_t* pre, lon
     }
     if (tid == 0) pre[R] = (uint32_t)all;
     __syncthreads();
+    if (!line_fits(all)) {
+        if (tid == 0) atomicOr(b.status, kStatusBoundCheck);
+        return 0;
+    }
     return (uint32_t)all;
 }
 

@@ -25,6 +25,18 @@ struct PagedLine {
     const uint32_t* pre;      // shared memory: [requests + 1] units before each request
 };
 
+// The table's shift for the largest batch a context allows (requests, tokens and positions per request): at most 10^9 units.
+inline int line_shift(double positions, double tokens, double requests, int KVH, int QB) {
+    const double units = (tokens / QB + requests) * KVH * ((positions + kLineOverhead + QB) / kLineUnit + 1.0);
+    int shift = 0;
+    while (units / (double)(1ll << shift) > 1.0e9) ++shift;
+    return shift;
+}
+// Whether a batch's units fit the table. They do where the requests' rows lie apart; arrays in which they overlap (starts
+// left at zero, say) can ask for thousands of times the context's tokens, and sums that wrapped would send the bisections
+// below to requests without work, whose cost of 0 no division ends on.
+__host__ __device__ inline bool line_fits(long long units) { return units >= 0 && units <= 0x7fffffffll; }
+
 struct LineCut { int r, kvh, p, t; };     // request, KV head, block of queries, key tile inside the item
 
 __host__ __device__ inline int line_blocks(int n, int QB) { return (n + QB - 1) / QB; }

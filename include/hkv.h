@@ -431,7 +431,9 @@ int hkv_paged_create(hkv_paged_ctx** out, const hkv_paged_geometry* geometry);
 int hkv_paged_destroy(hkv_paged_ctx* ctx);
 const char* hkv_paged_last_error(const hkv_paged_ctx* ctx);
 /* As hkv_ctx_device_status. Bit 2 is set by a block-table entry outside 0..num_pages-1 that attention
- * had to read (its rows count as zeros) or a slot >= num_pages*page_size (not stored). */
+ * had to read (its rows count as zeros), by a slot >= num_pages*page_size (not stored), or by requests
+ * whose rows overlap so often that the call is many times what the context was created for (their chunks
+ * are left out, their rows of `out` as they were). */
 int hkv_paged_device_status(hkv_paged_ctx* ctx, void* stream, int32_t* status_out);
 /* Bytes of device memory the context holds for attention. */
 size_t hkv_paged_workspace_bytes(const hkv_paged_ctx* ctx);

@@ -121,9 +121,60 @@ static void test_far_lengths() {
     passed("lengths up to 2^31 - 8");
 }
 
+// The table of one launch, as the kernels fill it in; returns the units of all in 64 bits.
+static long long fill(const PagedBatch& b, const PagedLine& l, int small, std::vector<uint32_t>& pre) {
+    pre.assign(b.requests + 1, 0);
+    long long at = 0;
+    for (int r = 0; r < b.requests; ++r) {
+        const PagedRequest q = paged_request(b, r);
+        pre[r] = (uint32_t)at;
+        at += q.n > 0 && !paged_is_small(q, l.G, small) ? line_units(b, l, q) : 0;
+    }
+    pre[b.requests] = (uint32_t)at;
+    return at;
+}
+
+// The units of the largest batches that contexts allow fit 31 bits; overlapping rows are told from them.
+static void test_units_fit() {
+    std::vector<uint32_t> pre;
+    for (int requests : {1, 7, 300, 4096})
+        for (int tokens : {1, 5000, 131072, 1 << 24})
+            for (int cols : {1, 8192, (int)((1ll << 31) / 16 - 1)})
+                for (int KVH : {1, 8, 128})
+                    for (int G : {1, 7, 16, 128})
+                        for (bool causal : {true, false}) {
+                            PagedLine l{};
+                            l.G = G; l.KVH = KVH; l.QB = 2 * (128 / G); l.keys = 128;
+                            l.shift = line_shift((double)cols * 16, tokens, requests, KVH, l.QB);
+                            // all tokens dealt evenly; all in the last request; one each and the rest in the first
+                            for (int deal = 0; deal < 3; ++deal) {
+                                std::vector<int32_t> start(requests), step(requests), len(requests, cols * 16);
+                                int at = 0;
+                                for (int r = 0; r < requests; ++r) {
+                                    step[r] = deal == 0 ? tokens / requests : deal == 1 ? (r + 1 == requests ? tokens : 0)
+                                            : r == 0 ? std::max(0, tokens - requests + 1) : (tokens >= requests ? 1 : 0);
+                                    start[r] = at;
+                                    at += step[r];
+                                }
+                                const Host h(start, step, len, cols, 16, tokens, tokens, 0, causal);
+                                const long long units = fill(h.b, l, 0, pre);
+                                REQUIRE(line_fits(units) && units <= 1100000000ll, "%lld units (%d requests, %d tokens, %d pages)", units, requests, tokens, cols);
+                            }
+                        }
+    // 4 096 requests that all start at row 0 and all have 16k tokens: beyond 32 bits, refused
+    PagedLine l{};
+    l.G = 4; l.KVH = 8; l.QB = 64; l.keys = 128;
+    l.shift = line_shift(131072.0, 16384, 4096, 8, 64);
+    const Host h(std::vector<int32_t>(4096, 0), std::vector<int32_t>(4096, 16384), std::vector<int32_t>(4096, 131072), 8192, 16, 16384, 16384, 0, true);
+    const long long units = fill(h.b, l, 0, pre);
+    REQUIRE(units > 0xffffffffll && !line_fits(units), "%lld units", units);
+    passed("units of the largest batches, and of overlapping ones");
+}
+
 int main() {
     test_tile_and_box_bounds();
     test_far_lengths();
+    test_units_fit();
     std::printf(g_failures ? "%d FAILED\n" : "ALL PASSED\n", g_failures);
     return g_failures ? 1 : 0;
 }

@@ -124,3 +124,28 @@ def test_broadcast_rows_are_refused(hkv, cuda):
     att(), cross(), rope(), paged()
     assert ctx.device_status() == 0
     ctx.close()
+
+
+# ---- arrays that no plan writes -------------------------------------------------------------------------------------------
+def test_overlapping_requests_beyond_the_work_table(hkv, cuda):
+    """4 096 requests that all claim the same 16 384 rows (starts left at zero): more work than the prompt kernel's table
+    counts. The call leaves the rows alone and sets bit 2; the next call of the context is right."""
+    torch = cuda
+    H, KVH, HD, page, R, T, cols = 32, 8, 64, 16, 4096, 16384, 8192
+    kc, vc = (torch.zeros(4, page, KVH, HD, dtype=torch.float16, device="cuda") for _ in range(2))
+    vc += 1
+    table = torch.zeros(R, cols, dtype=torch.int32, device="cuda")
+    q = torch.zeros(T, H, HD, dtype=torch.float16, device="cuda")
+    out = torch.full_like(q, 77.0)
+    ctx = hkv.PagedContext(hkv.PagedGeometry(num_heads=H, num_kv_heads=KVH, head_dim=HD, page_size=page, num_pages=4, max_requests=R,
+                                             max_pages=cols, max_tokens=T))
+    z = torch.zeros(R, dtype=torch.int32, device="cuda")
+    ctx.attention(q, kc, vc, out, table, z, z + T, z + cols * page)
+    assert ctx.device_status() == 2
+    assert (out == 77.0).all()
+    step = z.clone()
+    step[7] = 300
+    ctx.attention(q, kc, vc, out, table, z, step, step, max_step=300)
+    assert ctx.device_status() == 0
+    assert (out[:300] == 1.0).all() and (out[300:] == 77.0).all()
+    ctx.close()
