@@ -496,6 +496,9 @@ int hkv_paged_create(hkv_paged_ctx** out, const hkv_paged_geometry* geometry) {
         if ((e = cudaMemset(c->fix, 0, sizeof(int4) * (1 + kFixMax))) != cudaSuccess) return fail_cuda(c, e, "cudaMemset(list)");
         c->workspace_bytes += nb + sizeof(int4) * (2 * c->sm_count + 1 + kFixMax);
     }
+    // the memsets above went to the default stream, behind whatever is queued there; the first call may come on a stream
+    // that does not wait for it
+    if ((e = cudaStreamSynchronize(nullptr)) != cudaSuccess) return fail_cuda(c, e, "cudaStreamSynchronize(create)");
     c->ready = true;
     return HKV_OK;
 }
@@ -518,12 +521,17 @@ size_t hkv_paged_workspace_bytes(const hkv_paged_ctx* c) { return c ? c->workspa
 int hkv_paged_device_status(hkv_paged_ctx* c, void* stream, int32_t* status_out) {
     if (!c || !status_out) return HKV_ERR_INVALID_ARG;
     PAGED_CHECK(c);
-    cudaError_t e = cudaStreamSynchronize((cudaStream_t)stream);
+    // read and cleared on the caller's stream, and over when this returns: on the default stream the clearing could come
+    // after a kernel of a stream that does not wait for it, and take that kernel's bit
+    const cudaStream_t st = (cudaStream_t)stream;
+    cudaError_t e = cudaMemcpyAsync(status_out, c->d_status, sizeof(int32_t), cudaMemcpyDeviceToHost, st);
+    if (e != cudaSuccess) return fail_cuda(c, e, "cudaMemcpyAsync(status)");
+    e = cudaStreamSynchronize(st);
     if (e != cudaSuccess) return fail_cuda(c, e, "cudaStreamSynchronize");
-    e = cudaMemcpy(status_out, c->d_status, sizeof(int32_t), cudaMemcpyDeviceToHost);
-    if (e != cudaSuccess) return fail_cuda(c, e, "cudaMemcpy(status)");
     if (*status_out != 0) {
-        cudaMemset(c->d_status, 0, sizeof(int32_t));
+        e = cudaMemsetAsync(c->d_status, 0, sizeof(int32_t), st);
+        if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+        if (e != cudaSuccess) return fail_cuda(c, e, "cudaMemsetAsync(status)");
         return fail(c, HKV_ERR_DEVICE_FAULT, "device status word is non-zero");
     }
     return HKV_OK;

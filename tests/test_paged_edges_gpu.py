@@ -149,3 +149,34 @@ def test_overlapping_requests_beyond_the_work_table(hkv, cuda):
     assert ctx.device_status() == 0
     assert (out[:300] == 1.0).all() and (out[300:] == 77.0).all()
     ctx.close()
+
+
+# ---- streams ----------------------------------------------------------------------------------------------------------------
+def test_a_context_is_ready_for_any_stream(hkv, cuda):
+    """A context created (and its status read) while the default stream is busy, used at once on a stream that does not wait
+    for the default one: its words were cleared before, so the bit that the first call sets is still there."""
+    torch = cuda
+    g = hkv.PagedGeometry(num_heads=2, head_dim=64, page_size=16, num_pages=4, max_requests=1, max_pages=4, max_tokens=4)
+    hkv.PagedContext(g).close()                          # (modules loaded)
+    k = torch.zeros(4, 2, 64, dtype=torch.float16, device="cuda")
+    kc, vc = (torch.zeros(4, 16, 2, 64, dtype=torch.float16, device="cuda") for _ in range(2))
+    bad = torch.full((4,), 64, dtype=torch.int32, device="cuda")
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(200_000_000)                       # a tenth of a second
+    ctx = hkv.PagedContext(g)
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            ctx.append(k, k, kc, vc, bad)                # a slot behind the planes
+            assert ctx.device_status() == 2
+        assert ctx.device_status() == 0
+    torch.cuda._sleep(200_000_000)
+    with torch.cuda.stream(side):
+        ctx.append(k, k, kc, vc, bad)
+    assert ctx.device_status(side) == 2                  # not the current stream
+    with torch.cuda.stream(side):
+        ctx.append(k, k, kc, vc, bad)
+        side.synchronize()
+        assert ctx.device_status() == 2
+    torch.cuda.synchronize()
+    ctx.close()
