@@ -507,7 +507,16 @@ __global__ void __launch_bounds__(kPagedGenWarps * 32) hkv_paged_generic_kernel(
         const int mid = (lo + hi + 1) >> 1;
         if (a.b.q_start[mid] <= t) lo = mid; else hi = mid - 1;
     }
-    const PagedRequest rq = paged_request(a.b, lo);
+    PagedRequest rq = paged_request(a.b, lo);
+    // An empty request may start on or inside the rows of one before it: the nearest that has rows, 32 at a time, as far
+    // back as max_step rows reach.
+    while (rq.n == 0) {
+        if (lo == 0 || (long long)a.b.q_start[lo - 1] + a.b.max_step <= t) return;
+        const int r = lo - 1 - (int)(threadIdx.x & 31);
+        const unsigned some = __ballot_sync(0xffffffffu, r >= 0 && paged_request(a.b, r).n > 0);
+        lo = some ? lo - __ffs(some) : (lo > 32 ? lo - 32 : 0);
+        rq = paged_request(a.b, lo);
+    }
     const int i = t - rq.start;
     if (i < 0 || i >= rq.n) return;                  // a row of no query
     paged_row<T, kPagedGenWarps>(a, lo, rq, i, blockIdx.y);

@@ -392,6 +392,7 @@ int32_t hkv_preferred_prefill_chunk(const hkv_geometry* geometry, int32_t sm_cou
  *   block table    [max_requests][max_pages] int32, entries 0 .. num_pages-1, -1 = not assigned
  *   packed batch   the new tokens of all requests back to back: request r owns the rows
  *                  q_start[r] .. q_start[r] + step_len[r] - 1 of q, k_new, v_new, out; q_start ascends
+ *                  (an empty request may start anywhere in that order; rows of two requests do not overlap)
  *   slot           page * page_size + row; -1 = the token is not stored
  *
  * One step of a serving loop: hkv_paged_plan (block tables and slot maps from the request lengths),

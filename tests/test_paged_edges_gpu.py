@@ -180,3 +180,28 @@ def test_a_context_is_ready_for_any_stream(hkv, cuda):
         assert ctx.device_status() == 2
     torch.cuda.synchronize()
     ctx.close()
+
+
+# ---- starts that only ascend --------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kernel", [0, 1], ids=["staged", "generic"])
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "cross"])
+def test_empty_requests_may_start_anywhere_in_order(hkv, cuda, kernel, causal):
+    """q_start ascends, and an empty request's start may lie on or inside the rows of the one before it; gaps and padded rows
+    belong to nobody."""
+    torch = cuda
+    H, KVH, HD, page = 8, 2, 64, 16
+    starts, steps, keys = [0, 0, 2, 4, 9, 9, 9, 50, 50] + [50] * 40, [4, 0, 0, 3, 40, 0, 0, 0, 1] + [0] * 40, [9, 3, 0, 30, 77, 5, 0, 8, 20] + [1] * 40
+    gen = torch.Generator().manual_seed(19)
+    kc, vc, table = P.make_pages(torch, gen, keys, page, 70, 6, KVH, HD, torch.float16)
+    T = 60
+    q = torch.randn(T, H, HD, generator=gen).half().cuda()
+    out = torch.full_like(q, 77.0)
+    ctx = hkv.PagedContext(hkv.PagedGeometry(num_heads=H, num_kv_heads=KVH, head_dim=HD, page_size=page, num_pages=70,
+                                             max_requests=len(keys), max_pages=6, max_tokens=T, kernel_select=kernel))
+    call = ctx.attention if causal else ctx.cross_attention
+    call(q, kc, vc, out, table, i32(torch, starts), i32(torch, steps), i32(torch, keys), max_step=40)
+    ref, tol, live = P.attend_model(torch, q, kc, vc, table, starts, steps, keys, ctx.geometry.default_scale, page, 0, causal)
+    assert int(live.sum()) == sum(steps) and (out[~live] == 77.0).all()
+    assert ((out.double() - ref).abs() <= tol)[live].all()
+    assert ctx.device_status() == 0
+    ctx.close()
