@@ -1,8 +1,12 @@
 // hkv_paged_schedule_tests.cu — the host-callable arithmetic behind the paged attention kernels' schedules, run on the CPU
-// (no device call): which keys a query sees, which tiles a request has, at lengths up to the end of 31 bits.
+// (no device call): which keys a query sees, which tiles a request has, at lengths up to the end of 31 bits; how a ragged batch is cut into spans.
 #include <algorithm>
+#include <array>
 #include <cstdint>
 #include <cstdio>
+#include <map>
+#include <random>
+#include <set>
 #include <vector>
 
 #include "hkv_paged_decode.cuh"
@@ -171,10 +175,105 @@ static void test_units_fit() {
     passed("units of the largest batches, and of overlapping ones");
 }
 
+// Random ragged batches cut into spans: every key tile of every item is in exactly one piece, a piece that is not a whole
+// item lies in the workspace slot that the finishing kernel's entry for the item points at, and no slot is used twice.
+static void test_spans() {
+    std::mt19937 rng(31);
+    auto pick = [&](int lo, int hi) { return (int)(lo + rng() % (unsigned)(hi - lo + 1)); };
+    std::vector<uint32_t> pre;
+    long long batches = 0, pieces = 0, cut_items = 0;
+    for (int round = 0; round < 1500; ++round) {
+        const int R = round % 5 == 0 ? pick(1, 3) : pick(1, 60), page = 1 << pick(3, 8);
+        const bool causal = rng() % 3 != 0, wide = rng() % 2;
+        const int G = std::vector<int>{1, 2, 3, 7, 8, 16, 40, 128}[rng() % 8], KVH = pick(1, 9);
+        const int window = rng() % 2 ? 0 : pick(1, 2000), most = std::vector<int>{1, 20, 600, 5000}[rng() % 4];
+        std::vector<int32_t> start(R), step(R), len(R);
+        int at = 0, longest = 1;
+        for (int r = 0; r < R; ++r) {
+            step[r] = rng() % 6 == 0 ? 0 : pick(1, most);
+            len[r] = rng() % 8 == 0 ? pick(0, 50) : step[r] + pick(0, rng() % 3 ? 3000 : 60000);
+            start[r] = at;
+            at += step[r];
+            longest = std::max(longest, (int)len[r]);
+        }
+        const Host h(start, step, len, (longest + page - 1) / page, page, std::max(at, 1), most, window, causal);
+        PagedLine l{};
+        l.G = G; l.KVH = KVH; l.QB = (wide ? 1 : 2) * (128 / G); l.keys = wide ? 64 : 128;
+        l.shift = line_shift((double)h.b.cols * page, h.b.tokens, R, KVH, l.QB);
+        const int small = rng() % 2 ? 0 : G <= 8 ? 8 / G * G : G;
+        const uint32_t W = (uint32_t)fill(h.b, l, small, pre);
+        l.pre = pre.data();
+        const int grid = std::vector<int>{148, 148, 148, 7, 1}[rng() % 5], ctas = line_ctas(W, grid);
+        struct Piece { int cta, t0, t1, slot; };
+        std::map<std::array<int, 3>, std::vector<Piece>> items;
+        std::vector<LineCut> cut(ctas + 1);
+        for (int c = 0; c <= ctas; ++c) cut[c] = line_locate(h.b, l, line_boundary(W, ctas, c), W);
+        for (int cta = 0; cta < ctas && W > 0; ++cta) {          // as the producers walk
+            LineCut c = cut[cta];
+            const LineCut e = cut[cta + 1];
+            while (c.r < R && line_before(c, e)) {
+                if (pre[c.r + 1] == pre[c.r]) { ++c.r; c.kvh = c.p = c.t = 0; continue; }
+                const PagedRequest q = paged_request(h.b, c.r);
+                int kt0, nt;
+                line_tiles(h.b, l, q, c.p, kt0, nt);
+                const int end = line_same_item(c, e) ? e.t : nt;
+                if (end > c.t) items[{c.r, c.kvh, c.p}].push_back({cta, c.t, end, c.t == 0 && end == nt ? -1 : 2 * cta + (c.t == 0 ? 1 : 0)});
+                c.t = 0;
+                if (++c.p >= line_blocks(q.n, l.QB)) {
+                    c.p = 0;
+                    if (++c.kvh == l.KVH) { c.kvh = 0; ++c.r; }
+                }
+            }
+        }
+        std::map<std::array<int, 3>, std::pair<int, int>> entries;   // item -> first CTA, parts (as the entries are written)
+        for (int cta = 0; cta < ctas; ++cta) {
+            const LineCut c0 = cut[cta], c1 = cut[cta + 1];
+            if (c1.r >= R || c1.t == 0 || (line_same_item(c0, c1) && c0.t > 0)) continue;
+            int parts = 2;
+            for (int c = cta + 2; c < ctas && line_same_item(cut[c], c1) && cut[c].t > 0; ++c) ++parts;
+            entries[{c1.r, c1.kvh, c1.p}] = {cta, parts};
+        }
+        std::set<int> slots;
+        size_t expected = 0;
+        for (int r = 0; r < R; ++r) {
+            const PagedRequest q = paged_request(h.b, r);
+            if (q.n == 0 || paged_is_small(q, G, small)) continue;
+            for (int kvh = 0; kvh < KVH; ++kvh)
+                for (int p = 0; p < line_blocks(q.n, l.QB); ++p, ++expected) {
+                    int kt0, nt, t = 0;
+                    line_tiles(h.b, l, q, p, kt0, nt);
+                    const auto it = items.find({r, kvh, p});
+                    REQUIRE(it != items.end(), "item %d %d %d has no piece", r, kvh, p);
+                    if (it == items.end()) continue;
+                    const auto en = entries.find({r, kvh, p});
+                    for (size_t i = 0; i < it->second.size(); ++i) {
+                        const Piece& x = it->second[i];
+                        REQUIRE(x.t0 == t, "item %d %d %d: tile %d after %d", r, kvh, p, x.t0, t);
+                        t = x.t1;
+                        if (it->second.size() == 1) REQUIRE(x.slot == -1 && en == entries.end(), "a whole item with a slot or an entry");
+                        else REQUIRE(en != entries.end() && x.cta == en->second.first + (int)i && x.slot == 2 * x.cta + (i == 0) && slots.insert(x.slot).second,
+                                     "item %d %d %d: piece %d in CTA %d, slot %d", r, kvh, p, (int)i, x.cta, x.slot);
+                        ++pieces;
+                    }
+                    REQUIRE(t == nt, "item %d %d %d: %d of %d tiles", r, kvh, p, t, nt);
+                    if (en != entries.end()) {
+                        REQUIRE(en->second.second == (int)it->second.size(), "item %d %d %d: %d parts of %d", r, kvh, p, en->second.second, (int)it->second.size());
+                        ++cut_items;
+                    }
+                }
+        }
+        REQUIRE(items.size() == expected, "%d items of %d", (int)items.size(), (int)expected);
+        ++batches;
+    }
+    REQUIRE(batches == 1500 && pieces > 40000 && cut_items > 4000, "%lld pieces, %lld cut items", pieces, cut_items);
+    passed("spans of random batches");
+}
+
 int main() {
     test_tile_and_box_bounds();
     test_far_lengths();
     test_units_fit();
+    test_spans();
     std::printf(g_failures ? "%d FAILED\n" : "ALL PASSED\n", g_failures);
     return g_failures ? 1 : 0;
 }

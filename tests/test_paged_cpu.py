@@ -93,4 +93,4 @@ def test_schedule_arithmetic():
     binary = importlib.import_module("hector-engine_b200.build").build_schedule_tests()
     res = subprocess.run([binary], capture_output=True, text=True, timeout=300)
     assert res.returncode == 0, res.stdout + res.stderr
-    assert res.stdout.count("PASS:") == 3 and "ALL PASSED" in res.stdout
+    assert res.stdout.count("PASS:") == 4 and "ALL PASSED" in res.stdout

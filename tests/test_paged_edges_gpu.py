@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 
 import _paged as P
+import test_paged_gpu as base
 
 pytestmark = pytest.mark.gpu
 
@@ -205,3 +206,80 @@ def test_empty_requests_may_start_anywhere_in_order(hkv, cuda, kernel, causal):
     assert ((out.double() - ref).abs() <= tol)[live].all()
     assert ctx.device_status() == 0
     ctx.close()
+
+
+# ---- one rounding, every pass ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("case", base.ROPES, ids=lambda c: f"T{c[0]}h{c[1]}x{c[3]}r{c[4]}a{c[5]}")
+def test_norm_rope_rounds_once(hkv, cuda, case, dtype):
+    """The result is rounded to the type once: half a step of the RESULT, beside the 24 roundings of 32 bits that
+    test_paged_gpu.rope_tolerance counts, of the products' size (a second rounding, of the normalised row, would be half a
+    step of the operands) — 25 with the half step of that error itself. 2^-25: half a step of fp16 below 2^-14."""
+    torch = cuda
+    T, H, KVH, HD, rot, axes, sections, inter, norm = case
+    D, page = dt(torch, dtype), 16
+    num_pages = -(-T // page) + 2
+    gen = torch.Generator().manual_seed(T * HD + rot + 1)
+    q, k, v = (torch.randn(T, h, HD, generator=gen).to(D).cuda() for h in (H, KVH, KVH))
+    pos = torch.randint(-3, 1_000_000, (axes, T), generator=gen, dtype=torch.int32).cuda()
+    qw, kw = ((1 + 0.2 * torch.randn(HD, generator=gen)).to(D).cuda() for _ in range(2))
+    kc, vc = (torch.zeros(num_pages, page, KVH, HD, dtype=D, device="cuda") for _ in range(2))
+    slots = torch.randperm(num_pages * page, generator=gen)[:T].to(torch.int32).cuda()
+    q_out = torch.empty_like(q)
+    ctx = hkv.PagedContext(hkv.PagedGeometry(num_heads=H, num_kv_heads=KVH, head_dim=HD, page_size=page, num_pages=num_pages,
+                                             max_requests=1, max_pages=1, max_tokens=T, dtype=dtype, flags=hkv.FLAG_APPEND_ONLY))
+    ctx.norm_rope(q, k, v, pos, slots=slots, k_cache=kc, v_cache=vc, q_out=q_out, sections=sections, interleaved=inter, rotary_dim=rot,
+                  eps=1e-6, theta=1e6, scaling_factor=2.5, **(dict(q_norm_w=qw, k_norm_w=kw) if norm else {}))
+    for x, w, got in ((q, qw, q_out), (k, kw, kc.view(-1, KVH, HD)[slots.long()])):
+        ref, size = P.rope_model(torch, x, pos, w if norm else None, rot, axes, sections, inter, 1e-6, 1e6, 2.5)
+        off = (got.double() - ref).abs() - (P.unit(torch, D) * ref.abs() + 25 * 2.0 ** -24 * size + 2.0 ** -25)
+        assert off.max() <= 0, f"{off.max().item():.3e} over"
+    assert ctx.device_status() == 0
+    ctx.close()
+
+
+@pytest.mark.parametrize("heads", [(16, 8, 256), (28, 4, 128), (14, 2, 64)], ids=str)
+def test_every_pass_of_both_contexts_gives_the_same_bits(hkv, cuda, heads):
+    """Hundreds of passes over a ragged windowed batch, from two contexts in turn: each of them is compared."""
+    torch = cuda
+    H, KVH, HD = heads
+    gen = torch.Generator().manual_seed(23)
+    page, steps = 32, [1, 1, 400, 1, 1, 1, 1, 250] * 4
+    keys = [int(x) for x in torch.randint(2000, 6000, (len(steps),), generator=gen)]
+    cols = max(-(-k // page) for k in keys)
+    num_pages = sum(-(-k // page) for k in keys)
+    kc, vc, table = P.make_pages(torch, gen, keys, page, num_pages, cols, KVH, HD, torch.float16)
+    T = sum(steps)
+    q = torch.randn(T, H, HD, generator=gen).half().cuda()
+    args = (table, i32(torch, np.concatenate([[0], np.cumsum(steps)])), i32(torch, steps), i32(torch, keys))
+    ctxs = [hkv.PagedContext(hkv.PagedGeometry(num_heads=H, num_kv_heads=KVH, head_dim=HD, page_size=page, num_pages=num_pages,
+                                               max_requests=len(steps), max_pages=cols, max_tokens=T, window_size=1024)) for _ in range(2)]
+    first, out = torch.empty_like(q), torch.empty_like(q)
+    ctxs[0].attention(q, kc, vc, first, *args, max_step=400)
+    differ = torch.zeros(2, dtype=torch.int64, device="cuda")
+    for it in range(300):
+        out.fill_(55.0)
+        ctxs[it % 2].attention(q, kc, vc, out, *args, max_step=400)
+        differ[it % 2] += (out != first).sum()
+    assert [c.device_status() for c in ctxs] == [0, 0]
+    assert differ.tolist() == [0, 0]
+    for c in ctxs:
+        c.close()
+
+
+# ---- the largest batches and groups -----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("heads", [(128, 1, 64), (65, 1, 128), (254, 2, 96), (100, 1, 256), (128, 1, 256)], ids=str)
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "cross"])
+def test_large_groups(hkv, cuda, heads, causal):
+    """Groups up to the 128 that one query tile holds: one or two queries per item, all of them chunks."""
+    base.run_attention(hkv, cuda, heads=heads, page=16, steps=[1, 7, 0, 40], keys=[300, 7, 20, 555], causal=causal, dtype="bfloat16")
+    base.run_attention(hkv, cuda, heads=heads, page=64, steps=[1, 1], keys=[64, 2100], causal=causal)
+
+
+@pytest.mark.parametrize("heads", [(28, 4, 128), (4, 2, 256), (8, 8, 64), (6, 2, 80)], ids=str)
+def test_4096_requests(hkv, cuda, heads):
+    """The largest batch a context takes: tokens and chunks of a few rows, short requests, empty ones among them."""
+    rng = np.random.default_rng(29)
+    steps = rng.choice([0, 1, 1, 1, 2, 9], 4096)
+    keys = np.maximum(steps, rng.integers(1, 90, 4096))
+    base.run_attention(hkv, cuda, heads=heads, page=16, steps=[int(n) for n in steps], keys=[int(k) for k in keys])
