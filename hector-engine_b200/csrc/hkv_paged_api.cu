@@ -405,6 +405,8 @@ int attention(hkv_paged_ctx* c, const void* q, int64_t q_token_stride, const voi
         return fail(c, HKV_ERR_ALIGNMENT, "attention: the staged kernels need 16-byte aligned tensors and strides");
     const bool only_small = (long long)max_step * G <= kSmallCols;
     // (the prompt kernel takes the row maximum before the scale, which it can for a positive one)
+    if (!only_small && !(scale > 0.0f) && g.kernel_select == HKV_KERNEL_TMA)
+        return fail(c, HKV_ERR_GEOMETRY, "attention: the staged kernels take chunks with a positive scale only");
     if (staged && (only_small || scale > 0.0f)) {
         // Query rows per KV head of the few-token kernel: all that the call can have, or, beside the prompt kernel, as many
         // tokens as fit one n8 tile (16 rows where a single token has more than 8): with two tiles every request of the

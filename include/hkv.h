@@ -418,7 +418,8 @@ typedef struct hkv_paged_geometry {
     int32_t max_tokens;   /* upper bound of a call's packed tokens                               */
     int32_t window_size;  /* 0 = attend everything; W = the last W positions                     */
     int32_t kernel_select;/* hkv_kernel_select: AUTO, or GENERIC to force the any-geometry kernel,
-                             or TMA to require the staged kernels (HKV_ERR_GEOMETRY otherwise)   */
+                             or TMA to require the staged kernels (HKV_ERR_GEOMETRY otherwise: on
+                             creation, or by a call of chunks whose scale is not positive)       */
     int32_t flags;        /* HKV_FLAG_APPEND_ONLY: no attention workspace                        */
     int32_t reserved[4];
 } hkv_paged_geometry;

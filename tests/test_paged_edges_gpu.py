@@ -283,3 +283,17 @@ def test_4096_requests(hkv, cuda, heads):
     steps = rng.choice([0, 1, 1, 1, 2, 9], 4096)
     keys = np.maximum(steps, rng.integers(1, 90, 4096))
     base.run_attention(hkv, cuda, heads=heads, page=16, steps=[int(n) for n in steps], keys=[int(k) for k in keys])
+
+
+def test_staged_kernels_required(hkv, cuda):
+    """A context that requires the staged kernels never takes the any-geometry kernel instead: chunks with a scale that is not
+    positive are refused, single tokens and AUTO contexts answer."""
+    torch = cuda
+    steps, keys = [40, 3], [90, 70]
+    for heads in ((8, 2, 64), (4, 2, 256)):
+        base.run_attention(hkv, torch, heads=heads, page=16, steps=[1, 1], keys=keys, scale=-0.1, kernel=2)
+        base.run_attention(hkv, torch, heads=heads, page=16, steps=steps, keys=keys, scale=-0.1)
+        for scale in (-0.1, 0.0):
+            with pytest.raises(hkv.HkvError) as e:
+                base.run_attention(hkv, torch, heads=heads, page=16, steps=steps, keys=keys, scale=scale, kernel=2)
+            assert e.value.status == 2, e.value
