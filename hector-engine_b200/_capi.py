@@ -65,7 +65,7 @@ class HkvPagedRope(C.Structure):
         (n, C.c_int64) for n in ("q_token_stride", "kv_token_stride", "q_out_token_stride", "k_out_token_stride",
                                  "position_axis_stride")] + [
         ("tokens", C.c_int32), ("rotary_dim", C.c_int32), ("axes", C.c_int32), ("sections", C.c_int32 * ROPE_MAX_AXES),
-        ("interleaved", C.c_int32), ("eps", C.c_float), ("scaling_factor", C.c_float), ("theta", C.c_double),
+        ("interleaved", C.c_int32), ("eps", C.c_float), ("scaling_factor", C.c_double), ("theta", C.c_double),
     ]
 
 

@@ -697,7 +697,7 @@ int hkv_paged_norm_rope(hkv_paged_ctx* c, const hkv_paged_rope* r, void* stream)
     a.rows = (long long)g.num_pages * g.page_size;
     a.tokens = r->tokens; a.H = g.num_heads; a.KVH = g.num_kv_heads; a.HD = g.head_dim; a.rot = rot;
     a.eps = r->eps;
-    const double scaling = r->scaling_factor > 0.0f ? (double)r->scaling_factor : 1.0;
+    const double scaling = r->scaling_factor > 0.0 ? r->scaling_factor : 1.0;
     for (int i = 0; i < half; ++i) a.turns[i] = std::pow(r->theta, -2.0 * i / rot) / (scaling * 6.283185307179586476925);
     // 16-byte pieces whose pair partner is a whole piece away; everything else goes element by element
     bool pieces = g.head_dim % 16 == 0 && rot % 16 == 0 && a.q_stride % 8 == 0 && a.kv_stride % 8 == 0 && a.qo_stride % 8 == 0 &&

@@ -503,7 +503,8 @@ typedef struct hkv_paged_rope {
     int32_t axes;                       /* 1..HKV_ROPE_MAX_AXES; 0 = 1                            */
     int32_t sections[HKV_ROPE_MAX_AXES];
     int32_t interleaved;                /* 0 = blocks, 1 = interleaved                            */
-    float eps, scaling_factor;          /* scaling_factor <= 0 means 1                            */
+    float eps;
+    double scaling_factor;              /* <= 0 means 1                                           */
     double theta;
 } hkv_paged_rope;
 int hkv_paged_norm_rope(hkv_paged_ctx* ctx, const hkv_paged_rope* args, void* stream);

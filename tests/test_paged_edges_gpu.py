@@ -297,3 +297,26 @@ def test_staged_kernels_required(hkv, cuda):
             with pytest.raises(hkv.HkvError) as e:
                 base.run_attention(hkv, torch, heads=heads, page=16, steps=steps, keys=keys, scale=scale, kernel=2)
             assert e.value.status == 2, e.value
+
+
+# ---- scaling factors that 32 bits do not hold -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("scaling", [1.1, 0.3, 3.7])
+def test_far_positions_with_any_scaling_factor(hkv, cuda, scaling, dtype):
+    """Positions of a million over a factor that is no 32-bit number: rounding it alone would turn the first pairs by a
+    hundredth of a radian. Tolerance as in test_norm_rope_rounds_once, without a norm."""
+    torch = cuda
+    T, H, KVH, HD = 70, 4, 2, 128
+    D = dt(torch, dtype)
+    gen = torch.Generator().manual_seed(37)
+    q, k = (torch.randn(T, h, HD, generator=gen).to(D).cuda() for h in (H, KVH))
+    pos = torch.randint(900_000, 1_000_000, (1, T), generator=gen, dtype=torch.int32).cuda()
+    q_out, k_out = torch.empty_like(q), torch.empty_like(k)
+    ctx = hkv.PagedContext(hkv.PagedGeometry(num_heads=H, num_kv_heads=KVH, head_dim=HD, page_size=16, num_pages=1, max_requests=1,
+                                             max_pages=1, max_tokens=T, dtype=dtype, flags=hkv.FLAG_APPEND_ONLY))
+    ctx.norm_rope(q, k, None, pos, q_out=q_out, k_out=k_out, theta=1e4, scaling_factor=scaling)
+    for x, got in ((q, q_out), (k, k_out)):
+        ref, size = P.rope_model(torch, x, pos, None, HD, 1, None, False, 1e-6, 1e4, scaling)
+        off = (got.double() - ref).abs() - (P.unit(torch, D) * ref.abs() + 25 * 2.0 ** -24 * size + 2.0 ** -25)
+        assert off.max() <= 0, f"{off.max().item():.3e} over"
+    ctx.close()
