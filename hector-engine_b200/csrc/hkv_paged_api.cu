@@ -187,7 +187,11 @@ DecodeKernel pick_decode(int dtype, int hd, int nt, int groups) {
     return dtype == HKV_DTYPE_F16 ? pick_decode_t<__half>(hd, nt, groups) : pick_decode_t<__nv_bfloat16>(hd, nt, groups);
 }
 
-// CTAs that share a span: one per KV head, or two, four, eight heads per CTA where that leaves fewer CTAs idle.
+// CTAs that share a span: one per KV head, or two, four, eight heads per CTA where that leaves fewer CTAs idle. Up to 6 %
+// idle CTAs are taken rather than more heads one after the other, each with its own first copies and merge. (4 requests of
+// 4k keys, this rule / one head per CTA wherever they fit / the fewest idle: 64 heads of 64 49.6 / 50.9 / 55.1 us, 32 heads of 256
+// 94 / 87 / 111, 40 heads of 128 57 / 57 / 71, 12 heads of 64 14.4 / 14.4 / 15.5; 32 such requests: 64 heads of 64 334 / 348 / 346,
+// 40 of 128 387 / 390 / 406, 32 of 256 633 / 637 / 640.)
 int gang_for(int kv_heads, int grid) {
     int best = 1;
     double best_util = 0.0;
@@ -210,7 +214,10 @@ size_t part_bytes(const hkv_paged_geometry& g, int sm_count) {
 
 // Shape of the few-token kernel: two CTAs per SM with one consumer group each, or one CTA with two groups. Two stream a
 // little faster and hide each other's merges; they also double the spans, and with them the parts a request is cut into,
-// which is what a launch of one or two requests spends its time on.
+// which is what a launch of one or two requests spends its time on: one CTA where a request would be cut into more than 40.
+// (us, two CTAs / one: 1 request of 512 keys, 2 KV heads of 64 9.1 / 8.0, of 64k keys 17.4 / 18.6; 4 KV heads of 128 10.4 / 9.6
+// and 32.3 / 32.6. 4 requests of 512 9.5 / 8.5 and 11.6 / 10.5, of 64k keys 33.6 / 46.3 and 90 / 95; 16 requests of 64k keys 96 / 157 and
+// 315 / 340.)
 struct DecodeShape { int groups, grid, gang; PagedDecodePlan plan; };
 DecodeShape decode_shape(const hkv_paged_ctx* c, int cols, int requests) {
     const hkv_paged_geometry& g = c->g;
@@ -411,8 +418,9 @@ int attention(hkv_paged_ctx* c, const void* q, int64_t q_token_stride, const voi
         // Query rows per KV head of the few-token kernel: all that the call can have, or, beside the prompt kernel, as many
         // tokens as fit one n8 tile (16 rows where a single token has more than 8): with two tiles every request of the
         // launch pays for the registers (head_dim 256: one consumer group instead of two). A call whose requests have 64
-        // tokens or more on average leaves it out: single tokens among such prompts cost the prompt kernel a fraction of
-        // them, an empty launch costs 6 us.
+        // tokens or more on average leaves it out. (us, without / with, 28 heads of 4, 128 wide: 8 x 448 queries over 4k keys
+        // 206 / 212, 2 048 over 32k keys 741 / 794; a prompt of 4 096 beside 63 single tokens over 512 keys each 195 / 217, over 4k
+        // keys 299 / 287, over 32k keys 1 120 / 790 — there it loses, but the lengths that would tell are on the device.)
         const int small = only_small ? max_step * G : tokens / 64 >= requests ? 0 : G <= 8 ? 8 / G * G : G <= kSmallCols ? G : 0;
         PagedFinishArgs f{};
         f.t = a;

@@ -17,11 +17,11 @@
 //     its reference by 2^8. (Two threads per row halve nothing: the softmax is bound by its instructions, the exchange and
 //     the doubled bookkeeping cost a tenth.) P is rounded to the element type (its sum is not). In fp16 1 of
 //     8 pairs take a polynomial on the FMA pipe instead of ex2, the narrowest unit; bf16 takes none (kCkEmuOf8).
-//   * Measured (B200, one launch and the finishing one): 2 048 queries over 32k keys, 28 heads of 4, 128 wide: 727 us alone
-//     (1 282 TFLOP/s), 820 us back to back under the power limit; 8 x 448 queries over 2k to 4k keys 150 us. A pair of query
-//     tiles takes 2.0 us per 128 keys against 1.5 us of products at the library's rate. A call costs 10 us until its first
-//     scores are there, an item 2 us of output; a tile on the diagonal takes 3.8 us. A rehearsal of the tile code in front
-//     of the first tile, to warm the instruction caches, made every tile 7 % slower.
+//   * Measured (B200, one launch and the finishing one): 2 048 queries over 32k keys, 28 heads of 4, 128 wide, bf16: 716 us
+//     at full clocks (1 302 TFLOP/s), 785 to 850 us back to back under the power limit; 8 x 224 to 448 queries over 2k to 4k
+//     keys, fp16: 147 us. A pair of query tiles takes 2.0 us per 128 keys against 1.5 us of products at the library's rate.
+//     A call costs 10 us until its first scores are there, an item 2 us of output; a tile on the diagonal takes 3.8 us. A
+//     rehearsal of the tile code in front of the first tile, to warm the instruction caches, made every tile 7 % slower.
 //   * Every wait is bounded and reports through the status word; tensor memory is freed on every path.
 #pragma once
 
@@ -38,8 +38,8 @@ constexpr int kCkStages = 2;              // K tiles and V tiles in flight
 constexpr int kCkThreads = 384;
 // Pairs of every 8 whose exp2 runs on the FMA pipe, fp16 only. The polynomial ends at 2^-100, for a hidden key too: fp16
 // rounds that to zero, but bf16 carries it to the second product, where 2^-100 times a large hidden value is not nothing.
-// (2 048 queries over 32k keys, with and without in turn: head_dim 128 713 to 739 us against 721 to 747; head_dim 64 330
-// against 319. 8 x 448 queries over 4k keys 145 against 147. 2 and 3 of 8: 10 and 16 % slower than 1.)
+// (2 048 queries over 32k keys, with and without in turn, best of replays: head_dim 128 bf16 713 and 721 us, fp16 739 and
+// 747; head_dim 64 bf16 329 and 318. 8 x 224 to 448 queries over 4k keys 145 and 147. 2 and 3 of 8: 10 and 16 % slower than 1.)
 constexpr int kCkEmuOf8 = 1;
 constexpr int kCkDesc = 16;               // words of a work descriptor
 

@@ -12,12 +12,13 @@
 //   * Four consumer warps per tile, 16 rows each:  S^T = K Q^T  and  O^T += V^T P^T  with mma.m16n8k16, the query rows in
 //     N (8 or 16), K and V by ldmatrix, P^T from the score fragment by movmatrix; softmax over rows by shuffles, with a
 //     running maximum and sum in 32 bits. P is rounded to the element type for the second product (its sum is not), the
-//     usual choice: it keeps the product on the tensor cores and costs half a step of the type.
+//     usual choice: it keeps the product on the tensor cores and costs half a step of the type (against 64 bits 2.4e-4 to
+//     2.9e-4 of a row in fp16 where its rounding alone is 2.0e-4, 2.1e-3 to 2.3e-3 against 1.6e-3 in bf16).
 //   * A request inside one span is finished here. One that is cut leaves a partial row (o, maximum, sum) per span; a span
 //     has at most two (its first and its last request), so the workspace does not grow with the batch. The
 //     finishing kernel joins them.
-//   * Measured: 64 requests of 16k to 32k keys, 28 heads of 4, 128 wide, 16-row pages: 476 us (6.9 TB/s); 60 windows of
-//     1 024 keys, 8 KV heads 256 wide: 88 us (5.7 TB/s); 32 requests of 1 500 keys, 16 heads 64 wide: 34 us (4.3 TB/s), of
+//   * Measured: 64 requests of 16k to 32k keys, 28 heads of 4, 128 wide, 16-row pages: 470 us (7.0 TB/s); 60 windows of
+//     1 024 keys, 8 KV heads 256 wide: 88 us (5.7 TB/s); 32 requests of 1 500 keys, 16 heads 64 wide: 33 us (4.4 TB/s), of
 //     which 8 us are the two launches. With a copy per column block 8-row pages took 222 us where 64-row pages took 171,
 //     now 182 us: a copy costs some 50 ns whatever it brings.
 #pragma once

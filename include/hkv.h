@@ -516,7 +516,14 @@ int hkv_paged_norm_rope(hkv_paged_ctx* ctx, const hkv_paged_rope* args, void* st
  * and apart from q.
  * Rows of `out` that belong to no query are left as they were; a query that attends nothing gets zeros.
  * max_step: upper bound of step_len (queries beyond it are left out); with max_step * H / KVH <= 16 only
- * the single-token kernel is launched. */
+ * the single-token kernel is launched.
+ * Precision: scores, running maximum and sum, and partial rows are in 32 bits. The staged kernels round
+ * each probability to the element type before it meets V (the sum is of unrounded ones) and take the
+ * hardware's exp2 (fp16 prompts of head_dim <= 128: for one pair in eight a polynomial, 7.5e-5), so a row
+ * is off by 1.2 to 1.4 times what rounding it once costs: 2.9e-4 of its norm in fp16, 2.3e-3 in bf16.
+ * HKV_KERNEL_GENERIC keeps the probabilities in 32 bits. The same call gives the same bits. A key that a
+ * query does not attend never reaches its row, whatever its values; one it attends whose weight vanishes
+ * in 32 bits adds nothing if its values are finite. */
 int hkv_paged_attention(hkv_paged_ctx* ctx, const void* q, int64_t q_token_stride, const void* k_cache,
                         const void* v_cache, void* out, const int32_t* d_block_table, const int32_t* d_q_start,
                         const int32_t* d_step_len, const int32_t* d_total_len, int32_t requests, int32_t tokens,
